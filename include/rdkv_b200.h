@@ -607,6 +607,57 @@ int rdkv_knapsack_batched_static(const float* scores, int64_t row_stride, int n_
                                  const float* budget, const float* option_bits, const float* option_eps,
                                  int n_options, int max_iters, float tol, int64_t* out, void* stream);
 
+/* ── paged cache: uncompressed keys and values of running requests ────────────
+ * No counterpart in the reference.  Pages of page_size tokens, [n_pages][H_kv][page_size][128] in any strides
+ * (elements) whose rows are contiguous; a request's pages are listed in its row of block_tables. */
+
+/* Rotates q [n_tokens][H_q][128] and k [n_tokens][H_kv][128] (dtype: all of one type) by the tokens' positions
+ * on 1 to 4 axes into q_out / k_out (which may be q / k): axis a owns sections[a] (HOST array, sum 64) of the 64
+ * frequencies, angle = positions[a*axis_stride + t] * inv_freq[j] (int32, or int64 with positions_64; taken in 64 bits). */
+int rdkv_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out, int64_t q_out_tok_stride,
+                   int64_t q_out_head_stride, int H_q, const void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                   void* k_out, int64_t k_out_tok_stride, int64_t k_out_head_stride, int H_kv, int dtype, int n_tokens,
+                   const void* positions, int64_t axis_stride, int positions_64, const float* inv_freq,
+                   const int* sections, int n_axes, void* stream);
+
+/* Block tables and slot maps of a step: request i holds ctx_lens[i] tokens in its first ceil(ctx/page_size) pages and gets
+ * new_lens[i] more.  The pages it lacks are taken from free_pages [n_free], in request order from entry *free_start
+ * (NULL: 0) on, and written to its row of block_tables (-1 where the list is used up; entries behind the row's width
+ * are left out); the other entries stay as they were.  Out: slot_map / positions [n_tokens] (padding: -1 / 0), q_start
+ * [n_requests+1], kv_lens [n_requests] = ctx + new, free_next [1] (not free_start's address), missing [1] pages that could
+ * not be had.  n_requests up to 16384. */
+int rdkv_paged_tables(const int32_t* ctx_lens, const int32_t* new_lens, int n_requests, int32_t* block_tables,
+                      int64_t table_stride, int width, const int32_t* free_pages, int n_free, const int32_t* free_start,
+                      int page_size, int64_t n_tokens, int64_t* slot_map, int32_t* positions, int32_t* q_start,
+                      int32_t* kv_lens, int32_t* free_next, int32_t* missing, void* stream);
+
+/* Writes k / v [n_tokens][H_kv][128] to the slots of slot_map (outside [0, n_pages*page_size): not written).  n_axes > 0:
+ * the keys, and q into q_out (H_q > 0), are rotated as by rdkv_rope_axes. */
+int rdkv_paged_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
+                      int64_t v_head_stride, int H_kv, int dtype, int n_tokens, void* k_pages, int64_t k_page_stride,
+                      int64_t k_page_head_stride, int64_t k_page_row_stride, void* v_pages, int64_t v_page_stride,
+                      int64_t v_page_head_stride, int64_t v_page_row_stride, int n_pages, int page_size,
+                      const int64_t* slot_map, const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                      int64_t q_out_tok_stride, int64_t q_out_head_stride, int H_q, const void* positions,
+                      int64_t axis_stride, int positions_64, const float* inv_freq, const int* sections, int n_axes,
+                      void* stream);
+
+/* Attention of the new tokens of n_requests requests over their pages (fp16 / bf16; page_size a power of two, 16 to 1024;
+ * up to 16 query heads a KV head; bases on 16 bytes, strides of whole 16 bytes).  Query row q_start[i]+j is request i's
+ * token kv_lens[i]-n_i+j (n_i = q_start[i+1]-q_start[i], of which the first max_new are answered); it sees the tokens up to
+ * itself, under window > 0 only the last `window` of them and the first `sinks`, and none whose page number is
+ * outside [0, n_pages).  Either out [n_tokens][H_q][128] (rows behind q_start[n_requests]: zeroed with zero_padding, else left)
+ * or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace: rdkv_paged_attention_workspace() bytes (16-byte
+ * aligned; of one call at a time), contents arbitrary. */
+int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, int H_q, int H_kv, int max_new);
+int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype, int n_tokens, int H_q,
+                         const void* k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
+                         const void* v_pages, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
+                         int n_pages, int H_kv, int page_size, const int32_t* block_tables, int64_t table_stride,
+                         int width, const int32_t* q_start, const int32_t* kv_lens, int n_requests, int max_new,
+                         int window, int sinks, float scale, void* out, int64_t out_tok_stride, int64_t out_head_stride,
+                         int zero_padding, float* out_partial, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

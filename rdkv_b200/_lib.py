@@ -125,6 +125,13 @@ _PROTOTYPES = {
     "rdkv_decode_attn": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_decode_attn_tail": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_rope": ([_p, _i, _i, _i64, _p, _i, _i, _i64, _p, _p, _i, _p], _i),
+    "rdkv_rope_axes": ([_p, _i64, _i64, _p, _i64, _i64, _i, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _p, _i64, _i, _p, _p, _i, _p], _i),
+    "rdkv_paged_tables": ([_p, _p, _i, _p, _i64, _i, _p, _i, _p, _i, _i64, _p, _p, _p, _p, _p, _p, _p], _i),
+    "rdkv_paged_append": ([_p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _p,
+                           _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i64, _i, _p, _p, _i, _p], _i),
+    "rdkv_paged_attention_workspace": ([_i, _i, _i, _i, _i], _i64),
+    "rdkv_paged_attention": ([_p, _i64, _i64, _i, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _p, _i64, _i,
+                              _p, _p, _i, _i, _i, _i, _f, _p, _i64, _i64, _i, _p, _p, _i64, _p], _i),
     "rdkv_decode_attn_persistent": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_tail_attn_partial": ([_p, _i, _i64, _i, _i, _p, _p, _i, _i64, _i64, _i64, _i, _p, _i, _p, _p], _i),
     "rdkv_lse_combine": ([_p, _i64, _i, _i64, _i64, _p, _p, _p, _p], _i),

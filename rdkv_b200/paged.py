@@ -1,0 +1,241 @@
+"""The paged cache: uncompressed keys and values of running requests, before (or beside) their packed form.
+
+Keys and values live in pages of ``page_size`` tokens, ``k_pages`` / ``v_pages`` ``[n_pages,H_kv,page_size,128]``
+(any strides whose rows are contiguous), and a request owns the pages its row of ``block_tables`` lists.  A step of a
+batch whose requests have ``ctx_lens`` tokens in the cache and ``new_lens`` new ones is
+
+    plan = build_block_tables(ctx_lens, new_lens, block_tables, free_pages, page_size, n_tokens)   # once
+    q = append_kv(k, v, k_pages, v_pages, plan.slot_map, q=q, positions=plan.positions,            # in every layer
+                  inv_freq=inv_freq)
+    out = paged_attention(q, k_pages, v_pages, block_tables, plan.q_start, plan.kv_lens, max_new=...)
+
+for chunks of a prompt, single decoded tokens and both at once.  All lengths are read on the device: nothing
+here waits for the GPU, and a captured step can be replayed with other lengths.  The pages of a prompt that is complete
+are what :mod:`rdkv_b200.packing` compresses, and :func:`paged_attention` can leave records that
+:func:`rdkv_b200.decode.lse_combine` merges with those of packed layers.
+
+Every call launches on the current stream of its tensors' device.  A call's scratch memory is its own (allocated by
+the call), so calls on different streams and captured graphs do not share any.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+from torch import Tensor
+
+from ._lib import HEAD_DIM, PARTIAL_STRIDE, check, lib, q_dtype_tag, require_cuda, stream_ptr
+from .rope import _axes_args
+
+MAX_REQUESTS = 16384
+
+
+class PagedPlan(NamedTuple):
+    """What :func:`build_block_tables` worked out for a step."""
+    slot_map: Tensor      # int64 [n_tokens]  slot (page * page_size + row) of every new token, -1: none
+    positions: Tensor     # int32 [n_tokens]  its position in its request (padding: 0)
+    q_start: Tensor       # int32 [S+1]       first new token of every request
+    kv_lens: Tensor       # int32 [S]         tokens of every request, the new ones included
+    free_next: Tensor     # int32 [1]         first entry of the free list that is still free
+    missing: Tensor       # int32 [1]         pages that could not be had
+
+
+def _int32(t: Tensor, name: str, dim: int) -> None:
+    require_cuda(t, name)
+    if t.dtype != torch.int32 or t.dim() != dim or (t.dim() > 0 and t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be an int32 tensor of {dim} dimension(s) with contiguous rows")
+
+
+def _same_device(dev, **tensors: Optional[Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must live on {dev}, got {t.device}")
+
+
+def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor, free_pages: Tensor, page_size: int, n_tokens: int,
+                       *, free_start: Optional[Tensor] = None, out: Optional[PagedPlan] = None) -> PagedPlan:
+    """Gives the requests of a step the pages they lack and every new token its slot; one launch.
+
+    ctx_lens, new_lens int32 [S] (S up to 16384; negative counts as zero): tokens in the cache, new tokens.
+    block_tables int32 [S,width]: the pages a request holds (``ceil(ctx/page_size)`` entries) are read, those of its new
+    pages are written IN PLACE, everything behind them is left as it was.  free_pages int32 [F]: page numbers to hand
+    out, in request order, from entry ``free_start`` (int32 [1], default 0) on; the caller goes on at ``free_next`` (a
+    tensor of its own: ``free_start`` is not changed).  n_tokens: length of the step's token buffers; tokens behind
+    the last request's are padding (slot -1, position 0).
+
+    A page that is not to be had (the free list is used up: entry -1; the table is too narrow: no entry) leaves its
+    tokens without a slot (-1): :func:`append_kv` does not write them and :func:`paged_attention` does not see them.
+    ``missing`` counts such pages.  ``out``: a plan of the same S and n_tokens to write into (for captured steps)."""
+    _int32(ctx_lens, "ctx_lens", 1); _int32(new_lens, "new_lens", 1); _int32(block_tables, "block_tables", 2)
+    _int32(free_pages, "free_pages", 1)
+    S, T, dev = ctx_lens.shape[0], int(n_tokens), ctx_lens.device
+    if new_lens.shape[0] != S or block_tables.shape[0] != S:
+        raise ValueError(f"new_lens and block_tables must have {S} rows, got {new_lens.shape[0]} and {block_tables.shape[0]}")
+    if S > MAX_REQUESTS:
+        raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
+    if page_size < 1 or T < 0:
+        raise ValueError(f"bad page_size {page_size} or n_tokens {n_tokens}")
+    if S > 1 and block_tables.shape[1] > 0 and block_tables.stride(0) < block_tables.shape[1]:
+        raise ValueError("rows of block_tables overlap")
+    if free_start is not None:
+        _int32(free_start, "free_start", 1)
+        if free_start.shape[0] != 1:
+            raise ValueError("free_start must have one element")
+    _same_device(dev, new_lens=new_lens, block_tables=block_tables, free_pages=free_pages, free_start=free_start)
+    if out is None:
+        ints = torch.empty(T + 2 * S + 3, dtype=torch.int32, device=dev)
+        positions, q_start, kv_lens, free_next, missing = ints.split((T, S + 1, S, 1, 1))
+        out = PagedPlan(torch.empty(T, dtype=torch.int64, device=dev), positions, q_start, kv_lens, free_next, missing)
+    else:
+        for name, n in (("positions", T), ("q_start", S + 1), ("kv_lens", S), ("free_next", 1), ("missing", 1)):
+            t = getattr(out, name)
+            _int32(t, f"out.{name}", 1)
+            if t.shape[0] != n:
+                raise ValueError(f"out.{name} must have {n} elements")
+        if out.slot_map.dtype != torch.int64 or tuple(out.slot_map.shape) != (T,) or not out.slot_map.is_contiguous():
+            raise ValueError(f"out.slot_map must be a contiguous int64 tensor of {T} elements")
+        _same_device(dev, **{f"out.{n}": t for n, t in out._asdict().items()})
+        if free_start is not None and out.free_next.data_ptr() == free_start.data_ptr():
+            raise ValueError("out.free_next must not be free_start itself (other blocks of the launch still read it)")
+    check(lib().rdkv_paged_tables(
+        ctx_lens.data_ptr(), new_lens.data_ptr(), S, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+        free_pages.data_ptr(), free_pages.shape[0], None if free_start is None else free_start.data_ptr(), int(page_size), T,
+        out.slot_map.data_ptr(), out.positions.data_ptr(), out.q_start.data_ptr(), out.kv_lens.data_ptr(), out.free_next.data_ptr(),
+        out.missing.data_ptr(), stream_ptr(dev)), "rdkv_paged_tables")
+    return out
+
+
+def _check_pages(k_pages: Tensor, v_pages: Tensor) -> None:
+    require_cuda(k_pages, "k_pages"); require_cuda(v_pages, "v_pages")
+    if k_pages.dim() != 4 or k_pages.shape[3] != HEAD_DIM or k_pages.shape != v_pages.shape:
+        raise ValueError(f"k_pages and v_pages must be [n_pages,H_kv,page_size,{HEAD_DIM}], got {tuple(k_pages.shape)} and "
+                         f"{tuple(v_pages.shape)}")
+    if k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must have one dtype")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError("rows of k_pages and v_pages must be contiguous")
+
+
+def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: Tensor, *, q: Optional[Tensor] = None,
+              positions: Optional[Tensor] = None, inv_freq: Optional[Tensor] = None, sections: Optional[Sequence[int]] = None,
+              q_out: Optional[Tensor] = None) -> Optional[Tensor]:
+    """Writes the new tokens' keys and values to their slots; with ``positions`` the keys, and the queries
+    ``q``, are rotated on the way (as :func:`rdkv_b200.rope.rope_axes` does).  One launch.
+
+    k, v [T,H_kv,128]; k_pages, v_pages [n_pages,H_kv,page_size,128] of the same dtype (fp16 / bf16 / fp32); slot_map int64
+    [T]: slot of every token; a slot below zero or behind the last page is not written.  The slots of a call must
+    differ from one another.  q [T,H_q,128] of the same dtype goes to ``q_out`` (default: a new tensor; may be q
+    itself), which is returned; k is not changed.  positions [T] or [axes,T], inv_freq and sections: see ``rope_axes``."""
+    require_cuda(k, "k"); require_cuda(v, "v"); require_cuda(slot_map, "slot_map")
+    _check_pages(k_pages, v_pages)
+    n_pages, H_kv, page_size, _ = k_pages.shape
+    T, dev = k.shape[0], k.device
+    if k.dim() != 3 or tuple(k.shape) != (T, H_kv, HEAD_DIM) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [T,{H_kv},{HEAD_DIM}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
+        raise ValueError(f"k and v must have the pages' dtype {k_pages.dtype}")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("rows of k and v must be contiguous")
+    if slot_map.dtype != torch.int64 or tuple(slot_map.shape) != (T,) or (T > 1 and slot_map.stride(0) != 1):
+        raise ValueError(f"slot_map must be a contiguous int64 tensor of {T} elements")
+    tag = q_dtype_tag(k)
+    if (positions is None) != (inv_freq is None) or (positions is None and (q is not None or sections is not None)):
+        raise ValueError("q and sections need positions and inv_freq; positions needs inv_freq")
+    if positions is None:
+        rot = (None, 0, 0, None, None, 0)
+    else:
+        rot = _axes_args(positions, inv_freq, sections, T, dev)
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out needs q")
+        q_args = (None, 0, 0, None, 0, 0, 0)
+    else:
+        require_cuda(q, "q")
+        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != HEAD_DIM or q.dtype != k.dtype or q.stride(2) != 1:
+            raise ValueError(f"q must be [{T},H_q,{HEAD_DIM}] {k.dtype} with contiguous rows, got {tuple(q.shape)} {q.dtype}")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
+            raise ValueError("q_out must have q's shape and dtype and contiguous rows")
+        q_args = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1])
+    _same_device(dev, v=v, k_pages=k_pages, v_pages=v_pages, slot_map=slot_map, q=q, q_out=q_out)
+    ks, vs = k_pages.stride(), v_pages.stride()
+    check(lib().rdkv_paged_append(
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), H_kv, tag, T, k_pages.data_ptr(), ks[0], ks[1],
+        ks[2], v_pages.data_ptr(), vs[0], vs[1], vs[2], n_pages, page_size, slot_map.data_ptr(), *q_args, *rot, stream_ptr(dev)),
+        "rdkv_paged_append")
+    return q_out
+
+
+def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: Tensor, q_start: Tensor, kv_lens: Tensor, *,
+                    max_new: Optional[int] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
+                    out: Optional[Tensor] = None, out_partial: Optional[Tensor] = None) -> Tensor:
+    """Attention of a batch's new tokens over the pages of their requests.
+
+    q [T,H_q,128] (fp16 / bf16, the pages' dtype, after rotation); k_pages, v_pages [n_pages,H_kv,page_size,128] with
+    page_size a power of two from 16 to 1024 and up to 16 query heads a KV head; block_tables int32 [S,width], q_start
+    int32 [S+1], kv_lens int32 [S] (as :func:`build_block_tables` leaves them).  The last ``q_start[i+1]-q_start[i]`` of
+    request i's ``kv_lens[i]`` tokens are the new ones, whose keys and values are in the pages already.  A token
+    sees its request's tokens up to itself; with ``window`` > 0 only the last ``window`` of them (itself included)
+    and the request's first ``sinks``.  Tokens whose page is missing (an entry outside the pages) are not seen, and what
+    stands in masked places does not matter, whatever it is.  A token that sees nothing gets zeros.
+
+    max_new: the longest chunk of the batch, or a bound of it (default T); requests with more new tokens than that
+    get no result for the rest.  scale: of the scores, default 1/sqrt(128).
+    Returns ``out`` [T,H_q,128] in q's dtype.  Tokens behind the last request's are padding: zero in an ``out`` that the
+    call allocates, left as they were in one that it is given.  ``out_partial`` float32 [T*H_q,132] receives
+    un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
+    require_cuda(q, "q")
+    _check_pages(k_pages, v_pages)
+    n_pages, H_kv, page_size, _ = k_pages.shape
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM:
+        raise ValueError(f"q must be [T,H_q,{HEAD_DIM}], got {tuple(q.shape)}")
+    T, H_q, _ = q.shape
+    dev = q.device
+    if q.dtype != k_pages.dtype or q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"q and the pages must both be fp16 or both bf16, got {q.dtype} and {k_pages.dtype}")
+    if H_kv < 1 or H_q % H_kv or not 1 <= H_q // H_kv <= 16:
+        raise ValueError(f"{H_q} query heads over {H_kv} KV heads: 1 to 16 each are supported")
+    if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+    _int32(block_tables, "block_tables", 2); _int32(q_start, "q_start", 1); _int32(kv_lens, "kv_lens", 1)
+    S = kv_lens.shape[0]
+    if block_tables.shape[0] != S or q_start.shape[0] != S + 1:
+        raise ValueError(f"block_tables must have {S} rows and q_start {S + 1} elements")
+    if S > MAX_REQUESTS:
+        raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
+    if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
+        raise ValueError("window and sinks must not be negative, and sinks need a window")
+    max_new = T if max_new is None else min(int(max_new), T)
+    if max_new < 0:
+        raise ValueError("max_new must not be negative")
+    if q.stride(2) != 1 or q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+        q = q.clone(memory_format=torch.contiguous_format)
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16 or any(x % 8 for x in ks[:3] + vs[:3]):
+        raise ValueError("k_pages and v_pages must start on 16 bytes and have strides of whole 16 bytes")
+    allocated = False
+    if out_partial is not None:
+        if out is not None:
+            raise ValueError("either out or out_partial")
+        require_cuda(out_partial, "out_partial")
+        if out_partial.dtype != torch.float32 or not out_partial.is_contiguous() or out_partial.numel() != T * H_q * PARTIAL_STRIDE:
+            raise ValueError(f"out_partial must be contiguous float32 [{T * H_q},{PARTIAL_STRIDE}]")
+        o_args = (None, 0, 0, 0, out_partial.data_ptr())
+    else:
+        if out is None:
+            out, allocated = torch.empty((T, H_q, HEAD_DIM), dtype=q.dtype, device=dev), True
+        require_cuda(out, "out")
+        if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8:
+            raise ValueError(f"out must be {q.dtype} [{T},{H_q},{HEAD_DIM}] with contiguous rows on 16 bytes")
+        o_args = (out.data_ptr(), out.stride(0), out.stride(1), 1 if allocated else 0, None)
+    _same_device(dev, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, q_start=q_start, kv_lens=kv_lens, out=out,
+                 out_partial=out_partial)
+    n_ws = lib().rdkv_paged_attention_workspace(S, T, H_q, H_kv, max_new)
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws > 0 else None
+    check(lib().rdkv_paged_attention(
+        q.data_ptr(), q.stride(0), q.stride(1), q_dtype_tag(q), T, H_q, k_pages.data_ptr(), ks[0], ks[1], ks[2], v_pages.data_ptr(), vs[0],
+        vs[1], vs[2], n_pages, H_kv, page_size, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+        q_start.data_ptr(), kv_lens.data_ptr(), S, max_new, int(window), int(sinks), HEAD_DIM ** -0.5 if scale is None else float(scale),
+        *o_args, None if ws is None else ws.data_ptr(), n_ws, stream_ptr(dev)), "rdkv_paged_attention")
+    return out if out_partial is None else out_partial

@@ -3,10 +3,15 @@
 Drop-in for the reference's ``fused_rope`` (obkv_accel/triton_rope.py:111-138): same name,
 arguments and in-place behaviour.  Inside a decode step the rotation is part of the attention
 launch (:func:`rdkv_b200.decode.packed_decode_attention` with ``rope=``); this call is for
-callers that keep the two steps apart.
+callers that keep the two steps apart.  :func:`rope_axes` rotates the rows of many tokens, each by
+its own position on one to four axes.
 """
 from __future__ import annotations
 
+import ctypes as C
+from typing import Optional, Sequence
+
+import torch
 from torch import Tensor
 
 from ._lib import HEAD_DIM, check, lib, ptr, q_dtype_tag, require_cuda, stream_ptr
@@ -29,3 +34,67 @@ def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
                           k.stride(0), ptr(cos_half), ptr(sin_half), q_dtype_tag(cos_half), stream_ptr(q.device)),
           "rdkv_rope")
     return q, k
+
+
+_SECTIONS = {}                                             # section sizes -> the C array handed to the library
+
+
+def _axes_args(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[int]], T: int, dev):
+    """(positions, axis stride, 64 bits?, inv_freq, sections, axes) of a call, as the library takes them."""
+    half = HEAD_DIM // 2
+    require_cuda(positions, "positions"); require_cuda(inv_freq, "inv_freq")
+    n_axes = 1 if positions.dim() == 1 else positions.shape[0]
+    if positions.dim() not in (1, 2) or positions.shape[-1] != T or not 1 <= n_axes <= 4 or (T > 1 and positions.stride(-1) != 1):
+        raise ValueError(f"positions must be [{T}] or [1 to 4 axes,{T}] with contiguous rows, got {tuple(positions.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (half,) or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be a contiguous float32 tensor of {half} elements")
+    if positions.device != dev or inv_freq.device != dev:
+        raise ValueError(f"positions and inv_freq must live on {dev}")
+    if sections is None:
+        if n_axes != 1:
+            raise ValueError("positions of several axes need sections")
+        sections = (half,)
+    sections = tuple(sections)
+    sec = _SECTIONS.get(sections)
+    if sec is None:
+        if any(int(n) != n or n < 0 for n in sections) or sum(sections) != half:
+            raise ValueError(f"sections must be whole numbers that add up to {half}, got {sections}")
+        if len(_SECTIONS) >= 64:
+            _SECTIONS.clear()
+        sec = _SECTIONS[sections] = (C.c_int * len(sections))(*(int(n) for n in sections))
+    if len(sections) != n_axes:
+        raise ValueError(f"{len(sections)} sections for {n_axes} axes")
+    return (positions.data_ptr(), 0 if n_axes == 1 else positions.stride(0), 1 if positions.dtype == torch.int64 else 0,
+            inv_freq.data_ptr(), sec, n_axes)
+
+
+def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sections: Optional[Sequence[int]] = None,
+              q_out: Optional[Tensor] = None, k_out: Optional[Tensor] = None):
+    """Rotate q [T,H_q,128] and k [T,H_kv,128] (both fp16, bf16 or fp32) by the tokens' positions, half format as
+    :func:`fused_rope`.  One launch.
+
+    positions [T], or [axes,T] with 1 to 4 axes (time, height, width of images and video), int32 / int64; inv_freq
+    float32 [64]: the angle of frequency j is ``position * inv_freq[j]``, taken in 64 bits so that far positions
+    lose nothing (below 2^24).  sections: how many of the 64 frequencies each axis owns, in order (text
+    with one axis: all of them).  Returns (q_out, k_out): new tensors, or the given ones, which may be q and k
+    themselves."""
+    for name, t in (("q", q), ("k", k)):
+        require_cuda(t, name)
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
+            raise ValueError(f"{name} must be [T,heads,{HEAD_DIM}] with contiguous rows, got {tuple(t.shape)}")
+    T, dev = q.shape[0], q.device
+    if k.shape[0] != T or k.dtype != q.dtype or k.device != dev:
+        raise ValueError("q and k must have the same tokens, dtype and device")
+    tag = q_dtype_tag(q)
+    rot = _axes_args(positions, inv_freq, sections, T, dev)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if k_out is None else k_out
+    for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != dev or t.stride(2) != 1:
+            raise ValueError(f"{name} must have the shape, dtype and device of its input and contiguous rows")
+    check(lib().rdkv_rope_axes(q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1],
+                               k.data_ptr(), k.stride(0), k.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1), k.shape[1],
+                               tag, T, *rot, stream_ptr(dev)), "rdkv_rope_axes")
+    return q_out, k_out

@@ -1,84 +1,346 @@
-// Attention of the new tokens of a batch of requests over their paged keys and values.
+// Entry point of the attention over paged caches, and its kernel for few rows a KV head (single tokens).
 //
-// Request i's cache holds kv_len_i tokens, the last n_i = q_start[i+1] - q_start[i] of them new ones: query row j of
-// the request stands at position p = kv_len_i - n_i + j and sees key s if s <= p, and, under a window of w tokens,
-// s > p - w or s < sinks, and if the page of s is there (a page number outside the pages stands for none):
-//   o = sum_s softmax_s(scale * q.k_s) v_s;  a row that sees nothing is zero (record: m = -inf, l = 0).
-#include <algorithm>
-
-#include "rdkv_common.cuh"
+// paged_decode_kernel: an item is up to 16 rows (new tokens x query heads of a KV head), which is the M of mma.sync
+// m16n8k16; its keys and values are read once and are all the kernel moves, so it is bound by memory.  A CTA has four
+// computing warps and one that brings in tiles of 64 keys: one tiled TMA box per page (or per 64 rows of a larger one),
+// 64-channel panel and tensor, laid down with the 128-byte swizzle that ldmatrix reads without bank conflicts, three
+// tiles deep, two CTAs an SM.  Page numbers are fetched 32 boxes ahead.  Each computing warp takes 16 keys of a
+// tile on its own: scores (queries as A operand, keys as B), running maximum and sum, then the weights, which are
+// already in A operand form, times the values (ldmatrix.trans).  The four partial results meet in the slot of the
+// segment's last tile.  Why not tcgen05: its smallest M is 64 rows, of which 4 to 16 would be used, and scores would
+// have to go through tensor memory and shared memory between the products; the tensor pipe is idle most of the time as it is.
+//
+// Masks are applied only to 16-key blocks that reach past some row's limits.  There, values of keys that no row of
+// the item sees are set to zero (0 x NaN), and a value that is not finite at a key that only some rows see makes the
+// segment's rows be done again, one by one (paged_slow_row).
+#include "paged_attn.cuh"
 
 namespace rdkv {
 
-struct PagedArgs {
-  const uint16_t* q; const uint16_t* k; const uint16_t* v;
-  int64_t q_tok, q_head;                          // elements
-  int64_t k_page, k_head, k_row, v_page, v_head, v_row;
-  int n_pages, page, page_log2, H_q, H_kv, g;
-  const int32_t* table; int64_t table_stride; int width;
-  const int32_t* q_start; const int32_t* kv_lens; int S, T;
-  int window, sinks;                              // window 0: everything
-  float scale;
-  uint16_t* out; int64_t o_tok, o_head; int zero_pad;
-  float* rec;                                     // [T][H_q][132] instead of out
-};
+constexpr int DEC_KEYS = PAGED_DECODE_KEYS, DEC_ROWS = PAGED_DECODE_ROWS, DEC_STAGES = 3;
+constexpr int DEC_WARPS = 4, DEC_THREADS = DEC_WARPS * 32 + 32;
+constexpr int DEC_PANEL = DEC_KEYS * 128;         // bytes of 64 keys' 64 channels
+constexpr int DEC_STAGE = 4 * DEC_PANEL;          // K channels 0-63, 64-127, V channels 0-63, 64-127
+constexpr size_t DEC_SMEM = 1024 + (size_t)DEC_STAGES * DEC_STAGE;
+static_assert(DEC_STAGE == DEC_WARPS * DEC_ROWS * 128 * 4, "the warps' results fill a stage");
+constexpr int DEC_FIXED = 2, DEC_SNAP = 1;
 
 template <bool BF16>
-__device__ __forceinline__ float paged_up(uint16_t x) { return BF16 ? __uint_as_float((uint32_t)x << 16) : h2f(x); }
+__device__ __forceinline__ void dec_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void dec_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void dec_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void dec_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // the computing warps
+__device__ __forceinline__ bool dec_barrier_any(bool x) {                                            // and whether one of their threads has x
+  uint32_t any;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"((uint32_t)x) : "memory");
+  return any != 0;
+}
+// Whether one of the two 16-bit values that `which` selects is not finite.
 template <bool BF16>
-__device__ __forceinline__ uint16_t paged_down(float x) {
-  return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+__device__ __forceinline__ bool dec_not_finite(uint32_t v, uint32_t which) {
+  constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
+  const uint32_t x = v & which;
+  return (x & E) == E || ((x >> 16) & E) == E;
 }
 
-// One warp per (token, query head), four channels a lane, one key after the other.
 template <bool BF16>
-__global__ void __launch_bounds__(128)
-paged_attn_plain_kernel(const PagedArgs A) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)A.T * A.H_q) return;
-  const int t = (int)(row / A.H_q), hq = (int)(row - (int64_t)t * A.H_q), h = hq / A.g;
-  int lo = 0, hi = A.S;                                      // requests whose first token is at or before t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (A.q_start[mid + 1] <= t) lo = mid + 1; else hi = mid;
-  }
-  uint16_t* o16 = A.out + (int64_t)t * A.o_tok + (int64_t)hq * A.o_head + 4 * lane;
-  float* rec = A.rec + row * RDKV_PARTIAL_STRIDE;
-  if (lo >= A.S || A.q_start[lo] > t) {
-    if (A.rec == nullptr && A.zero_pad) *reinterpret_cast<uint2*>(o16) = make_uint2(0u, 0u);
-    return;
-  }
-  const int64_t len = min((int64_t)A.kv_lens[lo], (int64_t)A.width << A.page_log2);
-  const int64_t pos = (int64_t)A.kv_lens[lo] - (A.q_start[lo + 1] - t);
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+__global__ void __launch_bounds__(DEC_THREADS, 2)
+paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ unsigned char dec_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2 * DEC_STAGES];   // [slot] tile arrived, [DEC_STAGES + slot] slot free
+  __shared__ int2 s_info[DEC_STAGES];                       // first key of the tile, a bit per 16 keys whose page is there
+  __shared__ float2 s_ml[DEC_WARPS][DEC_ROWS];
+  __shared__ int s_again[2];                                // segment (its number + 1) whose rows are done again
+  __shared__ int s_trouble;
+  __shared__ PagedPlaceScratch s_place;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+  const uint32_t ring = (smem_addr(dec_raw) + 1023u) & ~1023u, bar = smem_addr(s_bar);
+  unsigned char* ring_ptr = dec_raw + (ring - smem_addr(dec_raw));
+  if (tid == 0) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) q[e] = paged_up<BF16>(A.q[(int64_t)t * A.q_tok + (int64_t)hq * A.q_head + 4 * lane + e]) * A.scale;
-  for (int64_t s = 0; s < len && s <= pos; ++s) {
-    if (A.window > 0 && s <= pos - A.window && s >= A.sinks) { s = max((int64_t)A.sinks - 1, pos - A.window); continue; }
-    const int id = A.table[lo * A.table_stride + (s >> A.page_log2)];
-    if (id < 0 || id >= A.n_pages) continue;
-    const int64_t r = s & (A.page - 1);
-    const uint16_t* kp = A.k + id * A.k_page + h * A.k_head + r * A.k_row + 4 * lane;
-    const uint16_t* vp = A.v + id * A.v_page + h * A.v_head + r * A.v_row + 4 * lane;
-    float x = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x = fmaf(q[e], paged_up<BF16>(kp[e]), x);
-    x = warp_sum(x);
-    x = __shfl_sync(0xffffffffu, x, 0);
-    const float n = fmaxf(m, x), a = m == -INFINITY ? 0.f : __expf(m - n), p = __expf(x - n);
-    l = fmaf(l, a, p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], a, p * paged_up<BF16>(vp[e]));
-    m = n;
+    for (int i = 0; i < DEC_STAGES; ++i) { bar_init(bar + 8 * i, 1); bar_init(bar + 8 * (DEC_STAGES + i), DEC_WARPS); }
+    bar_init_fence();
+    s_again[0] = s_again[1] = s_trouble = 0;
   }
-  if (A.rec != nullptr) {
-    *reinterpret_cast<float4*>(rec + 4 + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
-    if (lane == 0) { rec[0] = m; rec[1] = l; rec[2] = 0.f; rec[3] = 0.f; }
+  let_next_kernel_start();
+  paged_zero_padding(A, DEC_THREADS);
+  PagedPlace from, to;
+  paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP>(A, cta, PAGED_DECODE_CTAS, s_place, from, to);   // (its barriers order the set-up too)
+  PagedWalk<DEC_KEYS> walk(A, from, to);
+  PagedSegment s;
+
+  if (warp == DEC_WARPS) {
+    // ── the warp that brings in tiles ──
+    const int rows = min(A.page, DEC_KEYS), per_tile = DEC_KEYS / rows, batch = 32 / per_tile;   // boxes of a tile, tiles of a batch of page numbers
+    const int box = lane >> 2, what = lane & 3;              // this lane's box of a tile: sub-tile, (K | V) x panel
+    unsigned count = 0;
+    bool ok = true;
+    while (ok && walk.next(A, s)) {
+      const int32_t* table = A.table + s.i * A.table_stride;
+      auto page_of = [&](int k) {                            // lane's entry of the batch that starts with tile k
+        const int kk = k + lane / per_tile;
+        if (kk >= s.k1) return -1;
+        const int key = paged_tile(s.item, kk) * DEC_KEYS + (lane % per_tile) * rows;
+        return key < s.item.hi ? table[key >> A.page_log2] : -1;
+      };
+      int ids = page_of(s.k0), ids_next = -1;
+      for (int k = s.k0; k < s.k1; ++k, ++count) {
+        const int in_batch = (k - s.k0) % batch;
+        if (in_batch == 0) {
+          if (k > s.k0) ids = ids_next;
+          ids_next = page_of(k + batch);
+        }
+        const int slot = count % DEC_STAGES;
+        if (count >= DEC_STAGES && !bar_wait(bar + 8 * (DEC_STAGES + slot), (count / DEC_STAGES - 1) & 1)) { ok = false; break; }
+        const int key0 = paged_tile(s.item, k) * DEC_KEYS;
+        const int id = __shfl_sync(0xffffffffu, ids, in_batch * per_tile + (box < per_tile ? box : 0));
+        const bool there = box < per_tile && id >= 0 && id < A.n_pages;
+        const unsigned lanes = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) {
+          int mask = 0;
+          for (int b = 0; b < per_tile; ++b)
+            if (lanes >> (4 * b) & 1) mask |= ((1 << (rows / 16)) - 1) << (b * (rows / 16));
+          s_info[slot] = make_int2(key0, mask);
+          const uint32_t bytes = (uint32_t)__popc(lanes) * (uint32_t)rows * 128u;
+          if (bytes > 0) bar_arrive_tx(bar + 8 * slot, bytes);
+          else bar_arrive(bar + 8 * slot);
+        }
+        __syncwarp();
+        if (there)
+          tma_load_4d(ring + slot * DEC_STAGE + what * DEC_PANEL + box * rows * 128, what < 2 ? &tm_k : &tm_v, (what & 1) * 64,
+                      key0 & (A.page - 1), s.head, id, bar + 8 * slot);
+      }
+    }
+    if (!ok) {                                               // wait (again bounded) for the copies in flight
+      s_trouble = 1;
+      for (unsigned n = count < DEC_STAGES ? 0 : count - DEC_STAGES; n < count; ++n) bar_wait(bar + 8 * (n % DEC_STAGES), (n / DEC_STAGES) & 1);
+    }
   } else {
+    // ── the computing warps ──
+    constexpr float RAISE = PagedWeights<BF16>::RAISE, LIFT = PagedWeights<BF16>::LIFT;
+    const int r0 = lane >> 2, c2 = (lane & 3) * 2;           // this thread's rows r0, r0 + 8; its pair of columns
+    unsigned count = 0, segment = 0;
+    bool ok = true;
+    while (ok && walk.next(A, s)) {
+      const int rows = s.item.n_tok * A.g, p_first = s.item.p0, p_last = s.item.p0 + s.item.n_tok - 1;
+      if (s.k0 == s.k1) {                                    // an item without keys
+        for (int x = tid; x < rows * 32; x += DEC_WARPS * 32) {
+          const PagedRow d = paged_row<DEC_ROWS>(A, s, x >> 5, cta);
+          if (d.rec != nullptr) {
+            *reinterpret_cast<float4*>(d.rec + 4 + 4 * (x & 31)) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if ((x & 31) == 0) *reinterpret_cast<float4*>(d.rec) = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+          } else {
+            *reinterpret_cast<uint2*>(d.out + 4 * (x & 31)) = make_uint2(0u, 0u);
+          }
+        }
+        continue;
+      }
+      // the query rows as A operand: channels 16 kk + c2, + 8 of rows r0, r0 + 8
+      uint32_t qa[8][4];
+      int pos[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o16[e] = paged_down<BF16>(l > 0.f || l != l ? o[e] / l : 0.f);
+      for (int e = 0; e < 2; ++e) {
+        const int row = r0 + 8 * e, tok = row / A.g;
+        pos[e] = row < rows ? s.item.p0 + tok : -1;
+        const uint16_t* src = A.q + (int64_t)(s.item.tok0 + tok) * A.q_tok + (int64_t)(s.head * A.g + row - tok * A.g) * A.q_head + c2;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qa[kk][e] = row < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * kk) : 0u;
+          qa[kk][2 + e] = row < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * kk + 8) : 0u;
+        }
+      }
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      float o[16][4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      bool again = false;
+      for (int k = s.k0; k < s.k1; ++k, ++count) {
+        const int slot = count % DEC_STAGES;
+        ok = ok && bar_wait(bar + 8 * slot, (count / DEC_STAGES) & 1);
+        if (!ok) break;
+        const int2 info = s_info[slot];
+        const int key0 = info.x + warp * 16;
+        if ((info.y >> warp & 1) != 0 && key0 < s.item.hi) {
+          const uint32_t kb = ring + slot * DEC_STAGE, vb = kb + 2 * DEC_PANEL;
+          // scores of 16 keys: two tiles of 8
+          float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          {
+            // matrices of an ldmatrix: keys 0-7 / 8-15 (lane bit 4), channels 0-7 / 8-15 of the step (lane bit 3)
+            const int row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), half = lane >> 3 & 1;
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              uint32_t b[4];
+              const int c16 = 2 * kk + half;
+              dec_ldmatrix(b, kb + (c16 >> 3) * DEC_PANEL + row * 128 + (((c16 & 7) ^ (row & 7)) << 4));
+              dec_mma<BF16>(sc[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[0], b[1]);
+              dec_mma<BF16>(sc[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2], b[3]);
+            }
+          }
+          const bool edge = key0 + 15 > p_first || key0 + 16 > s.item.hi ||
+                            (A.window > 0 && key0 <= p_last - A.window && key0 + 15 >= A.sinks);
+          uint32_t live0 = 0xFFFFFFFFu, live1 = 0xFFFFFFFFu, some0 = 0u, some1 = 0u;   // this thread's keys of the V operand
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] *= A.scale_log2;
+          if (edge) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              uint32_t live = 0xFFFFFFFFu, some = 0u;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 8 * n + c2 + e;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const bool hidden = key > pos[r] || key >= s.item.hi || (A.window > 0 && key <= pos[r] - A.window && key >= A.sinks);
+                  if (hidden) sc[n][2 * r + e] = -INFINITY;
+                }
+                const bool low = A.window > 0 && key >= A.sinks;
+                const bool none = key >= s.item.hi || (low && key <= p_first - A.window);       // no row sees the key
+                const bool not_all = key > p_first || (low && key <= p_last - A.window);
+                if (none) live &= e == 0 ? 0xFFFF0000u : 0x0000FFFFu;
+                else if (not_all) some |= e == 0 ? 0x0000FFFFu : 0xFFFF0000u;
+              }
+              if (n == 0) { live0 = live; some0 = some; } else { live1 = live; some1 = some; }
+            }
+          }
+          float top[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            top[r] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          }
+          if (__any_sync(0xffffffffu, top[0] > m[0] + RAISE || top[1] > m[1] + RAISE)) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float n = fmaxf(m[r], top[r]), f = n == -INFINITY ? 1.f : exp2_approx(m[r] - n);   // (m = -inf: 0)
+              m[r] = n; l[r] *= f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) { o[i][2 * r] *= f; o[i][2 * r + 1] *= f; }
+            }
+          }
+          uint32_t pa[4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float base = (m[r] == -INFINITY ? 0.f : m[r]) - LIFT;
+            float p[4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) p[2 * n + e] = exp2_approx(sc[n][2 * r + e] - base);
+            l[r] += (p[0] + p[1]) + (p[2] + p[3]);
+            pa[r] = paged_pack<BF16>(p[0], p[1]); pa[2 + r] = paged_pack<BF16>(p[2], p[3]);
+          }
+          // values: matrices of an ldmatrix: keys 0-7 / 8-15 (lane bit 3), channels 0-7 / 8-15 of the step (lane bit 4)
+          const int row = warp * 16 + (lane & 15), half = lane >> 4;
+#pragma unroll
+          for (int cc = 0; cc < 8; ++cc) {
+            uint32_t b[4];
+            const int c16 = 2 * cc + half;
+            dec_ldmatrix_t(b, vb + (c16 >> 3) * DEC_PANEL + row * 128 + (((c16 & 7) ^ (row & 7)) << 4));
+            if (edge) {
+              if ((some0 | some1) != 0u)
+                again |= dec_not_finite<BF16>(b[0], some0) || dec_not_finite<BF16>(b[1], some1) || dec_not_finite<BF16>(b[2], some0) ||
+                         dec_not_finite<BF16>(b[3], some1);
+              b[0] &= live0; b[1] &= live1; b[2] &= live0; b[3] &= live1;
+            }
+            dec_mma<BF16>(o[2 * cc], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+            dec_mma<BF16>(o[2 * cc + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+          }
+        }
+        if (k + 1 < s.k1) {                                  // (the last tile's slot is used below)
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar + 8 * (DEC_STAGES + slot));
+        }
+      }
+      // the four warps' results meet in the last tile's slot
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      }
+      if (again) s_again[segment & 1] = (int)segment + 1;
+      ok = !dec_barrier_any(!ok);                            // (all four warps go on, or none does)
+      if (!ok) s_trouble = 1;
+      const int slot = (count - 1) % DEC_STAGES;
+      float* buf = reinterpret_cast<float*>(ring_ptr + slot * DEC_STAGE);
+      if (ok) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = r0 + 8 * r;
+          if (row < rows) {
+            if ((lane & 3) == 0) s_ml[warp][row] = make_float2(m[r], l[r]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              *reinterpret_cast<float2*>(buf + ((warp * DEC_ROWS + row) * 128 + 8 * i + c2)) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+          }
+        }
+      }
+      dec_barrier();
+      if (ok) {
+        if (s_again[segment & 1] == (int)segment + 1) {
+          const PagedSegment copy = s;
+          for (int row = warp; row < rows; row += DEC_WARPS) paged_slow_row<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, cta);
+        } else {
+          for (int row = warp; row < rows; row += DEC_WARPS) {   // four channels a lane
+            float M = -INFINITY, L = 0.f;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < DEC_WARPS; ++w) M = fmaxf(M, s_ml[w][row].x);
+#pragma unroll
+            for (int w = 0; w < DEC_WARPS; ++w) {
+              const float2 ml = s_ml[w][row];
+              const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
+              const float4 x = *reinterpret_cast<const float4*>(buf + ((w * DEC_ROWS + row) * 128 + 4 * lane));
+              if (ml.x != -INFINITY || ml.y != 0.f) {        // (a warp that saw nothing of the row adds nothing)
+                L = fmaf(ml.y, f, L);
+                sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
+              }
+            }
+            const PagedRow d = paged_row<DEC_ROWS>(A, s, row, cta);
+            if (d.rec != nullptr) {
+              *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = sum;
+              if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4((M - LIFT) * PAGED_LN2, L, 0.f, 0.f);
+            } else {
+              const float w = paged_over(L);
+              *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(sum.x * w, sum.y * w), paged_pack<BF16>(sum.z * w, sum.w * w));
+            }
+          }
+        }
+        fence_async_smem();                                  // (the slot's next writer is a TMA copy)
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar + 8 * (DEC_STAGES + slot));
+      }
+      ++segment;
+    }
   }
+  __syncthreads();
+  if (tid == 0) A.status[cta] = s_trouble;
+}
+
+int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  auto go = [&](auto kernel, auto join) -> int {
+    const cudaError_t e = allow_dynamic_smem(kernel, DEC_SMEM);
+    if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
+    kernel<<<PAGED_DECODE_CTAS, DEC_THREADS, DEC_SMEM, st>>>(A, tm_k, tm_v);
+    const int rc = launch_status();
+    if (rc != RDKV_OK) return rc;
+    return paged_launch_join(join, A, dim3(PAGED_DECODE_CTAS - 1, DEC_ROWS / PAGED_JOIN_WARPS), st);
+  };
+  if (bf16) return go(paged_decode_kernel<true>, paged_join_kernel<true, DEC_KEYS, DEC_ROWS, PAGED_DECODE_CTAS>);
+  return go(paged_decode_kernel<false>, paged_join_kernel<false, DEC_KEYS, DEC_ROWS, PAGED_DECODE_CTAS>);
 }
 
 }  // namespace rdkv
@@ -87,7 +349,8 @@ using namespace rdkv;
 
 extern "C" int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, int H_q, int H_kv, int max_new) {
   if (n_requests < 0 || n_tokens < 0 || H_q <= 0 || H_kv <= 0 || max_new < 0) return -1;
-  return 0;
+  if (n_tokens == 0) return 0;
+  return paged_workspace_bytes(PAGED_DECODE_CTAS, PAGED_DECODE_ROWS);
 }
 
 extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype, int n_tokens, int H_q,
@@ -106,6 +369,9 @@ extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t
   if (q == nullptr || q_start == nullptr || (out == nullptr) == (out_partial == nullptr)) return RDKV_ERR_BAD_ARG;
   if (n_requests > 0 && (kv_lens == nullptr || (width > 0 && block_tables == nullptr))) return RDKV_ERR_BAD_ARG;
   if (n_pages > 0 && (k_pages == nullptr || v_pages == nullptr)) return RDKV_ERR_BAD_ARG;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+      workspace_bytes < rdkv_paged_attention_workspace(n_requests, n_tokens, H_q, H_kv, max_new))
+    return RDKV_ERR_BAD_ARG;
   PagedArgs A = {};
   A.q = (const uint16_t*)q; A.k = (const uint16_t*)k_pages; A.v = (const uint16_t*)v_pages;
   A.q_tok = q_tok_stride; A.q_head = q_head_stride;
@@ -113,12 +379,18 @@ extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t
   A.v_page = v_page_stride; A.v_head = v_head_stride; A.v_row = v_row_stride;
   A.n_pages = n_pages; A.page = page_size; A.H_q = H_q; A.H_kv = H_kv; A.g = H_q / H_kv;
   for (A.page_log2 = 0; (1 << A.page_log2) < page_size; ++A.page_log2) {}
-  A.table = block_tables; A.table_stride = table_stride; A.width = width; A.q_start = q_start; A.kv_lens = kv_lens;
-  A.S = n_requests; A.T = n_tokens; A.window = window; A.sinks = sinks; A.scale = scale;
+  A.table = block_tables; A.table_stride = table_stride; A.width = width;
+  A.cap = (int)std::min<int64_t>((int64_t)width * page_size, 0x7fff0000);
+  A.q_start = q_start; A.kv_lens = kv_lens; A.S = n_requests; A.T = n_tokens;
+  A.window = std::min(window, 1 << 30); A.sinks = std::min(sinks, 1 << 30); A.scale_log2 = scale * PAGED_LOG2E;
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
-  const int64_t blocks = ((int64_t)n_tokens * H_q + 3) / 4;
-  if (blocks > 0x7fffffffLL) return RDKV_ERR_TOO_LARGE;
-  if (dtype == RDKV_BF16) paged_attn_plain_kernel<true><<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(A);
-  else paged_attn_plain_kernel<false><<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(A);
-  return launch_status();
+  const bool bf = dtype == RDKV_BF16;
+  A.group = PAGED_DECODE_ROWS / A.g;
+  paged_workspace(&A, workspace, PAGED_DECODE_CTAS);
+  CUtensorMap tm_k, tm_v;
+  const int box = std::min(page_size, PAGED_DECODE_KEYS);
+  if (!paged_map(&tm_k, k_pages, bf, k_page_stride, k_head_stride, k_row_stride, n_pages, H_kv, page_size, box) ||
+      !paged_map(&tm_v, v_pages, bf, v_page_stride, v_head_stride, v_row_stride, n_pages, H_kv, page_size, box))
+    return RDKV_ERR_BAD_SHAPE;
+  return paged_decode_launch(A, bf, tm_k, tm_v, (cudaStream_t)stream);
 }

@@ -1,0 +1,448 @@
+// Attention of the new tokens of a batch of requests over their paged keys and values: what its two kernels share.
+//
+// Request i's cache holds kv_len_i tokens, the last n_i = q_start[i+1] - q_start[i] of them new ones: query row j of
+// the request stands at position p = kv_len_i - n_i + j and sees key s if s <= p, and, under a window of w tokens,
+// s > p - w or s < sinks, and if the page of s is there (a page number outside the pages stands for none):
+//   o = sum_s softmax_s(scale * q.k_s) v_s;  a row that sees nothing is zero (record: m = -inf, l = 0).
+//
+// Both kernels cut their work the same way.  An ITEM is (request, group of its new tokens, KV head): the rows (token, query
+// head of the KV head) of the group stand one under the other in one tile of the tensor cores.  Its keys come in
+// tiles; only tiles that some row of the group can see count (the sinks' tiles, then the window's).  All items in order,
+// their tiles one after another and a fixed cost each, make one line of units, which is cut into as many equal parts
+// as there are CTAs: long contexts and short ones, chunks and single tokens balance without a plan from the host.
+// Every CTA finds its part of the line from the lengths alone (paged_place), so nothing has to be known or copied
+// before the launch.  An item that a cut goes through leaves records (m, l, o) of its parts, which a small dependent
+// kernel joins in order: the same bits every time.
+#pragma once
+
+#include <algorithm>
+#include <cstring>
+
+#include "sm100.cuh"
+
+namespace rdkv {
+
+constexpr float PAGED_LOG2E = 1.4426950408889634f, PAGED_LN2 = 0.6931471805599453f;
+constexpr int PAGED_SMS = 148;
+constexpr int PAGED_CHANNELS = 128;
+
+struct PagedArgs {
+  const uint16_t* q; const uint16_t* k; const uint16_t* v;
+  int64_t q_tok, q_head;                          // elements
+  int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+  int n_pages, page, page_log2, H_q, H_kv, g;
+  const int32_t* table; int64_t table_stride; int width;
+  int cap;                                        // tokens a row of the table has room for
+  const int32_t* q_start; const int32_t* kv_lens; int S, T;
+  int window, sinks;                              // window 0: everything
+  int group;                                      // new tokens of an item
+  float scale_log2;                               // scale * log2 e: scores are kept in base 2
+  uint16_t* out; int64_t o_tok, o_head; int zero_pad;
+  float* rec;                                     // [T][H_q][132] instead of out
+  // workspace
+  int4* place;                                    // [G+1] where CTA c starts: request, head, group, tile
+  int* status;                                    // [G] 1: a wait of the CTA ran out
+  float* part;                                    // [2 G][rows of an item][132] records of cut items
+};
+
+template <bool BF16>
+__device__ __forceinline__ float paged_up(uint16_t x) { return BF16 ? __uint_as_float((uint32_t)x << 16) : h2f(x); }
+template <bool BF16>
+__device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {   // two values rounded to the 16-bit type
+  if (BF16) { const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&v); }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Softmax weights are rounded to the 16-bit type for the second product (its operands have one type, and the values
+// have that one): half a step of each weight's own size, against which the total is kept unrounded in 32 bits.  The
+// running maximum only moves when a score passes it by more than RAISE (in base 2), so that accumulators are rarely
+// rescaled; fp16 weights are 2^LIFT times larger, which keeps all that are over 2^-24 of the largest out of its subnormals.
+template <bool BF16> struct PagedWeights { static constexpr float RAISE = 8.f, LIFT = 0.f; };
+template <> struct PagedWeights<false> { static constexpr float RAISE = 4.f, LIFT = 10.f; };
+
+// ── items ───────────────────────────────────────────────────────────────────
+struct PagedRequest { int q0, n, len; };          // first query row, new tokens, tokens
+struct PagedItem {
+  int tok0, n_tok;                                // query rows of the group
+  int p0;                                         // position of the first (below zero: it sees nothing)
+  int hi;                                         // keys [0, hi) are in front of the last one's end
+  int t_lo, t_sink, n;                            // tiles [0, t_sink) and from t_lo on: n in all
+};
+
+__device__ __forceinline__ PagedRequest paged_request(const PagedArgs& A, int i) {
+  PagedRequest r;
+  r.q0 = min(max(A.q_start[i], 0), A.T);
+  r.n = min(max(A.q_start[i + 1], r.q0), A.T) - r.q0;
+  r.len = max(A.kv_lens[i], 0);
+  return r;
+}
+__device__ __forceinline__ int paged_groups(const PagedArgs& A, const PagedRequest& r) { return (r.n + A.group - 1) / A.group; }
+
+template <int KEYS>
+__device__ __forceinline__ PagedItem paged_item(const PagedArgs& A, const PagedRequest& r, int group) {
+  PagedItem it;
+  const int j0 = group * A.group;
+  it.tok0 = r.q0 + j0;
+  it.n_tok = min(A.group, r.n - j0);
+  it.p0 = r.len - r.n + j0;
+  it.hi = max(0, min(it.p0 + it.n_tok, A.cap));
+  const int t_hi = (it.hi + KEYS - 1) / KEYS;
+  const int lo = A.window > 0 ? max(0, it.p0 - A.window + 1) : 0;
+  it.t_lo = min(lo / KEYS, t_hi);
+  it.t_sink = A.window > 0 ? min((min(A.sinks, it.hi) + KEYS - 1) / KEYS, it.t_lo) : 0;
+  it.n = it.t_sink + t_hi - it.t_lo;
+  return it;
+}
+__device__ __forceinline__ int paged_tile(const PagedItem& it, int k) { return k < it.t_sink ? k : it.t_lo + k - it.t_sink; }
+
+// ── the line of units ───────────────────────────────────────────────────────
+struct PagedPlace { int i, head, group, tile; };  // i = S: the end
+
+struct PagedPlaceScratch { uint64_t part[32]; uint64_t at[2], width[2]; int request[2]; int4 found[2]; };
+
+// Where the parts of CTA c of G start and end.  All threads of the block (NT, whole warps) call it.  FIXED: cost of an item besides its
+// tiles; a cut that would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.
+template <int KEYS, int NT, int FIXED, int SNAP>
+__device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, PagedPlaceScratch& s, PagedPlace& from, PagedPlace& to) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // units of a head of request i
+  auto units = [&](int i) -> uint32_t {
+    PagedRequest r = {0, 0, 0};
+    if (i < A.S) r = paged_request(A, i);
+    const int groups = paged_groups(A, r);
+    uint32_t sum = 0;
+    if (groups <= 4)
+      for (int x = 0; x < groups; ++x) sum += paged_item<KEYS>(A, r, x).n + FIXED;
+    unsigned many = __ballot_sync(0xffffffffu, groups > 4);   // long chunks: the warp's lanes take their groups
+    while (many != 0) {
+      const int from_lane = __ffs(many) - 1;
+      many &= many - 1;
+      PagedRequest o;
+      o.q0 = __shfl_sync(0xffffffffu, r.q0, from_lane); o.n = __shfl_sync(0xffffffffu, r.n, from_lane);
+      o.len = __shfl_sync(0xffffffffu, r.len, from_lane);
+      const int n = paged_groups(A, o);
+      uint32_t mine = 0;
+      for (int x = lane; x < n; x += 32) mine += paged_item<KEYS>(A, o, x).n + FIXED;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+      if (lane == from_lane) sum = mine;
+    }
+    return sum;
+  };
+  auto block_scan = [&](uint64_t x, uint64_t& before, uint64_t& all) {   // exclusive sum over the block's threads
+    uint64_t incl = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    __syncthreads();
+    if (lane == 31) s.part[warp] = incl;
+    __syncthreads();
+    before = incl - x; all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < warp) before += s.part[w];
+      all += s.part[w];
+    }
+  };
+  if (tid < 2) s.request[tid] = A.S;
+  uint64_t total = 0, before = 0, all;
+  uint32_t mine = 0;
+  for (int base = 0; base < A.S; base += NT) {
+    mine = units(base + tid);
+    block_scan(mine, before, all);
+    total += all;
+  }
+  total *= (uint64_t)A.H_kv;
+  const uint64_t cut[2] = {(uint64_t)c * total / (uint64_t)G, (uint64_t)(c + 1) * total / (uint64_t)G};
+  uint64_t run = 0;
+  for (int base = 0; base < A.S; base += NT) {
+    if (A.S > NT) { mine = units(base + tid); block_scan(mine, before, all); }
+    const uint64_t a = (run + before) * A.H_kv, b = a + (uint64_t)mine * A.H_kv;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (cut[e] >= a && cut[e] < b) { s.request[e] = base + tid; s.at[e] = cut[e] - a; s.width[e] = mine; }
+    run += all;
+  }
+  __syncthreads();
+  if (warp < 2) {                                 // warp e: the head, group and tile of cut e
+    const int i = s.request[warp];
+    int4 found = make_int4(A.S, 0, 0, 0);
+    if (i < A.S) {
+      const PagedRequest r = paged_request(A, i);
+      const int groups = paged_groups(A, r), head = (int)(s.at[warp] / s.width[warp]);
+      uint32_t left = (uint32_t)(s.at[warp] - (uint64_t)head * s.width[warp]);
+      for (int x0 = 0; x0 < groups; x0 += 32) {
+        const int n = x0 + lane < groups ? paged_item<KEYS>(A, r, x0 + lane).n : 0;
+        const uint32_t cost = x0 + lane < groups ? n + FIXED : 0;
+        uint32_t incl = cost;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const uint32_t y = __shfl_up_sync(0xffffffffu, incl, d);
+          if (lane >= d) incl += y;
+        }
+        const uint32_t sum = __shfl_sync(0xffffffffu, incl, 31);
+        if (left < sum) {
+          if (left >= incl - cost && left < incl) {
+            int tile = max(0, (int)(left - (incl - cost)) - FIXED);
+            if (tile < SNAP) tile = 0;
+            else if (n - tile < SNAP) tile = n;
+            s.found[warp] = make_int4(i, head, x0 + lane, tile);
+          }
+          break;
+        }
+        left -= sum;
+      }
+    } else if (lane == 0) {
+      s.found[warp] = found;
+    }
+  }
+  __syncthreads();
+  const int4 f = s.found[0], t = s.found[1];
+  from = {f.x, f.y, f.z, f.w};
+  to = {t.x, t.y, t.z, t.w};
+  if (tid == 0) {
+    A.place[c] = f;
+    if (c == G - 1) A.place[G] = make_int4(A.S, 0, 0, 0);
+  }
+}
+
+// The segments of a CTA: runs of tiles of one item.  Every role of the CTA walks them by itself.
+struct PagedSegment {
+  PagedRequest request;
+  PagedItem item;
+  int i, head, group, k0, k1;
+};
+template <int KEYS>
+struct PagedWalk {
+  PagedPlace at, to;
+  PagedRequest r;
+  int groups;
+  bool done;
+  __device__ __forceinline__ PagedWalk(const PagedArgs& A, const PagedPlace& from, const PagedPlace& end) : at(from), to(end), done(false) {
+    load(A);
+  }
+  __device__ __forceinline__ void load(const PagedArgs& A) {
+    groups = 0;
+    if (at.i < A.S) { r = paged_request(A, at.i); groups = paged_groups(A, r); }
+  }
+  __device__ __forceinline__ bool next(const PagedArgs& A, PagedSegment& s) {
+    while (!done && at.i < A.S) {
+      if (at.i > to.i) { done = true; break; }
+      if (groups == 0) { ++at.i; at.head = at.group = at.tile = 0; load(A); continue; }
+      const bool last = at.i == to.i && at.head == to.head && at.group == to.group;
+      s.request = r; s.i = at.i; s.head = at.head; s.group = at.group;
+      s.item = paged_item<KEYS>(A, r, at.group);
+      s.k0 = at.tile;
+      s.k1 = last ? min(to.tile, s.item.n) : s.item.n;
+      const bool some = s.k0 < s.k1 || (s.item.n == 0 && s.k0 == 0 && !last);
+      at.tile = 0;
+      if (last) done = true;
+      else if (++at.group == groups) {
+        at.group = 0;
+        if (++at.head == A.H_kv) { at.head = 0; ++at.i; load(A); }
+      }
+      if (some) return true;
+    }
+    return false;
+  }
+};
+
+// ── results ─────────────────────────────────────────────────────────────────
+// Where a row of a segment goes: the result (normalised, 16 bits), the caller's record, or a record in the workspace.
+struct PagedRow { uint16_t* out; float* rec; };
+template <int ROWS>
+__device__ __forceinline__ PagedRow paged_row(const PagedArgs& A, const PagedSegment& s, int row, int cta) {
+  PagedRow d = {nullptr, nullptr};
+  if (s.k0 == 0 && s.k1 == s.item.n) {
+    const int tok = row / A.g, hq = s.head * A.g + (row - tok * A.g);
+    const int64_t t = s.item.tok0 + tok;
+    if (A.rec != nullptr) d.rec = A.rec + (t * A.H_q + hq) * RDKV_PARTIAL_STRIDE;
+    else d.out = A.out + t * A.o_tok + hq * A.o_head;
+  } else {
+    d.rec = A.part + ((int64_t)(2 * cta + (s.k0 > 0 ? 0 : 1)) * ROWS + row) * RDKV_PARTIAL_STRIDE;
+  }
+  return d;
+}
+// 1 / l, or zero for a row that saw nothing (NaN stays NaN).
+__device__ __forceinline__ float paged_over(float l) { return l == 0.f ? 0.f : __fdividef(1.f, l); }
+
+// One row of a segment, by one warp in 32 bits, a key after the other: for rows whose tile holds values that are not
+// finite at keys that some of its rows see and others do not (a product with a zero weight would carry them over).
+template <bool BF16, int KEYS, int ROWS>
+__device__ __noinline__ void paged_slow_row(const PagedArgs& A, const PagedSegment& s, int row, int cta) {
+  const int lane = threadIdx.x & 31, tok = row / A.g, hq = s.head * A.g + (row - tok * A.g);
+  const int pos = s.item.p0 + tok;
+  const uint2 qw = *reinterpret_cast<const uint2*>(A.q + (int64_t)(s.item.tok0 + tok) * A.q_tok + (int64_t)hq * A.q_head + 4 * lane);
+  const float q[4] = {paged_up<BF16>(qw.x & 0xFFFF), paged_up<BF16>(qw.x >> 16), paged_up<BF16>(qw.y & 0xFFFF), paged_up<BF16>(qw.y >> 16)};
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = s.k0; k < s.k1; ++k) {
+    const int key0 = paged_tile(s.item, k) * KEYS;
+    for (int key = key0; key < min(key0 + KEYS, s.item.hi); ++key) {
+      if (key > pos || (A.window > 0 && key <= pos - A.window && key >= A.sinks)) continue;
+      const int id = A.table[s.i * A.table_stride + (key >> A.page_log2)];
+      if (id < 0 || id >= A.n_pages) continue;
+      const int64_t r = key & (A.page - 1);
+      const uint2 kw = *reinterpret_cast<const uint2*>(A.k + id * A.k_page + s.head * A.k_head + r * A.k_row + 4 * lane);
+      const uint2 vw = *reinterpret_cast<const uint2*>(A.v + id * A.v_page + s.head * A.v_head + r * A.v_row + 4 * lane);
+      float x = q[0] * paged_up<BF16>(kw.x & 0xFFFF);
+      x = fmaf(q[1], paged_up<BF16>(kw.x >> 16), x); x = fmaf(q[2], paged_up<BF16>(kw.y & 0xFFFF), x);
+      x = fmaf(q[3], paged_up<BF16>(kw.y >> 16), x);
+      x = warp_sum(x) * A.scale_log2;
+      const float n = fmaxf(m, x), base = n == -INFINITY ? 0.f : n;
+      const float a = exp2_approx(m - base), p = exp2_approx(x - base);   // (m = -inf: 0)
+      l = fmaf(l, a, p);
+      o[0] = fmaf(o[0], a, p * paged_up<BF16>(vw.x & 0xFFFF)); o[1] = fmaf(o[1], a, p * paged_up<BF16>(vw.x >> 16));
+      o[2] = fmaf(o[2], a, p * paged_up<BF16>(vw.y & 0xFFFF)); o[3] = fmaf(o[3], a, p * paged_up<BF16>(vw.y >> 16));
+      m = n;
+    }
+  }
+  const PagedRow d = paged_row<ROWS>(A, s, row, cta);
+  if (d.rec != nullptr) {
+    *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4(m * PAGED_LN2, l, 0.f, 0.f);
+  } else {
+    const float w = paged_over(l);
+    *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(o[0] * w, o[1] * w), paged_pack<BF16>(o[2] * w, o[3] * w));
+  }
+}
+
+// Rows that belong to no request, in a result that the call allocated: zeros.  All threads of the grid.
+__device__ __forceinline__ void paged_zero_padding(const PagedArgs& A, int n_threads) {
+  if (!A.zero_pad || A.rec != nullptr) return;
+  const int first = A.S > 0 ? min(max(A.q_start[0], 0), A.T) : A.T;
+  const int end = A.S > 0 ? min(max(A.q_start[A.S], first), A.T) : A.T;
+  const int64_t rows = (int64_t)(first + A.T - end) * A.H_q * 16;           // 16 bytes a step
+  for (int64_t x = (int64_t)blockIdx.x * n_threads + threadIdx.x; x < rows; x += (int64_t)gridDim.x * n_threads) {
+    const int64_t row = x >> 4, tk = row / A.H_q, hq = row - tk * A.H_q;
+    const int64_t t = tk < first ? tk : end + (tk - first);
+    *reinterpret_cast<uint4*>(A.out + t * A.o_tok + hq * A.o_head + (x & 15) * 8) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// Joins the records of items that a cut went through.  Block (c, y): if the cut in front of CTA c is the first one inside an
+// item, rows y, y + gridDim.y * 8, ... of that item, a warp each.
+constexpr int PAGED_JOIN_WARPS = 8;
+template <bool BF16, int KEYS, int ROWS, int G>
+__global__ void __launch_bounds__(PAGED_JOIN_WARPS * 32)
+paged_join_kernel(const PagedArgs A) {
+  __shared__ float s_w[PAGED_JOIN_WARPS][G];
+  __shared__ uint8_t s_some[G];
+  wait_for_previous_kernel();
+  const int c = blockIdx.x + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int4 at = A.place[c], prev = A.place[c - 1];
+  if (at.x >= A.S || at.w == 0) return;
+  PagedSegment s;
+  s.request = paged_request(A, at.x);
+  s.item = paged_item<KEYS>(A, s.request, at.z);
+  s.i = at.x; s.head = at.y; s.group = at.z; s.k0 = 0; s.k1 = s.item.n;
+  if (at.w >= s.item.n) return;
+  if (prev.x == at.x && prev.y == at.y && prev.z == at.z && prev.w > 0) return;   // an earlier cut is in this item
+  // the CTAs from c on that start inside the item (a run), and which of them have tiles of it
+  int n_more = 0;
+  for (int base = c; base < G; base += PAGED_JOIN_WARPS * 32) {
+    const int x = base + tid;
+    bool in = false;
+    if (x < G) {
+      const int4 a = A.place[x], b = A.place[x + 1];
+      in = a.x == at.x && a.y == at.y && a.z == at.z && a.w > 0 && a.w < s.item.n;
+      s_some[x - c] = in && !(b.x == at.x && b.y == at.y && b.z == at.z && b.w == a.w);
+    }
+    const int n = __syncthreads_count(in);
+    n_more += n;
+    if (n < PAGED_JOIN_WARPS * 32) break;
+  }
+  const int n_parts = 1 + n_more, rows = s.item.n_tok * A.g;
+  // record of part x (0: the CTA in front of the cut, its last segment; others: the first segment of CTA c + x - 1)
+  auto record = [&](int x, int row) {
+    return A.part + ((int64_t)(x == 0 ? 2 * (c - 1) + 1 : 2 * (c + x - 1)) * ROWS + row) * RDKV_PARTIAL_STRIDE;
+  };
+  for (int row = blockIdx.y * PAGED_JOIN_WARPS + warp; row < rows; row += gridDim.y * PAGED_JOIN_WARPS) {
+    float M = -INFINITY;
+    for (int x = lane; x < n_parts; x += 32) {
+      const float m = x == 0 || s_some[x - 1] ? record(x, row)[0] : -INFINITY;
+      s_w[warp][x] = m;
+      M = fmaxf(M, m);
+    }
+    M = warp_max(M);
+    float L = 0.f;
+    for (int x = lane; x < n_parts; x += 32) {
+      const float m = s_w[warp][x];
+      float w = 0.f;
+      if (x == 0 || s_some[x - 1]) {
+        w = m == -INFINITY ? 0.f : exp2_approx((m - M) * PAGED_LOG2E);
+        L = fmaf(record(x, row)[1], w, L);
+      }
+      s_w[warp][x] = w;
+    }
+    L = warp_sum(L);
+    __syncwarp();
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int x = 0; x < n_parts; ++x) {
+      const float w = s_w[warp][x];
+      if (x > 0 && !s_some[x - 1]) continue;
+      const float4 p = *reinterpret_cast<const float4*>(record(x, row) + 4 + 4 * lane);
+      o.x = fmaf(p.x, w, o.x); o.y = fmaf(p.y, w, o.y); o.z = fmaf(p.z, w, o.z); o.w = fmaf(p.w, w, o.w);
+    }
+    const PagedRow d = paged_row<ROWS>(A, s, row, 0);
+    if (d.rec != nullptr) {
+      *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = o;
+      if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4(M, L, 0.f, 0.f);
+    } else {
+      const float w = paged_over(L);
+      *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(o.x * w, o.y * w), paged_pack<BF16>(o.z * w, o.w * w));
+    }
+    __syncwarp();
+  }
+}
+
+// A map over pages [n_pages][H_kv][page][128] (strides in elements) whose boxes are `rows` tokens of 64 channels, laid down with the
+// 128-byte swizzle.  No pages: an empty map, which no kernel uses then.
+inline bool paged_map(CUtensorMap* tm, const void* base, bool bf16, int64_t page_stride, int64_t head_stride, int64_t row_stride,
+                      int64_t n_pages, int64_t heads, int64_t page, int rows) {
+  memset(tm, 0, sizeof(*tm));
+  if (n_pages == 0) return true;
+  TensorMapEncoder enc = tensor_map_encoder();
+  if (enc == nullptr || (reinterpret_cast<uintptr_t>(base) & 15) != 0) return false;
+  if (heads == 1) head_stride = PAGED_CHANNELS;               // (strides of dimensions of one element mean nothing)
+  if (n_pages == 1) page_stride = PAGED_CHANNELS;
+  const cuuint64_t dims[4] = {PAGED_CHANNELS, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)row_stride * 2u, (cuuint64_t)head_stride * 2u, (cuuint64_t)page_stride * 2u};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)rows, 1u, 1u}, elem[4] = {1u, 1u, 1u, 1u};
+  if (row_stride <= 0 || head_stride <= 0 || page_stride <= 0 || (row_stride & 7) || (head_stride & 7) || (page_stride & 7)) return false;
+  return enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+             elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Workspace of a launch of G CTAs whose items have up to `rows` rows.
+inline int64_t paged_workspace_bytes(int G, int rows) {
+  return (int64_t)(G + 1) * 16 + (((int64_t)G * 4 + 15) / 16) * 16 + (int64_t)2 * G * rows * RDKV_PARTIAL_STRIDE * 4;
+}
+inline void paged_workspace(PagedArgs* A, void* workspace, int G) {
+  char* p = static_cast<char*>(workspace);
+  A->place = reinterpret_cast<int4*>(p); p += (int64_t)(G + 1) * 16;
+  A->status = reinterpret_cast<int*>(p); p += (((int64_t)G * 4 + 15) / 16) * 16;
+  A->part = reinterpret_cast<float*>(p);
+}
+
+template <class Kernel>
+inline int paged_launch_join(Kernel join, const PagedArgs& A, dim3 grid, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+  cfg.gridDim = grid; cfg.blockDim = dim3(PAGED_JOIN_WARPS * 32);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join, A);
+  if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
+  return launch_status();
+}
+
+int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st);
+constexpr int PAGED_DECODE_ROWS = 16, PAGED_DECODE_CTAS = 2 * PAGED_SMS, PAGED_DECODE_KEYS = 64;
+
+}  // namespace rdkv

@@ -13,7 +13,7 @@ def _lib():
 def _attention(**change):
     a = dict(q=1 << 12, q_tok=1024, q_head=128, dtype=0, T=4, H_q=8, k=1 << 12, k_page=1, k_head=1, k_row=128, v=1 << 12, v_page=1, v_head=1,
              v_row=128, n_pages=2, H_kv=2, page=16, table=1 << 12, stride=4, width=4, q_start=1 << 12, lens=1 << 12, S=1, max_new=4, window=0,
-             sinks=0, scale=1.0, out=1 << 12, o_tok=1024, o_head=128, pad=0, rec=None, ws=None, ws_bytes=0, stream=None)
+             sinks=0, scale=1.0, out=1 << 12, o_tok=1024, o_head=128, pad=0, rec=None, ws=1 << 12, ws_bytes=1 << 40, stream=None)
     assert set(change) <= set(a)
     return _lib().rdkv_paged_attention(*{**a, **change}.values())
 
@@ -22,7 +22,8 @@ def _attention(**change):
     (dict(T=-1), 1), (dict(S=-1), 1), (dict(H_q=0), 1), (dict(H_kv=0), 1), (dict(dtype=2), 1), (dict(dtype=7), 1), (dict(window=-1), 1),
     (dict(sinks=-1), 1), (dict(max_new=-1), 1), (dict(width=-1), 1), (dict(n_pages=-1), 1), (dict(H_kv=3), 2), (dict(H_q=34), 2), (dict(page=8), 2),
     (dict(page=24), 2), (dict(page=2048), 2), (dict(q=None), 1), (dict(q_start=None), 1), (dict(lens=None), 1), (dict(table=None), 1),
-    (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(rec=1 << 12), 1), (dict(T=0, q=None), 0)])
+    (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(rec=1 << 12), 1), (dict(ws=None), 1), (dict(ws=(1 << 12) + 8), 1), (dict(ws_bytes=100), 1),
+    (dict(T=0, q=None), 0)])
 def test_attention_refusals(change, status):
     assert _attention(**change) == status
 

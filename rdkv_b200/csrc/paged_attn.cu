@@ -46,14 +46,6 @@ __device__ __forceinline__ bool dec_barrier_any(bool x) {                       
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"((uint32_t)x) : "memory");
   return any != 0;
 }
-// Whether one of the two 16-bit values that `which` selects is not finite.
-template <bool BF16>
-__device__ __forceinline__ bool dec_not_finite(uint32_t v, uint32_t which) {
-  constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
-  const uint32_t x = v & which;
-  return (x & E) == E || ((x >> 16) & E) == E;
-}
-
 template <bool BF16>
 __global__ void __launch_bounds__(DEC_THREADS, 2)
 paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
@@ -102,7 +94,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
           ids_next = page_of(k + batch);
         }
         const int slot = count % DEC_STAGES;
-        if (count >= DEC_STAGES && !bar_wait(bar + 8 * (DEC_STAGES + slot), (count / DEC_STAGES - 1) & 1)) { ok = false; break; }
+        if (count >= DEC_STAGES && !bar_wait_warp(bar + 8 * (DEC_STAGES + slot), (count / DEC_STAGES - 1) & 1)) { ok = false; break; }
         const int key0 = paged_tile(s.item, k) * DEC_KEYS;
         const int id = __shfl_sync(0xffffffffu, ids, in_batch * per_tile + (box < per_tile ? box : 0));
         const bool there = box < per_tile && id >= 0 && id < A.n_pages;
@@ -167,7 +159,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       bool again = false;
       for (int k = s.k0; k < s.k1; ++k, ++count) {
         const int slot = count % DEC_STAGES;
-        ok = ok && bar_wait(bar + 8 * slot, (count / DEC_STAGES) & 1);
+        ok = bar_wait_warp(bar + 8 * slot, (count / DEC_STAGES) & 1);
         if (!ok) break;
         const int2 info = s_info[slot];
         const int key0 = info.x + warp * 16;
@@ -252,8 +244,8 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
             dec_ldmatrix_t(b, vb + (c16 >> 3) * DEC_PANEL + row * 128 + (((c16 & 7) ^ (row & 7)) << 4));
             if (edge) {
               if ((some0 | some1) != 0u)
-                again |= dec_not_finite<BF16>(b[0], some0) || dec_not_finite<BF16>(b[1], some1) || dec_not_finite<BF16>(b[2], some0) ||
-                         dec_not_finite<BF16>(b[3], some1);
+                again |= paged_not_finite<BF16>(b[0] & some0) || paged_not_finite<BF16>(b[1] & some1) || paged_not_finite<BF16>(b[2] & some0) ||
+                         paged_not_finite<BF16>(b[3] & some1);
               b[0] &= live0; b[1] &= live1; b[2] &= live0; b[3] &= live1;
             }
             dec_mma<BF16>(o[2 * cc], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
@@ -347,10 +339,14 @@ int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, 
 
 using namespace rdkv;
 
+// Rows of a request's longest chunk under one KV head decide the kernel: up to 16 fill one tile of the decode kernel.
+static bool paged_few_rows(int max_new, int g) { return (int64_t)max_new * g <= PAGED_DECODE_ROWS; }
+
 extern "C" int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, int H_q, int H_kv, int max_new) {
   if (n_requests < 0 || n_tokens < 0 || H_q <= 0 || H_kv <= 0 || max_new < 0) return -1;
   if (n_tokens == 0) return 0;
-  return paged_workspace_bytes(PAGED_DECODE_CTAS, PAGED_DECODE_ROWS);
+  return paged_few_rows(max_new, H_q / H_kv) ? paged_workspace_bytes(PAGED_DECODE_CTAS, PAGED_DECODE_ROWS)
+                                             : paged_workspace_bytes(PAGED_CHUNK_CTAS, PAGED_CHUNK_ROWS);
 }
 
 extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype, int n_tokens, int H_q,
@@ -360,7 +356,7 @@ extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t
                                     int width, const int32_t* q_start, const int32_t* kv_lens, int n_requests, int max_new,
                                     int window, int sinks, float scale, void* out, int64_t out_tok_stride, int64_t out_head_stride,
                                     int zero_padding, float* out_partial, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (n_tokens < 0 || n_requests < 0 || H_q <= 0 || H_kv <= 0 || n_pages < 0 || width < 0 || window < 0 || sinks < 0 || max_new < 0)
+  if (n_tokens < 0 || n_requests < 0 || H_q <= 0 || H_kv <= 0 || n_pages < 0 || width < 0 || window < 0 || sinks < 0 || max_new < 0 || !(scale > 0.f))
     return RDKV_ERR_BAD_ARG;
   if (dtype != RDKV_F16 && dtype != RDKV_BF16) return RDKV_ERR_BAD_ARG;
   if (H_q % H_kv != 0 || H_q / H_kv > MAX_GROUP) return RDKV_ERR_BAD_SHAPE;
@@ -385,12 +381,13 @@ extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t
   A.window = std::min(window, 1 << 30); A.sinks = std::min(sinks, 1 << 30); A.scale_log2 = scale * PAGED_LOG2E;
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
   const bool bf = dtype == RDKV_BF16;
-  A.group = PAGED_DECODE_ROWS / A.g;
-  paged_workspace(&A, workspace, PAGED_DECODE_CTAS);
+  const bool few = paged_few_rows(max_new, A.g);
+  A.group = few ? PAGED_DECODE_ROWS / A.g : 2 * (128 / A.g);
+  paged_workspace(&A, workspace, few ? PAGED_DECODE_CTAS : PAGED_CHUNK_CTAS);
   CUtensorMap tm_k, tm_v;
-  const int box = std::min(page_size, PAGED_DECODE_KEYS);
+  const int box = std::min(page_size, few ? PAGED_DECODE_KEYS : PAGED_CHUNK_KEYS);
   if (!paged_map(&tm_k, k_pages, bf, k_page_stride, k_head_stride, k_row_stride, n_pages, H_kv, page_size, box) ||
       !paged_map(&tm_v, v_pages, bf, v_page_stride, v_head_stride, v_row_stride, n_pages, H_kv, page_size, box))
     return RDKV_ERR_BAD_SHAPE;
-  return paged_decode_launch(A, bf, tm_k, tm_v, (cudaStream_t)stream);
+  return few ? paged_decode_launch(A, bf, tm_k, tm_v, (cudaStream_t)stream) : paged_chunk_launch(A, bf, tm_k, tm_v, (cudaStream_t)stream);
 }

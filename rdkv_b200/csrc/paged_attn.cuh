@@ -61,6 +61,18 @@ __device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {   // two va
 template <bool BF16> struct PagedWeights { static constexpr float RAISE = 8.f, LIFT = 0.f; };
 template <> struct PagedWeights<false> { static constexpr float RAISE = 4.f, LIFT = 10.f; };
 
+int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st);
+int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st);
+constexpr int PAGED_CHUNK_ROWS = 256, PAGED_CHUNK_CTAS = PAGED_SMS, PAGED_CHUNK_KEYS = 128;
+constexpr int PAGED_DECODE_ROWS = 16, PAGED_DECODE_CTAS = 2 * PAGED_SMS, PAGED_DECODE_KEYS = 64;
+
+// Whether one of a pair of 16-bit values is not finite.
+template <bool BF16>
+__device__ __forceinline__ bool paged_not_finite(uint32_t x) {
+  constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
+  return (x & E) == E || ((x >> 16) & E) == E;
+}
+
 // ── items ───────────────────────────────────────────────────────────────────
 struct PagedRequest { int q0, n, len; };          // first query row, new tokens, tokens
 struct PagedItem {
@@ -441,8 +453,5 @@ inline int paged_launch_join(Kernel join, const PagedArgs& A, dim3 grid, cudaStr
   if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
   return launch_status();
 }
-
-int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st);
-constexpr int PAGED_DECODE_ROWS = 16, PAGED_DECODE_CTAS = 2 * PAGED_SMS, PAGED_DECODE_KEYS = 64;
 
 }  // namespace rdkv

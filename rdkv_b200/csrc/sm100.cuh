@@ -43,6 +43,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
     if (bar_try(bar, parity)) return true;
   return false;
 }
+// The same for a whole warp: all its lanes go on, or none does.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ── dependent launches ──────────────────────────────────────────────────────
@@ -61,6 +63,79 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm,
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
                : "memory");
 }
+
+// ── tensor memory and tcgen05 ───────────────────────────────────────────────
+// Shared-memory matrix descriptors of operands laid down with the 128-byte swizzle.  Bits [0,14) start address / 16,
+// [16,30) leading-dimension offset / 16, [32,46) stride-dimension offset / 16, [46,48) version 1, [61,64) 2 = 128-byte swizzle.
+// K-major (rows of 64 16-bit elements along K, 8 rows 1024 bytes apart): the leading offset is not used.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// MN-major (a row of 64 16-bit elements along N for every step of K, 8 steps 1024 bytes apart): `panel` bytes to the next 64 of N.
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t panel) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor of a dense 16-bit MMA of 128 x n with fp32 accumulation: bits [4,6) accumulator 1 = fp32, [7,10) and
+// [10,13) operand types (0 = fp16, 1 = bf16), 16: B is MN-major, [17,23) N / 8, [24,29) M / 16.
+template <bool BF16>
+__device__ __forceinline__ constexpr uint32_t mma_idesc(int n, bool b_mn_major) {
+  return 1u << 4 | (BF16 ? 1u : 0u) << 7 | (BF16 ? 1u : 0u) << 10 | (b_mn_major ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 |
+         (uint32_t)(128 >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {   // A in shared memory
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {   // A in tensor memory
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {   // the barrier gets an arrival once the MMAs issued so far are done
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define RDKV_R8(v, i) "=r"((v)[i]), "=r"((v)[i + 1]), "=r"((v)[i + 2]), "=r"((v)[i + 3]), "=r"((v)[i + 4]), "=r"((v)[i + 5]), "=r"((v)[i + 6]), "=r"((v)[i + 7])
+#define RDKV_S8(v, i) "r"((v)[i]), "r"((v)[i + 1]), "r"((v)[i + 2]), "r"((v)[i + 3]), "r"((v)[i + 4]), "r"((v)[i + 5]), "r"((v)[i + 6]), "r"((v)[i + 7])
+// 32 consecutive 32-bit columns of this thread's row (lane i of warp w: row 32*(w&3)+i).  The wait is part of the statement, so
+// that no use of the registers can move ahead of it.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : RDKV_R8(v, 0), RDKV_R8(v, 8), RDKV_R8(v, 16), RDKV_R8(v, 24)
+      : "r"(taddr)
+      : "memory");
+}
+// 128 columns.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "{\n"
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, "
+      "%46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, "
+      "%72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, "
+      "%98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, "
+      "%120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      "}\n"
+      : RDKV_R8(v, 0), RDKV_R8(v, 8), RDKV_R8(v, 16), RDKV_R8(v, 24), RDKV_R8(v, 32), RDKV_R8(v, 40), RDKV_R8(v, 48), RDKV_R8(v, 56),
+        RDKV_R8(v, 64), RDKV_R8(v, 72), RDKV_R8(v, 80), RDKV_R8(v, 88), RDKV_R8(v, 96), RDKV_R8(v, 104), RDKV_R8(v, 112), RDKV_R8(v, 120)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+      ::"r"(taddr), RDKV_S8(v, 0), RDKV_S8(v, 8), RDKV_S8(v, 16), RDKV_S8(v, 24)
+      : "memory");
+}
+#undef RDKV_R8
+#undef RDKV_S8
 
 // The driver's tensor-map encoder, found through the runtime (the library does not link the driver).
 using TensorMapEncoder = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -206,6 +206,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
         raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError("window and sinks must not be negative, and sinks need a window")
+    if scale is not None and not scale > 0:
+        raise ValueError(f"scale must be positive, got {scale}")
     max_new = T if max_new is None else min(int(max_new), T)
     if max_new < 0:
         raise ValueError("max_new must not be negative")

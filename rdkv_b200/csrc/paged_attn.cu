@@ -10,6 +10,9 @@
 // segment's last tile.  Why not tcgen05: its smallest M is 64 rows, of which 4 to 16 would be used, and scores would
 // have to go through tensor memory and shared memory between the products; the tensor pipe is idle most of the time as it is.
 //
+// Few items (CLUSTER): each is cut evenly over a cluster of 8 or 16 CTAs, which exchange their records through distributed
+// shared memory; there is no line of units to find a place in and no second launch.
+//
 // Masks are applied only to 16-key blocks that reach past some row's limits.  There, values of keys that no row of
 // the item sees are set to zero (0 x NaN), and a value that is not finite at a key that only some rows see makes the
 // segment's rows be done again, one by one (paged_slow_row).
@@ -46,7 +49,44 @@ __device__ __forceinline__ bool dec_barrier_any(bool x) {                       
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"((uint32_t)x) : "memory");
   return any != 0;
 }
-template <bool BF16>
+__device__ __forceinline__ uint32_t dec_cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t dec_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void dec_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t dec_map(uint32_t addr, uint32_t rank) {   // this shared-memory address in CTA `rank` of the cluster
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 dec_remote4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// The segments of a CTA: of the line of units, or, in a cluster, an even part of every group of the cluster's (request, head).
+template <bool CLUSTER> struct DecWalk;
+template <> struct DecWalk<false> : PagedWalk<DEC_KEYS> { using PagedWalk<DEC_KEYS>::PagedWalk; };
+template <> struct DecWalk<true> {
+  PagedRequest r;
+  int i, head, group, groups, rank, size;
+  __device__ __forceinline__ explicit DecWalk(const PagedArgs& A) : group(0), rank((int)dec_cluster_rank()), size((int)dec_cluster_size()) {
+    const int item = blockIdx.x / size;
+    i = item / A.H_kv; head = item - i * A.H_kv;
+    r = paged_request(A, i);
+    groups = paged_groups(A, r);
+  }
+  __device__ __forceinline__ bool next(const PagedArgs& A, PagedSegment& s) {
+    if (group >= groups) return false;
+    s.request = r; s.i = i; s.head = head; s.group = group;
+    s.item = paged_item<DEC_KEYS>(A, r, group++);
+    s.k0 = (int)((int64_t)s.item.n * rank / size); s.k1 = (int)((int64_t)s.item.n * (rank + 1) / size);
+    return true;
+  }
+};
+
+template <bool BF16, bool CLUSTER>
 __global__ void __launch_bounds__(DEC_THREADS, 2)
 paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   extern __shared__ unsigned char dec_raw[];
@@ -56,6 +96,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
   __shared__ int s_again[2];                                // segment (its number + 1) whose rows are done again
   __shared__ int s_trouble;
   __shared__ PagedPlaceScratch s_place;
+  __shared__ __align__(16) float s_rec[CLUSTER ? DEC_ROWS : 1][RDKV_PARTIAL_STRIDE];   // this CTA's records (m in base 2; word 2 of the first: done again)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
   const uint32_t ring = (smem_addr(dec_raw) + 1023u) & ~1023u, bar = smem_addr(s_bar);
   unsigned char* ring_ptr = dec_raw + (ring - smem_addr(dec_raw));
@@ -65,11 +106,19 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     bar_init_fence();
     s_again[0] = s_again[1] = s_trouble = 0;
   }
-  let_next_kernel_start();
-  paged_zero_padding(A, DEC_THREADS);
-  PagedPlace from, to;
-  paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP>(A, cta, PAGED_DECODE_CTAS, s_place, from, to);   // (its barriers order the set-up too)
-  PagedWalk<DEC_KEYS> walk(A, from, to);
+  auto begin = [&]() {
+    if constexpr (CLUSTER) {
+      DecWalk<true> walk(A);
+      __syncthreads();
+      return walk;
+    } else {
+      let_next_kernel_start();
+      PagedPlace from, to;
+      paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP>(A, cta, PAGED_DECODE_CTAS, s_place, from, to);   // (its barriers order the set-up too)
+      return DecWalk<false>(A, from, to);
+    }
+  };
+  auto walk = begin();
   PagedSegment s;
 
   if (warp == DEC_WARPS) {
@@ -78,7 +127,8 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     const int box = lane >> 2, what = lane & 3;              // this lane's box of a tile: sub-tile, (K | V) x panel
     unsigned count = 0;
     bool ok = true;
-    while (ok && walk.next(A, s)) {
+    while ((ok || CLUSTER) && walk.next(A, s)) {             // (a cluster's barriers want every CTA, whatever happened)
+      if (CLUSTER && !ok) s.k1 = s.k0;
       const int32_t* table = A.table + s.i * A.table_stride;
       auto page_of = [&](int k) {                            // lane's entry of the batch that starts with tile k
         const int kk = k + lane / per_tile;
@@ -113,6 +163,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
           tma_load_4d(ring + slot * DEC_STAGE + what * DEC_PANEL + box * rows * 128, what < 2 ? &tm_k : &tm_v, (what & 1) * 64,
                       key0 & (A.page - 1), s.head, id, bar + 8 * slot);
       }
+      if (CLUSTER) { __syncwarp(); dec_cluster_sync(); dec_cluster_sync(); }
     }
     if (!ok) {                                               // wait (again bounded) for the copies in flight
       s_trouble = 1;
@@ -124,9 +175,11 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     const int r0 = lane >> 2, c2 = (lane & 3) * 2;           // this thread's rows r0, r0 + 8; its pair of columns
     unsigned count = 0, segment = 0;
     bool ok = true;
-    while (ok && walk.next(A, s)) {
+    while ((ok || CLUSTER) && walk.next(A, s)) {
       const int rows = s.item.n_tok * A.g, p_first = s.item.p0, p_last = s.item.p0 + s.item.n_tok - 1;
-      if (s.k0 == s.k1) {                                    // an item without keys
+      const bool none_mine = s.k0 == s.k1;
+      if (CLUSTER && !ok) s.k1 = s.k0;
+      if (!CLUSTER && none_mine) {                           // an item without keys
         for (int x = tid; x < rows * 32; x += DEC_WARPS * 32) {
           const PagedRow d = paged_row<DEC_ROWS>(A, s, x >> 5, cta);
           if (d.rec != nullptr) {
@@ -266,9 +319,10 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       if (again) s_again[segment & 1] = (int)segment + 1;
       ok = !dec_barrier_any(!ok);                            // (all four warps go on, or none does)
       if (!ok) s_trouble = 1;
-      const int slot = (count - 1) % DEC_STAGES;
+      const int slot = (count + DEC_STAGES - 1) % DEC_STAGES;   // (without tiles of its own, a CTA of a cluster has only empty records)
+      const bool some = !CLUSTER || s.k0 < s.k1;
       float* buf = reinterpret_cast<float*>(ring_ptr + slot * DEC_STAGE);
-      if (ok) {
+      if (ok && some) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int row = r0 + 8 * r;
@@ -282,7 +336,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       }
       dec_barrier();
       if (ok) {
-        if (s_again[segment & 1] == (int)segment + 1) {
+        if (!CLUSTER && s_again[segment & 1] == (int)segment + 1) {
           const PagedSegment copy = s;
           for (int row = warp; row < rows; row += DEC_WARPS) paged_slow_row<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, cta);
         } else {
@@ -290,9 +344,10 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
             float M = -INFINITY, L = 0.f;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < DEC_WARPS; ++w) M = fmaxf(M, s_ml[w][row].x);
+            for (int w = 0; w < DEC_WARPS; ++w) if (some) M = fmaxf(M, s_ml[w][row].x);
 #pragma unroll
             for (int w = 0; w < DEC_WARPS; ++w) {
+              if (!some) break;
               const float2 ml = s_ml[w][row];
               const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
               const float4 x = *reinterpret_cast<const float4*>(buf + ((w * DEC_ROWS + row) * 128 + 4 * lane));
@@ -300,6 +355,11 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
                 L = fmaf(ml.y, f, L);
                 sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
               }
+            }
+            if (CLUSTER) {
+              *reinterpret_cast<float4*>(&s_rec[row][4 + 4 * lane]) = sum;
+              if (lane == 0) *reinterpret_cast<float4*>(&s_rec[row][0]) = make_float4(M, L, 0.f, 0.f);
+              continue;
             }
             const PagedRow d = paged_row<DEC_ROWS>(A, s, row, cta);
             if (d.rec != nullptr) {
@@ -313,16 +373,84 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
         }
         fence_async_smem();                                  // (the slot's next writer is a TMA copy)
         __syncwarp();
-        if (lane == 0) bar_arrive(bar + 8 * (DEC_STAGES + slot));
+        if (lane == 0 && some) bar_arrive(bar + 8 * (DEC_STAGES + slot));
+      }
+      if constexpr (CLUSTER) {
+        // the cluster's records of a row, added up in rank order by one warp of one CTA
+        const int size = walk.size, rank = walk.rank;
+        const uint32_t recs = smem_addr(s_rec), flag = smem_addr(&s_again[segment & 1]);
+        __syncwarp();
+        dec_cluster_sync();
+        bool redo = false;
+        if (lane < size) {
+          int x;
+          asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(dec_map(flag, lane)) : "memory");
+          redo = x == (int)segment + 1;
+        }
+        redo = __any_sync(0xffffffffu, redo);
+        s.k0 = 0; s.k1 = s.item.n;
+        for (int row = rank + warp * size; row < rows; row += DEC_WARPS * size) {
+          if (redo) {
+            const PagedSegment copy = s;
+            paged_slow_row<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, cta);
+            continue;
+          }
+          const uint32_t at = recs + (uint32_t)row * RDKV_PARTIAL_STRIDE * 4u;
+          float4 ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+          if (lane < size) ml = dec_remote4(dec_map(at, lane));
+          const float M = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
+          const float L = warp_sum(ml.y * f);
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int x0 = 0; x0 < size; x0 += 8) {             // (clusters are of 8 or 16)
+            float4 p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = dec_remote4(dec_map(at + 16u + 16u * lane, x0 + e));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float w = __shfl_sync(0xffffffffu, f, x0 + e);
+              sum.x = fmaf(p[e].x, w, sum.x); sum.y = fmaf(p[e].y, w, sum.y); sum.z = fmaf(p[e].z, w, sum.z); sum.w = fmaf(p[e].w, w, sum.w);
+            }
+          }
+          const PagedRow d = paged_row<DEC_ROWS>(A, s, row, cta);
+          if (d.rec != nullptr) {
+            *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = sum;
+            if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4((M - LIFT) * PAGED_LN2, L, 0.f, 0.f);
+          } else {
+            const float w = paged_over(L);
+            *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(sum.x * w, sum.y * w), paged_pack<BF16>(sum.z * w, sum.w * w));
+          }
+        }
+        __syncwarp();
+        dec_cluster_sync();                                  // (records stay until everybody has read them)
       }
       ++segment;
     }
   }
   __syncthreads();
+  paged_zero_padding(A, DEC_THREADS);
   if (tid == 0) A.status[cta] = s_trouble;
 }
 
 int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  // Few items: a cluster each, as long as eight CTAs an item fit the GPU at once.  (One request of 1061 tokens, 8 heads: see above.)
+  const int64_t items = (int64_t)A.S * A.H_kv;
+  if (items > 0 && items * 8 <= PAGED_DECODE_CTAS) {
+    const int size = items * 16 <= PAGED_DECODE_CTAS ? 16 : 8;
+    auto go = [&](auto kernel) -> int {
+      cudaError_t e = allow_dynamic_smem(kernel, DEC_SMEM);
+      if (e == cudaSuccess && size > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)size; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+      cfg.gridDim = dim3((unsigned)(items * size)); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = DEC_SMEM;
+      if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, A, tm_k, tm_v);
+      if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
+      return launch_status();
+    };
+    return bf16 ? go(paged_decode_kernel<true, true>) : go(paged_decode_kernel<false, true>);
+  }
   auto go = [&](auto kernel, auto join) -> int {
     const cudaError_t e = allow_dynamic_smem(kernel, DEC_SMEM);
     if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
@@ -331,8 +459,8 @@ int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, 
     if (rc != RDKV_OK) return rc;
     return paged_launch_join(join, A, dim3(PAGED_DECODE_CTAS - 1, DEC_ROWS / PAGED_JOIN_WARPS), st);
   };
-  if (bf16) return go(paged_decode_kernel<true>, paged_join_kernel<true, DEC_KEYS, DEC_ROWS, PAGED_DECODE_CTAS>);
-  return go(paged_decode_kernel<false>, paged_join_kernel<false, DEC_KEYS, DEC_ROWS, PAGED_DECODE_CTAS>);
+  if (bf16) return go(paged_decode_kernel<true, false>, paged_join_kernel<true, DEC_ROWS, PAGED_DECODE_CTAS>);
+  return go(paged_decode_kernel<false, false>, paged_join_kernel<false, DEC_ROWS, PAGED_DECODE_CTAS>);
 }
 
 }  // namespace rdkv

@@ -40,7 +40,7 @@ struct PagedArgs {
   uint16_t* out; int64_t o_tok, o_head; int zero_pad;
   float* rec;                                     // [T][H_q][132] instead of out
   // workspace
-  int4* place;                                    // [G+1] where CTA c starts: request, head, group, tile
+  int4* place;                                    // [G+1][2] where CTA c starts: request, head, group, tile; the item's tiles, rows, first query row
   int* status;                                    // [G] 1: a wait of the CTA ran out
   float* part;                                    // [2 G][rows of an item][132] records of cut items
 };
@@ -111,7 +111,7 @@ __device__ __forceinline__ int paged_tile(const PagedItem& it, int k) { return k
 // ── the line of units ───────────────────────────────────────────────────────
 struct PagedPlace { int i, head, group, tile; };  // i = S: the end
 
-struct PagedPlaceScratch { uint64_t part[32]; uint64_t at[2], width[2]; int request[2]; int4 found[2]; };
+struct PagedPlaceScratch { uint64_t part[32]; uint64_t at[2], width[2]; int request[2]; int4 found[2], item; };
 
 // Where the parts of CTA c of G start and end.  All threads of the block (NT, whole warps) call it.  FIXED: cost of an item besides its
 // tiles; a cut that would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.
@@ -187,7 +187,8 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
       const int groups = paged_groups(A, r), head = (int)(s.at[warp] / s.width[warp]);
       uint32_t left = (uint32_t)(s.at[warp] - (uint64_t)head * s.width[warp]);
       for (int x0 = 0; x0 < groups; x0 += 32) {
-        const int n = x0 + lane < groups ? paged_item<KEYS>(A, r, x0 + lane).n : 0;
+        const PagedItem it = paged_item<KEYS>(A, r, min(x0 + lane, groups - 1));
+        const int n = it.n;
         const uint32_t cost = x0 + lane < groups ? n + FIXED : 0;
         uint32_t incl = cost;
 #pragma unroll
@@ -202,6 +203,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
             if (tile < SNAP) tile = 0;
             else if (n - tile < SNAP) tile = n;
             s.found[warp] = make_int4(i, head, x0 + lane, tile);
+            if (warp == 0) s.item = make_int4(n, it.n_tok * A.g, it.tok0, 0);
           }
           break;
         }
@@ -209,6 +211,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
       }
     } else if (lane == 0) {
       s.found[warp] = found;
+      if (warp == 0) s.item = make_int4(0, 0, 0, 0);
     }
   }
   __syncthreads();
@@ -216,8 +219,8 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
   from = {f.x, f.y, f.z, f.w};
   to = {t.x, t.y, t.z, t.w};
   if (tid == 0) {
-    A.place[c] = f;
-    if (c == G - 1) A.place[G] = make_int4(A.S, 0, 0, 0);
+    A.place[2 * c] = f; A.place[2 * c + 1] = s.item;
+    if (c == G - 1) A.place[2 * G] = make_int4(A.S, 0, 0, 0);
   }
 }
 
@@ -335,69 +338,74 @@ __device__ __forceinline__ void paged_zero_padding(const PagedArgs& A, int n_thr
 }
 
 // Joins the records of items that a cut went through.  Block (c, y): if the cut in front of CTA c is the first one inside an
-// item, rows y, y + gridDim.y * 8, ... of that item, a warp each.
+// item, rows y, y + gridDim.y * 8, ... of that item, a warp each.  Its loads are three round trips: the places, the parts' m
+// and l together with the first parts' sums, the rest.
 constexpr int PAGED_JOIN_WARPS = 8;
-template <bool BF16, int KEYS, int ROWS, int G>
+template <bool BF16, int ROWS, int G>
 __global__ void __launch_bounds__(PAGED_JOIN_WARPS * 32)
 paged_join_kernel(const PagedArgs A) {
   __shared__ float s_w[PAGED_JOIN_WARPS][G];
-  __shared__ uint8_t s_some[G];
-  wait_for_previous_kernel();
+  __shared__ uint8_t s_some[G + 1];                          // [0] the CTA in front of the cut
   const int c = blockIdx.x + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int4 at = A.place[c], prev = A.place[c - 1];
-  if (at.x >= A.S || at.w == 0) return;
-  PagedSegment s;
-  s.request = paged_request(A, at.x);
-  s.item = paged_item<KEYS>(A, s.request, at.z);
-  s.i = at.x; s.head = at.y; s.group = at.z; s.k0 = 0; s.k1 = s.item.n;
-  if (at.w >= s.item.n) return;
+  wait_for_previous_kernel();
+  const int4 at = A.place[2 * c], item = A.place[2 * c + 1], prev = A.place[2 * c - 2];
+  int4 a = A.place[2 * min(c + tid, G)], b = A.place[2 * min(c + tid + 1, G)];
+  if (at.x >= A.S || at.w == 0 || at.w >= item.x) return;
   if (prev.x == at.x && prev.y == at.y && prev.z == at.z && prev.w > 0) return;   // an earlier cut is in this item
   // the CTAs from c on that start inside the item (a run), and which of them have tiles of it
-  int n_more = 0;
-  for (int base = c; base < G; base += PAGED_JOIN_WARPS * 32) {
+  int n_parts = 1;
+  for (int base = c;; base += PAGED_JOIN_WARPS * 32) {
     const int x = base + tid;
-    bool in = false;
-    if (x < G) {
-      const int4 a = A.place[x], b = A.place[x + 1];
-      in = a.x == at.x && a.y == at.y && a.z == at.z && a.w > 0 && a.w < s.item.n;
-      s_some[x - c] = in && !(b.x == at.x && b.y == at.y && b.z == at.z && b.w == a.w);
-    }
+    const bool in = x < G && a.x == at.x && a.y == at.y && a.z == at.z && a.w > 0 && a.w < item.x;
+    if (x < G) s_some[x - c + 1] = in && !(b.x == at.x && b.y == at.y && b.z == at.z && b.w == a.w);
     const int n = __syncthreads_count(in);
-    n_more += n;
+    n_parts += n;
     if (n < PAGED_JOIN_WARPS * 32) break;
+    a = A.place[2 * min(x + PAGED_JOIN_WARPS * 32, G)]; b = A.place[2 * min(x + PAGED_JOIN_WARPS * 32 + 1, G)];
   }
-  const int n_parts = 1 + n_more, rows = s.item.n_tok * A.g;
+  if (tid == 0) s_some[0] = 1;
+  __syncthreads();
+  PagedSegment s;
+  s.item.tok0 = item.z; s.item.n = item.x; s.head = at.y; s.k0 = 0; s.k1 = item.x;
   // record of part x (0: the CTA in front of the cut, its last segment; others: the first segment of CTA c + x - 1)
   auto record = [&](int x, int row) {
     return A.part + ((int64_t)(x == 0 ? 2 * (c - 1) + 1 : 2 * (c + x - 1)) * ROWS + row) * RDKV_PARTIAL_STRIDE;
   };
-  for (int row = blockIdx.y * PAGED_JOIN_WARPS + warp; row < rows; row += gridDim.y * PAGED_JOIN_WARPS) {
-    float M = -INFINITY;
+  auto sums = [&](int x, int row) {
+    return x < n_parts && s_some[x] ? *reinterpret_cast<const float4*>(record(x, row) + 4 + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  for (int row = blockIdx.y * PAGED_JOIN_WARPS + warp; row < item.y; row += gridDim.y * PAGED_JOIN_WARPS) {
+    constexpr int EARLY = 8;
+    float4 p[EARLY];
+#pragma unroll
+    for (int e = 0; e < EARLY; ++e) p[e] = sums(e, row);
+    float M = -INFINITY, L = 0.f, l0 = 0.f;
     for (int x = lane; x < n_parts; x += 32) {
-      const float m = x == 0 || s_some[x - 1] ? record(x, row)[0] : -INFINITY;
-      s_w[warp][x] = m;
-      M = fmaxf(M, m);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (s_some[x]) ml = *reinterpret_cast<const float2*>(record(x, row));
+      if (x == lane) l0 = ml.y;
+      s_w[warp][x] = ml.x;
+      M = fmaxf(M, ml.x);
     }
     M = warp_max(M);
-    float L = 0.f;
     for (int x = lane; x < n_parts; x += 32) {
-      const float m = s_w[warp][x];
-      float w = 0.f;
-      if (x == 0 || s_some[x - 1]) {
-        w = m == -INFINITY ? 0.f : exp2_approx((m - M) * PAGED_LOG2E);
-        L = fmaf(record(x, row)[1], w, L);
-      }
+      const float m = s_w[warp][x], w = m == -INFINITY ? 0.f : exp2_approx((m - M) * PAGED_LOG2E);
+      const float l = x == lane ? l0 : s_some[x] ? record(x, row)[1] : 0.f;
+      L = fmaf(l, w, L);
       s_w[warp][x] = w;
     }
     L = warp_sum(L);
     __syncwarp();
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int x = 0; x < n_parts; ++x) {
-      const float w = s_w[warp][x];
-      if (x > 0 && !s_some[x - 1]) continue;
-      const float4 p = *reinterpret_cast<const float4*>(record(x, row) + 4 + 4 * lane);
-      o.x = fmaf(p.x, w, o.x); o.y = fmaf(p.y, w, o.y); o.z = fmaf(p.z, w, o.z); o.w = fmaf(p.w, w, o.w);
+    for (int x0 = 0; x0 < n_parts; x0 += EARLY) {
+#pragma unroll
+      for (int e = 0; e < EARLY; ++e) {
+        const float w = x0 + e < n_parts ? s_w[warp][x0 + e] : 0.f;
+        o.x = fmaf(p[e].x, w, o.x); o.y = fmaf(p[e].y, w, o.y); o.z = fmaf(p[e].z, w, o.z); o.w = fmaf(p[e].w, w, o.w);
+      }
+      if (x0 + EARLY < n_parts)
+#pragma unroll
+        for (int e = 0; e < EARLY; ++e) p[e] = sums(x0 + EARLY + e, row);
     }
     const PagedRow d = paged_row<ROWS>(A, s, row, 0);
     if (d.rec != nullptr) {
@@ -432,11 +440,11 @@ inline bool paged_map(CUtensorMap* tm, const void* base, bool bf16, int64_t page
 
 // Workspace of a launch of G CTAs whose items have up to `rows` rows.
 inline int64_t paged_workspace_bytes(int G, int rows) {
-  return (int64_t)(G + 1) * 16 + (((int64_t)G * 4 + 15) / 16) * 16 + (int64_t)2 * G * rows * RDKV_PARTIAL_STRIDE * 4;
+  return (int64_t)(G + 1) * 32 + (((int64_t)G * 4 + 15) / 16) * 16 + (int64_t)2 * G * rows * RDKV_PARTIAL_STRIDE * 4;
 }
 inline void paged_workspace(PagedArgs* A, void* workspace, int G) {
   char* p = static_cast<char*>(workspace);
-  A->place = reinterpret_cast<int4*>(p); p += (int64_t)(G + 1) * 16;
+  A->place = reinterpret_cast<int4*>(p); p += (int64_t)(G + 1) * 32;
   A->status = reinterpret_cast<int*>(p); p += (((int64_t)G * 4 + 15) / 16) * 16;
   A->part = reinterpret_cast<float*>(p);
 }

@@ -384,7 +384,6 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   let_next_kernel_start();
-  paged_zero_padding(A, CH_THREADS);
   tmem_fence_before();
   PagedPlace from, to;
   paged_place<CH_KEYS, CH_THREADS, CH_FIXED, CH_SNAP>(A, cta, PAGED_CHUNK_CTAS, s_place, from, to);   // (its barriers order the set-up too)
@@ -407,6 +406,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   __syncthreads();
   tmem_fence_after();
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  paged_zero_padding(A, CH_THREADS);
   if (tid == 0) A.status[cta] = s_trouble;
 }
 
@@ -440,8 +440,8 @@ int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, c
     if (rc != RDKV_OK) return rc;
     return paged_launch_join(join, A, dim3(PAGED_CHUNK_CTAS - 1, 8), st);
   };
-  if (bf16) return go(paged_chunk_kernel<true>, paged_join_kernel<true, CH_KEYS, CH_ROWS, PAGED_CHUNK_CTAS>);
-  return go(paged_chunk_kernel<false>, paged_join_kernel<false, CH_KEYS, CH_ROWS, PAGED_CHUNK_CTAS>);
+  if (bf16) return go(paged_chunk_kernel<true>, paged_join_kernel<true, CH_ROWS, PAGED_CHUNK_CTAS>);
+  return go(paged_chunk_kernel<false>, paged_join_kernel<false, CH_ROWS, PAGED_CHUNK_CTAS>);
 }
 
 }  // namespace rdkv

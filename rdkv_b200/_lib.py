@@ -230,6 +230,25 @@ def stream_ptr(device=None) -> int:
     return torch._C._cuda_getCurrentRawStream(current)     # (the handle alone: a Stream object costs 5 us more)
 
 
+def raw_stream(index: int) -> int:
+    """:func:`stream_ptr` for a device number, without the detours (calls that a step makes in every layer)."""
+    if index != torch._C._cuda_getDevice():
+        stream_ptr(torch.device("cuda", index))            # (raises, with the reason)
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class CallCache(dict):
+    """What the checks of a call worked out from the shapes, strides, types and devices of its arguments, under just
+    those: the next call of the same kind skips the checks.  Nothing of the arguments' contents, addresses or identity."""
+    MOST = 256
+
+    def remember(self, key, value):
+        if len(self) >= self.MOST:                         # (a caller that keeps changing its shapes)
+            self.clear()
+        self[key] = value
+        return value
+
+
 def q_dtype_tag(t: torch.Tensor) -> int:
     if t.dtype == torch.float16:
         return RDKV_F16

@@ -24,10 +24,11 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import HEAD_DIM, PARTIAL_STRIDE, check, lib, q_dtype_tag, require_cuda, stream_ptr
-from .rope import _axes_args
+from ._lib import HEAD_DIM, PARTIAL_STRIDE, CallCache, check, lib, q_dtype_tag, raw_stream, require_cuda
+from .rope import axes_check
 
 MAX_REQUESTS = 16384
+_TABLES_CALLS, _APPEND_CALLS, _ATTENTION_CALLS = CallCache(), CallCache(), CallCache()
 
 
 class PagedPlan(NamedTuple):
@@ -66,42 +67,52 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
     A page that is not to be had (the free list is used up: entry -1; the table is too narrow: no entry) leaves its
     tokens without a slot (-1): :func:`append_kv` does not write them and :func:`paged_attention` does not see them.
     ``missing`` counts such pages.  ``out``: a plan of the same S and n_tokens to write into (for captured steps)."""
-    _int32(ctx_lens, "ctx_lens", 1); _int32(new_lens, "new_lens", 1); _int32(block_tables, "block_tables", 2)
-    _int32(free_pages, "free_pages", 1)
-    S, T, dev = ctx_lens.shape[0], int(n_tokens), ctx_lens.device
-    if new_lens.shape[0] != S or block_tables.shape[0] != S:
-        raise ValueError(f"new_lens and block_tables must have {S} rows, got {new_lens.shape[0]} and {block_tables.shape[0]}")
-    if S > MAX_REQUESTS:
-        raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
-    if page_size < 1 or T < 0:
-        raise ValueError(f"bad page_size {page_size} or n_tokens {n_tokens}")
-    if S > 1 and block_tables.shape[1] > 0 and block_tables.stride(0) < block_tables.shape[1]:
-        raise ValueError("rows of block_tables overlap")
-    if free_start is not None:
-        _int32(free_start, "free_start", 1)
-        if free_start.shape[0] != 1:
-            raise ValueError("free_start must have one element")
-    _same_device(dev, new_lens=new_lens, block_tables=block_tables, free_pages=free_pages, free_start=free_start)
+    n_tokens, page_size = int(n_tokens), int(page_size)
+    key = (ctx_lens.shape, ctx_lens.stride(), ctx_lens.dtype, ctx_lens.get_device(), new_lens.shape, new_lens.stride(), new_lens.dtype,
+           new_lens.get_device(), block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.get_device(), free_pages.shape,
+           free_pages.stride(), free_pages.dtype, free_pages.get_device(), page_size, n_tokens,
+           None if free_start is None else (free_start.shape, free_start.dtype, free_start.get_device()))
+    call = _TABLES_CALLS.get(key)
+    if call is None:
+        _int32(ctx_lens, "ctx_lens", 1); _int32(new_lens, "new_lens", 1); _int32(block_tables, "block_tables", 2)
+        _int32(free_pages, "free_pages", 1)
+        S, dev = ctx_lens.shape[0], ctx_lens.device
+        if new_lens.shape[0] != S or block_tables.shape[0] != S:
+            raise ValueError(f"new_lens and block_tables must have {S} rows, got {new_lens.shape[0]} and {block_tables.shape[0]}")
+        if S > MAX_REQUESTS:
+            raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
+        if page_size < 1 or n_tokens < 0:
+            raise ValueError(f"bad page_size {page_size} or n_tokens {n_tokens}")
+        if S > 1 and block_tables.shape[1] > 0 and block_tables.stride(0) < block_tables.shape[1]:
+            raise ValueError("rows of block_tables overlap")
+        if free_start is not None:
+            _int32(free_start, "free_start", 1)
+            if free_start.shape[0] != 1:
+                raise ValueError("free_start must have one element")
+        _same_device(dev, new_lens=new_lens, block_tables=block_tables, free_pages=free_pages, free_start=free_start)
+        call = _TABLES_CALLS.remember(key, (S, (block_tables.stride(0), block_tables.shape[1]), free_pages.shape[0], dev.index))
+    S, table, n_free, index = call
     if out is None:
-        ints = torch.empty(T + 2 * S + 3, dtype=torch.int32, device=dev)
-        positions, q_start, kv_lens, free_next, missing = ints.split((T, S + 1, S, 1, 1))
-        out = PagedPlan(torch.empty(T, dtype=torch.int64, device=dev), positions, q_start, kv_lens, free_next, missing)
+        ints = ctx_lens.new_empty(n_tokens + 2 * S + 3)
+        out = PagedPlan(ctx_lens.new_empty(n_tokens, dtype=torch.int64), *ints.split_with_sizes((n_tokens, S + 1, S, 1, 1)))
     else:
-        for name, n in (("positions", T), ("q_start", S + 1), ("kv_lens", S), ("free_next", 1), ("missing", 1)):
+        for name, n in (("positions", n_tokens), ("q_start", S + 1), ("kv_lens", S), ("free_next", 1), ("missing", 1)):
             t = getattr(out, name)
             _int32(t, f"out.{name}", 1)
             if t.shape[0] != n:
                 raise ValueError(f"out.{name} must have {n} elements")
-        if out.slot_map.dtype != torch.int64 or tuple(out.slot_map.shape) != (T,) or not out.slot_map.is_contiguous():
-            raise ValueError(f"out.slot_map must be a contiguous int64 tensor of {T} elements")
-        _same_device(dev, **{f"out.{n}": t for n, t in out._asdict().items()})
+        if out.slot_map.dtype != torch.int64 or tuple(out.slot_map.shape) != (n_tokens,) or not out.slot_map.is_contiguous():
+            raise ValueError(f"out.slot_map must be a contiguous int64 tensor of {n_tokens} elements")
+        _same_device(ctx_lens.device, **{f"out.{n}": t for n, t in out._asdict().items()})
         if free_start is not None and out.free_next.data_ptr() == free_start.data_ptr():
             raise ValueError("out.free_next must not be free_start itself (other blocks of the launch still read it)")
-    check(lib().rdkv_paged_tables(
-        ctx_lens.data_ptr(), new_lens.data_ptr(), S, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
-        free_pages.data_ptr(), free_pages.shape[0], None if free_start is None else free_start.data_ptr(), int(page_size), T,
-        out.slot_map.data_ptr(), out.positions.data_ptr(), out.q_start.data_ptr(), out.kv_lens.data_ptr(), out.free_next.data_ptr(),
-        out.missing.data_ptr(), stream_ptr(dev)), "rdkv_paged_tables")
+    slot_map, positions, q_start, kv_lens, free_next, missing = out
+    status = lib().rdkv_paged_tables(
+        ctx_lens.data_ptr(), new_lens.data_ptr(), S, block_tables.data_ptr(), *table, free_pages.data_ptr(), n_free,
+        None if free_start is None else free_start.data_ptr(), page_size, n_tokens, slot_map.data_ptr(), positions.data_ptr(),
+        q_start.data_ptr(), kv_lens.data_ptr(), free_next.data_ptr(), missing.data_ptr(), raw_stream(index))
+    if status:
+        check(status, "rdkv_paged_tables")
     return out
 
 
@@ -126,6 +137,29 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     [T]: slot of every token; a slot below zero or behind the last page is not written.  The slots of a call must
     differ from one another.  q [T,H_q,128] of the same dtype goes to ``q_out`` (default: a new tensor; may be q
     itself), which is returned; k is not changed.  positions [T] or [axes,T], inv_freq and sections: see ``rope_axes``."""
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), k_pages.shape, k_pages.stride(),
+           k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype, v_pages.get_device(), slot_map.shape,
+           slot_map.stride(), slot_map.dtype, slot_map.get_device(), None if sections is None else tuple(sections),
+           None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.get_device()),
+           None if inv_freq is None else (inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.get_device()),
+           None if q is None else (q.shape, q.stride(), q.dtype, q.get_device()),
+           None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device()))
+    call = _APPEND_CALLS.get(key)
+    if call is None:
+        call = _APPEND_CALLS.remember(key, _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sections, q_out))
+    ks, vs, kps, vps, qs, qos, ax, sec, index = call
+    status = lib().rdkv_paged_append(
+        k.data_ptr(), *ks, v.data_ptr(), *vs, k_pages.data_ptr(), *kps, v_pages.data_ptr(), *vps, slot_map.data_ptr(),
+        None if q is None else q.data_ptr(), *qs, None if q is None else q_out.data_ptr(), *qos,
+        None if positions is None else positions.data_ptr(), *ax, None if positions is None else inv_freq.data_ptr(), *sec, raw_stream(index))
+    if status:
+        check(status, "rdkv_paged_append")
+    return q_out
+
+
+def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sections, q_out):
     require_cuda(k, "k"); require_cuda(v, "v"); require_cuda(slot_map, "slot_map")
     _check_pages(k_pages, v_pages)
     n_pages, H_kv, page_size, _ = k_pages.shape
@@ -141,30 +175,21 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     tag = q_dtype_tag(k)
     if (positions is None) != (inv_freq is None) or (positions is None and (q is not None or sections is not None)):
         raise ValueError("q and sections need positions and inv_freq; positions needs inv_freq")
-    if positions is None:
-        rot = (None, 0, 0, None, None, 0)
-    else:
-        rot = _axes_args(positions, inv_freq, sections, T, dev)
+    axes = (0, 0, None, 0) if positions is None else axes_check(positions, inv_freq, sections, T, dev)
+    qs, qos = (0, 0), (0, 0, 0)
     if q is None:
         if q_out is not None:
             raise ValueError("q_out needs q")
-        q_args = (None, 0, 0, None, 0, 0, 0)
     else:
         require_cuda(q, "q")
         if q.dim() != 3 or q.shape[0] != T or q.shape[2] != HEAD_DIM or q.dtype != k.dtype or q.stride(2) != 1:
             raise ValueError(f"q must be [{T},H_q,{HEAD_DIM}] {k.dtype} with contiguous rows, got {tuple(q.shape)} {q.dtype}")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
+        if q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
             raise ValueError("q_out must have q's shape and dtype and contiguous rows")
-        q_args = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1])
+        qs, qos = q.stride()[:2], (*q_out.stride()[:2], q.shape[1])
     _same_device(dev, v=v, k_pages=k_pages, v_pages=v_pages, slot_map=slot_map, q=q, q_out=q_out)
-    ks, vs = k_pages.stride(), v_pages.stride()
-    check(lib().rdkv_paged_append(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), H_kv, tag, T, k_pages.data_ptr(), ks[0], ks[1],
-        ks[2], v_pages.data_ptr(), vs[0], vs[1], vs[2], n_pages, page_size, slot_map.data_ptr(), *q_args, *rot, stream_ptr(dev)),
-        "rdkv_paged_append")
-    return q_out
+    return (k.stride()[:2], (*v.stride()[:2], H_kv, tag, T), k_pages.stride()[:3], (*v_pages.stride()[:3], n_pages, page_size), qs, qos,
+            axes[:2], axes[2:], dev.index)
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: Tensor, q_start: Tensor, kv_lens: Tensor, *,
@@ -185,13 +210,54 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     Returns ``out`` [T,H_q,128] in q's dtype.  Tokens behind the last request's are padding: zero in an ``out`` that the
     call allocates, left as they were in one that it is given.  ``out_partial`` float32 [T*H_q,132] receives
     un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape,
+           v_pages.stride(), v_pages.dtype, v_pages.get_device(), block_tables.shape, block_tables.stride(), block_tables.dtype,
+           block_tables.get_device(), q_start.shape, q_start.stride(), q_start.dtype, q_start.get_device(), kv_lens.shape, kv_lens.stride(),
+           kv_lens.dtype, kv_lens.get_device(), max_new, window, sinks, scale)
+    call = _ATTENTION_CALLS.get(key)
+    if call is None:
+        call = _ATTENTION_CALLS.remember(key, _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_new, window, sinks, scale))
+    qs, ks, vs, shape, table, numbers, n_ws, index, tail = call
+    if not qs or q.data_ptr() & 15:                        # (rows that no 16-byte copy can fetch)
+        q = q.clone(memory_format=torch.contiguous_format)
+        qs = (*q.stride()[:2], *tail)
+    k_ptr, v_ptr = k_pages.data_ptr(), v_pages.data_ptr()
+    if (k_ptr | v_ptr) & 15:
+        raise ValueError("k_pages and v_pages must start on 16 bytes")
+    if out_partial is None:
+        zero = 0
+        if out is None:
+            out, zero = torch.empty_like(q, memory_format=torch.contiguous_format), 1
+        else:
+            require_cuda(out, "out")
+            if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() % 16
+                    or out.stride(0) % 8 or out.stride(1) % 8):
+                raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} on {q.device} with contiguous rows on 16 bytes")
+        os, out_ptr, rec_ptr = out.stride(), out.data_ptr(), None
+    else:
+        if out is not None:
+            raise ValueError("either out or out_partial")
+        require_cuda(out_partial, "out_partial")
+        if (out_partial.dtype != torch.float32 or not out_partial.is_contiguous() or out_partial.device != q.device
+                or out_partial.numel() != q.shape[0] * q.shape[1] * PARTIAL_STRIDE):
+            raise ValueError(f"out_partial must be contiguous float32 [{q.shape[0] * q.shape[1]},{PARTIAL_STRIDE}] on {q.device}")
+        os, out_ptr, rec_ptr, zero = (0, 0), None, out_partial.data_ptr(), 0
+    ws = kv_lens.new_empty(n_ws)
+    status = lib().rdkv_paged_attention(
+        q.data_ptr(), *qs, k_ptr, *ks, v_ptr, *vs, *shape, block_tables.data_ptr(), *table, q_start.data_ptr(), kv_lens.data_ptr(), *numbers,
+        out_ptr, os[0], os[1], zero, rec_ptr, ws.data_ptr(), 4 * n_ws, raw_stream(index))
+    if status:
+        check(status, "rdkv_paged_attention")
+    return out if out_partial is None else out_partial
+
+
+def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_new, window, sinks, scale):
     require_cuda(q, "q")
     _check_pages(k_pages, v_pages)
     n_pages, H_kv, page_size, _ = k_pages.shape
     if q.dim() != 3 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be [T,H_q,{HEAD_DIM}], got {tuple(q.shape)}")
     T, H_q, _ = q.shape
-    dev = q.device
     if q.dtype != k_pages.dtype or q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"q and the pages must both be fp16 or both bf16, got {q.dtype} and {k_pages.dtype}")
     if H_kv < 1 or H_q % H_kv or not 1 <= H_q // H_kv <= 16:
@@ -206,38 +272,18 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
         raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError("window and sinks must not be negative, and sinks need a window")
-    if scale is not None and not scale > 0:
+    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    if not scale > 0:
         raise ValueError(f"scale must be positive, got {scale}")
     max_new = T if max_new is None else min(int(max_new), T)
     if max_new < 0:
         raise ValueError("max_new must not be negative")
-    if q.stride(2) != 1 or q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
-        q = q.clone(memory_format=torch.contiguous_format)
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16 or any(x % 8 for x in ks[:3] + vs[:3]):
-        raise ValueError("k_pages and v_pages must start on 16 bytes and have strides of whole 16 bytes")
-    allocated = False
-    if out_partial is not None:
-        if out is not None:
-            raise ValueError("either out or out_partial")
-        require_cuda(out_partial, "out_partial")
-        if out_partial.dtype != torch.float32 or not out_partial.is_contiguous() or out_partial.numel() != T * H_q * PARTIAL_STRIDE:
-            raise ValueError(f"out_partial must be contiguous float32 [{T * H_q},{PARTIAL_STRIDE}]")
-        o_args = (None, 0, 0, 0, out_partial.data_ptr())
-    else:
-        if out is None:
-            out, allocated = torch.empty((T, H_q, HEAD_DIM), dtype=q.dtype, device=dev), True
-        require_cuda(out, "out")
-        if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8:
-            raise ValueError(f"out must be {q.dtype} [{T},{H_q},{HEAD_DIM}] with contiguous rows on 16 bytes")
-        o_args = (out.data_ptr(), out.stride(0), out.stride(1), 1 if allocated else 0, None)
-    _same_device(dev, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, q_start=q_start, kv_lens=kv_lens, out=out,
-                 out_partial=out_partial)
-    n_ws = lib().rdkv_paged_attention_workspace(S, T, H_q, H_kv, max_new)
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws > 0 else None
-    check(lib().rdkv_paged_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), q_dtype_tag(q), T, H_q, k_pages.data_ptr(), ks[0], ks[1], ks[2], v_pages.data_ptr(), vs[0],
-        vs[1], vs[2], n_pages, H_kv, page_size, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
-        q_start.data_ptr(), kv_lens.data_ptr(), S, max_new, int(window), int(sinks), HEAD_DIM ** -0.5 if scale is None else float(scale),
-        *o_args, None if ws is None else ws.data_ptr(), n_ws, stream_ptr(dev)), "rdkv_paged_attention")
-    return out if out_partial is None else out_partial
+    ks, vs = k_pages.stride()[:3], v_pages.stride()[:3]
+    if any(x % 8 for x in ks + vs):
+        raise ValueError("k_pages and v_pages must have strides of whole 16 bytes")
+    _same_device(q.device, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, q_start=q_start, kv_lens=kv_lens)
+    tail = (q_dtype_tag(q), T, H_q)
+    qs = () if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 else (*q.stride()[:2], *tail)
+    n_ws = -(-lib().rdkv_paged_attention_workspace(S, T, H_q, H_kv, max_new) // 4)
+    return (qs, ks, vs, (n_pages, H_kv, page_size), (block_tables.stride(0), block_tables.shape[1]), (S, max_new, int(window), int(sinks), scale),
+            n_ws, q.device.index, tail)

@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import HEAD_DIM, check, lib, ptr, q_dtype_tag, require_cuda, stream_ptr
+from ._lib import HEAD_DIM, CallCache, check, lib, ptr, q_dtype_tag, raw_stream, require_cuda, stream_ptr
 
 
 def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
@@ -36,17 +36,17 @@ def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
     return q, k
 
 
-_SECTIONS = {}                                             # section sizes -> the C array handed to the library
+_AXES_TAG = {torch.int32: 0, torch.int64: 1}
 
 
-def _axes_args(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[int]], T: int, dev):
-    """(positions, axis stride, 64 bits?, inv_freq, sections, axes) of a call, as the library takes them."""
+def axes_check(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[int]], T: int, dev):
+    """(axis stride, 64-bit positions, C array of the sections, axes) of a call, as the library takes them."""
     half = HEAD_DIM // 2
     require_cuda(positions, "positions"); require_cuda(inv_freq, "inv_freq")
     n_axes = 1 if positions.dim() == 1 else positions.shape[0]
     if positions.dim() not in (1, 2) or positions.shape[-1] != T or not 1 <= n_axes <= 4 or (T > 1 and positions.stride(-1) != 1):
         raise ValueError(f"positions must be [{T}] or [1 to 4 axes,{T}] with contiguous rows, got {tuple(positions.shape)}")
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype not in _AXES_TAG:
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
     if inv_freq.dtype != torch.float32 or tuple(inv_freq.shape) != (half,) or not inv_freq.is_contiguous():
         raise ValueError(f"inv_freq must be a contiguous float32 tensor of {half} elements")
@@ -56,18 +56,12 @@ def _axes_args(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[
         if n_axes != 1:
             raise ValueError("positions of several axes need sections")
         sections = (half,)
-    sections = tuple(sections)
-    sec = _SECTIONS.get(sections)
-    if sec is None:
-        if any(int(n) != n or n < 0 for n in sections) or sum(sections) != half:
-            raise ValueError(f"sections must be whole numbers that add up to {half}, got {sections}")
-        if len(_SECTIONS) >= 64:
-            _SECTIONS.clear()
-        sec = _SECTIONS[sections] = (C.c_int * len(sections))(*(int(n) for n in sections))
-    if len(sections) != n_axes:
-        raise ValueError(f"{len(sections)} sections for {n_axes} axes")
-    return (positions.data_ptr(), 0 if n_axes == 1 else positions.stride(0), 1 if positions.dtype == torch.int64 else 0,
-            inv_freq.data_ptr(), sec, n_axes)
+    if any(int(n) != n or n < 0 for n in sections) or sum(sections) != half or len(sections) != n_axes:
+        raise ValueError(f"sections must be {n_axes} whole numbers (one an axis) that add up to {half}, got {tuple(sections)}")
+    return (0 if n_axes == 1 else positions.stride(0), _AXES_TAG[positions.dtype], (C.c_int * n_axes)(*(int(n) for n in sections)), n_axes)
+
+
+_ROPE_CALLS = CallCache()
 
 
 def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sections: Optional[Sequence[int]] = None,
@@ -80,21 +74,32 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     lose nothing (below 2^24).  sections: how many of the 64 frequencies each axis owns, in order (text
     with one axis: all of them).  Returns (q_out, k_out): new tensors, or the given ones, which may be q and k
     themselves."""
-    for name, t in (("q", q), ("k", k)):
-        require_cuda(t, name)
-        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
-            raise ValueError(f"{name} must be [T,heads,{HEAD_DIM}] with contiguous rows, got {tuple(t.shape)}")
-    T, dev = q.shape[0], q.device
-    if k.shape[0] != T or k.dtype != q.dtype or k.device != dev:
-        raise ValueError("q and k must have the same tokens, dtype and device")
-    tag = q_dtype_tag(q)
-    rot = _axes_args(positions, inv_freq, sections, T, dev)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if k_out is None else k_out
-    for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if t.shape != x.shape or t.dtype != x.dtype or t.device != dev or t.stride(2) != 1:
-            raise ValueError(f"{name} must have the shape, dtype and device of its input and contiguous rows")
-    check(lib().rdkv_rope_axes(q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1],
-                               k.data_ptr(), k.stride(0), k.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1), k.shape[1],
-                               tag, T, *rot, stream_ptr(dev)), "rdkv_rope_axes")
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), positions.shape, positions.stride(),
+           positions.dtype, positions.get_device(), inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.get_device(),
+           None if sections is None else tuple(sections), q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device(), k_out.shape,
+           k_out.stride(), k_out.dtype, k_out.get_device())
+    call = _ROPE_CALLS.get(key)
+    if call is None:
+        for name, t in (("q", q), ("k", k)):
+            require_cuda(t, name)
+            if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
+                raise ValueError(f"{name} must be [T,heads,{HEAD_DIM}] with contiguous rows, got {tuple(t.shape)}")
+        T, dev = q.shape[0], q.device
+        if k.shape[0] != T or k.dtype != q.dtype or k.device != dev:
+            raise ValueError("q and k must have the same tokens, dtype and device")
+        for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
+            if t.shape != x.shape or t.dtype != x.dtype or t.device != dev or t.stride(2) != 1:
+                raise ValueError(f"{name} must have the shape, dtype and device of its input and contiguous rows")
+        axes = axes_check(positions, inv_freq, sections, T, dev)
+        call = _ROPE_CALLS.remember(key, (q.stride()[:2], (*q_out.stride()[:2], q.shape[1]), k.stride()[:2],
+                                          (*k_out.stride()[:2], k.shape[1], q_dtype_tag(q), T), axes[:2], axes[2:], dev.index))
+    qs, qos, ks, kos, ax, sec, index = call
+    status = lib().rdkv_rope_axes(q.data_ptr(), *qs, q_out.data_ptr(), *qos, k.data_ptr(), *ks, k_out.data_ptr(), *kos, positions.data_ptr(),
+                                  *ax, inv_freq.data_ptr(), *sec, raw_stream(index))
+    if status:
+        check(status, "rdkv_rope_axes")
     return q_out, k_out

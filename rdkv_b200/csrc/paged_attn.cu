@@ -26,7 +26,7 @@ constexpr int DEC_PANEL = DEC_KEYS * 128;         // bytes of 64 keys' 64 channe
 constexpr int DEC_STAGE = 4 * DEC_PANEL;          // K channels 0-63, 64-127, V channels 0-63, 64-127
 constexpr size_t DEC_SMEM = 1024 + (size_t)DEC_STAGES * DEC_STAGE;
 static_assert(DEC_STAGE == DEC_WARPS * DEC_ROWS * 128 * 4, "the warps' results fill a stage");
-constexpr int DEC_FIXED = 2, DEC_SNAP = 1;
+constexpr int DEC_FIXED = 2, DEC_SNAP = 1, DEC_WHOLE = 4;
 
 template <bool BF16>
 __device__ __forceinline__ void dec_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -106,6 +106,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     bar_init_fence();
     s_again[0] = s_again[1] = s_trouble = 0;
   }
+  if (tid == 32) { tma_prefetch_map(&tm_k); tma_prefetch_map(&tm_v); }
   auto begin = [&]() {
     if constexpr (CLUSTER) {
       DecWalk<true> walk(A);
@@ -114,7 +115,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     } else {
       let_next_kernel_start();
       PagedPlace from, to;
-      paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP>(A, cta, PAGED_DECODE_CTAS, s_place, from, to);   // (its barriers order the set-up too)
+      paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP, DEC_WHOLE>(A, cta, PAGED_DECODE_CTAS, s_place, from, to);   // (its barriers order the set-up too)
       return DecWalk<false>(A, from, to);
     }
   };
@@ -123,7 +124,8 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
 
   if (warp == DEC_WARPS) {
     // ── the warp that brings in tiles ──
-    const int rows = min(A.page, DEC_KEYS), per_tile = DEC_KEYS / rows, batch = 32 / per_tile;   // boxes of a tile, tiles of a batch of page numbers
+    // rows of a box, boxes of a tile, tiles of a batch of page numbers: powers of two
+    const int rows_log2 = min(A.page_log2, 6), rows = 1 << rows_log2, per_log2 = 6 - rows_log2, per_tile = 1 << per_log2, batch = 32 >> per_log2;
     const int box = lane >> 2, what = lane & 3;              // this lane's box of a tile: sub-tile, (K | V) x panel
     unsigned count = 0;
     bool ok = true;
@@ -131,14 +133,14 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       if (CLUSTER && !ok) s.k1 = s.k0;
       const int32_t* table = A.table + s.i * A.table_stride;
       auto page_of = [&](int k) {                            // lane's entry of the batch that starts with tile k
-        const int kk = k + lane / per_tile;
+        const int kk = k + (lane >> per_log2);
         if (kk >= s.k1) return -1;
-        const int key = paged_tile(s.item, kk) * DEC_KEYS + (lane % per_tile) * rows;
+        const int key = paged_tile(s.item, kk) * DEC_KEYS + ((lane & (per_tile - 1)) << rows_log2);
         return key < s.item.hi ? table[key >> A.page_log2] : -1;
       };
       int ids = page_of(s.k0), ids_next = -1;
       for (int k = s.k0; k < s.k1; ++k, ++count) {
-        const int in_batch = (k - s.k0) % batch;
+        const int in_batch = (k - s.k0) & (batch - 1);
         if (in_batch == 0) {
           if (k > s.k0) ids = ids_next;
           ids_next = page_of(k + batch);
@@ -151,8 +153,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
         const unsigned lanes = __ballot_sync(0xffffffffu, there);
         if (lane == 0) {
           int mask = 0;
-          for (int b = 0; b < per_tile; ++b)
-            if (lanes >> (4 * b) & 1) mask |= ((1 << (rows / 16)) - 1) << (b * (rows / 16));
+          for (int x = 0; x < 4; ++x) mask |= (int)(lanes >> (4 * (x * 16 >> rows_log2)) & 1u) << x;
           s_info[slot] = make_int2(key0, mask);
           const uint32_t bytes = (uint32_t)__popc(lanes) * (uint32_t)rows * 128u;
           if (bytes > 0) bar_arrive_tx(bar + 8 * slot, bytes);

@@ -66,11 +66,21 @@ int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, c
 constexpr int PAGED_CHUNK_ROWS = 256, PAGED_CHUNK_CTAS = PAGED_SMS, PAGED_CHUNK_KEYS = 128;
 constexpr int PAGED_DECODE_ROWS = 16, PAGED_DECODE_CTAS = 2 * PAGED_SMS, PAGED_DECODE_KEYS = 64;
 
-// Whether one of a pair of 16-bit values is not finite.
+// A pair of 16-bit values: bits 15 and 31 of the result say which of them is not finite (its exponent is all ones: one more carries over).
 template <bool BF16>
-__device__ __forceinline__ bool paged_not_finite(uint32_t x) {
-  constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
-  return (x & E) == E || ((x >> 16) & E) == E;
+__device__ __forceinline__ uint32_t paged_exponent_full(uint32_t x) {
+  return BF16 ? (x & 0x7F807F80u) + 0x00800080u : (x & 0x7C007C00u) + 0x04000400u;
+}
+template <bool BF16>
+__device__ __forceinline__ bool paged_not_finite(uint32_t x) { return (paged_exponent_full<BF16>(x) & 0x80008000u) != 0u; }
+
+// x * y + z of pairs of 16-bit values.
+template <bool BF16>
+__device__ __forceinline__ uint32_t paged_fma2(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t r;
+  if (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
+  return r;
 }
 
 // ── items ───────────────────────────────────────────────────────────────────
@@ -111,21 +121,27 @@ __device__ __forceinline__ int paged_tile(const PagedItem& it, int k) { return k
 // ── the line of units ───────────────────────────────────────────────────────
 struct PagedPlace { int i, head, group, tile; };  // i = S: the end
 
-struct PagedPlaceScratch { uint64_t part[32]; uint64_t at[2], width[2]; int request[2]; int4 found[2], item; };
+struct PagedPlaceScratch { uint64_t part[32]; uint32_t most[32]; uint64_t at[2]; uint32_t width[2]; int request[2]; int4 found[2], item; };
 
 // Where the parts of CTA c of G start and end.  All threads of the block (NT, whole warps) call it.  FIXED: cost of an item besides its
-// tiles; a cut that would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.
-template <int KEYS, int NT, int FIXED, int SNAP>
+// tiles; a cut that would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.  With no more
+// items than CTAs, and none more than WHOLE units over its share, every CTA gets a whole item: a cut costs both its sides
+// an item's records, written and read again.
+template <int KEYS, int NT, int FIXED, int SNAP, int WHOLE>
 __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, PagedPlaceScratch& s, PagedPlace& from, PagedPlace& to) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // units of a head of request i
-  auto units = [&](int i) -> uint32_t {
+  // units of a head of request i, its groups, its costliest item
+  auto units = [&](int i, int& groups, uint32_t& most) -> uint32_t {
     PagedRequest r = {0, 0, 0};
     if (i < A.S) r = paged_request(A, i);
-    const int groups = paged_groups(A, r);
+    groups = paged_groups(A, r);
     uint32_t sum = 0;
+    most = 0;
     if (groups <= 4)
-      for (int x = 0; x < groups; ++x) sum += paged_item<KEYS>(A, r, x).n + FIXED;
+      for (int x = 0; x < groups; ++x) {
+        const uint32_t cost = paged_item<KEYS>(A, r, x).n + FIXED;
+        sum += cost; most = max(most, cost);
+      }
     unsigned many = __ballot_sync(0xffffffffu, groups > 4);   // long chunks: the warp's lanes take their groups
     while (many != 0) {
       const int from_lane = __ffs(many) - 1;
@@ -134,11 +150,14 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
       o.q0 = __shfl_sync(0xffffffffu, r.q0, from_lane); o.n = __shfl_sync(0xffffffffu, r.n, from_lane);
       o.len = __shfl_sync(0xffffffffu, r.len, from_lane);
       const int n = paged_groups(A, o);
-      uint32_t mine = 0;
-      for (int x = lane; x < n; x += 32) mine += paged_item<KEYS>(A, o, x).n + FIXED;
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-      if (lane == from_lane) sum = mine;
+      uint32_t mine = 0, top = 0;
+      for (int x = lane; x < n; x += 32) {
+        const uint32_t cost = paged_item<KEYS>(A, o, x).n + FIXED;
+        mine += cost; top = max(top, cost);
+      }
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == from_lane) { sum = mine; most = top; }
     }
     return sum;
   };
@@ -160,22 +179,40 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
     }
   };
   if (tid < 2) s.request[tid] = A.S;
-  uint64_t total = 0, before = 0, all;
-  uint32_t mine = 0;
+  // units in the low 40 bits, items above them
+  constexpr int BITS = 40;
+  constexpr uint64_t LOW = ((uint64_t)1 << BITS) - 1;
+  uint64_t total = 0, before = 0, all = 0, mine = 0;
+  uint32_t most = 0;
   for (int base = 0; base < A.S; base += NT) {
-    mine = units(base + tid);
+    int groups;
+    uint32_t top;
+    mine = units(base + tid, groups, top);
+    mine |= (uint64_t)groups << BITS;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s.most[warp] = top;
     block_scan(mine, before, all);
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) most = max(most, s.most[w]);
     total += all;
   }
-  total *= (uint64_t)A.H_kv;
-  const uint64_t cut[2] = {(uint64_t)c * total / (uint64_t)G, (uint64_t)(c + 1) * total / (uint64_t)G};
+  const uint64_t n_items = (total >> BITS) * (uint64_t)A.H_kv, n_units = (total & LOW) * (uint64_t)A.H_kv;
+  const bool whole = n_items <= (uint64_t)G && most <= (uint32_t)(n_units / (uint64_t)G) + WHOLE;
+  auto pick = [&](uint64_t x) { return whole ? x >> BITS : x & LOW; };
+  const uint64_t cut[2] = {whole ? (uint64_t)c : (uint64_t)c * n_units / (uint64_t)G, whole ? (uint64_t)c + 1 : (uint64_t)(c + 1) * n_units / (uint64_t)G};
   uint64_t run = 0;
   for (int base = 0; base < A.S; base += NT) {
-    if (A.S > NT) { mine = units(base + tid); block_scan(mine, before, all); }
-    const uint64_t a = (run + before) * A.H_kv, b = a + (uint64_t)mine * A.H_kv;
+    if (A.S > NT) {
+      int groups;
+      uint32_t top;
+      mine = units(base + tid, groups, top);
+      mine |= (uint64_t)groups << BITS;
+      block_scan(mine, before, all);
+    }
+    const uint64_t a = (pick(run) + pick(before)) * A.H_kv, b = a + pick(mine) * A.H_kv;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (cut[e] >= a && cut[e] < b) { s.request[e] = base + tid; s.at[e] = cut[e] - a; s.width[e] = mine; }
+      if (cut[e] >= a && cut[e] < b) { s.request[e] = base + tid; s.at[e] = cut[e] - a; s.width[e] = (uint32_t)pick(mine); }
     run += all;
   }
   __syncthreads();
@@ -184,12 +221,15 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
     int4 found = make_int4(A.S, 0, 0, 0);
     if (i < A.S) {
       const PagedRequest r = paged_request(A, i);
-      const int groups = paged_groups(A, r), head = (int)(s.at[warp] / s.width[warp]);
-      uint32_t left = (uint32_t)(s.at[warp] - (uint64_t)head * s.width[warp]);
+      const int groups = paged_groups(A, r);
+      const uint32_t width = s.width[warp];
+      const uint64_t at = s.at[warp];
+      const int head = at >> 32 == 0 ? (int)((uint32_t)at / width) : (int)(at / width);
+      uint32_t left = (uint32_t)(at - (uint64_t)head * width);
       for (int x0 = 0; x0 < groups; x0 += 32) {
         const PagedItem it = paged_item<KEYS>(A, r, min(x0 + lane, groups - 1));
         const int n = it.n;
-        const uint32_t cost = x0 + lane < groups ? n + FIXED : 0;
+        const uint32_t cost = x0 + lane < groups ? (whole ? 1 : n + FIXED) : 0;
         uint32_t incl = cost;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {

@@ -1,18 +1,18 @@
 // Attention of chunks of new tokens over paged caches on the fifth-generation tensor cores.
 //
 // An item is two halves of up to 128 rows (floor(128/g) new tokens x g query heads of a KV head each); its keys come in
-// tiles of 128.  Per half and tile: S = Q.K^T (tcgen05.mma, both operands in shared memory, fp32 scores in tensor memory),
-// softmax of S by a warpgroup with one row per thread, the weights P written over S as 16-bit values, O += P.V
-// (tcgen05.mma, P from tensor memory, V as it lies in the cache: MN-major).  Tensor memory is full: two score tiles and two
-// accumulators of 128 columns.  While one half's scores are turned into weights, the other half's products run, so
-// the tensor cores and the exponential units take turns on both halves; 2 x 128 rows share every key tile in
-// shared memory.
+// tiles of 128, which a half takes 64 at a time.  Per half and 64 keys: S = Q.K^T (tcgen05.mma, both operands in shared
+// memory, fp32 scores in tensor memory), softmax of S by a warpgroup with one row per thread, the weights P written over S as
+// 16-bit values, O += P.V (tcgen05.mma, P from tensor memory, V as it lies in the cache: MN-major).  Tensor memory is full:
+// per half two buffers of 64 scores and an accumulator of 128 columns.  The scores of step t + 2 are asked for as soon as
+// the weights of step t are used up, so a warpgroup always has its next scores waiting (with one buffer of 128 a half
+// had nothing to do between its weights and its next scores, 1700 cycles of 3900 a tile).
 //
-// 12 warps: two warpgroups of softmax (half 0, half 1), and one of helpers: warp 8 brings in Q and the tiles (tiled TMA, one
-// box per page and 64-channel panel, 128-byte swizzle, four slots of 32 KB for K and V in turn), warps 9 and 10
-// issue the products of a half each, warp 11 looks after masked values: 0 x NaN is NaN, so in tiles that some row of the item does
-// not see whole it sets values of keys that no row sees to zero before the product, and looks for values that are not
-// finite among the others; such a segment's rows are done again one by one (paged_slow_row).
+// 12 warps: two warpgroups of softmax (half 0, half 1), and one of helpers: one warp brings in Q and the tiles (tiled TMA, one box
+// per page and 64-channel panel, 128-byte swizzle, four slots of 32 KB for K and V in turn), two issue the products of a
+// half each, one looks after masked values: 0 x NaN is NaN, so in tiles that some row of the item does not see whole it
+// sets values of keys that no row sees to zero before the product, and looks for values that are not finite among the
+// others; such a segment's rows are done again one by one (paged_slow_row).
 //
 // An accumulator is rescaled by the threads that own its rows, and only when a score passes the row's reference by more
 // than PagedWeights::RAISE.  Every wait is bounded; a wait that runs out ends the CTA's work and sets its status word.
@@ -20,19 +20,22 @@
 
 namespace rdkv {
 
-constexpr int CH_KEYS = PAGED_CHUNK_KEYS, CH_ROWS = PAGED_CHUNK_ROWS, CH_SLOTS = 4, CH_THREADS = 384;
+constexpr int CH_KEYS = PAGED_CHUNK_KEYS, CH_ROWS = PAGED_CHUNK_ROWS, CH_SLOTS = 4, CH_SOFTMAX_WARPS = 8, CH_THREADS = CH_SOFTMAX_WARPS * 32 + 128;
+constexpr int CH_STEP = 64;                       // keys of a step
 constexpr int CH_PANEL = 128 * 128;               // bytes: 128 rows of 64 channels
 constexpr int CH_SLOT = 2 * CH_PANEL;
 constexpr int CH_STAGE = 32 * 128;                // bytes a softmax warp's results pass through on their way out
-constexpr size_t CH_SMEM = 1024 + (size_t)(2 + CH_SLOTS) * CH_SLOT + 8 * CH_STAGE;
+constexpr size_t CH_SMEM = (size_t)(2 + CH_SLOTS) * CH_SLOT + CH_SOFTMAX_WARPS * CH_STAGE;   // (starts on 1024 bytes)
 constexpr int CH_INFO = 8;                        // tiles whose description is kept (a softmax warp is at most three behind the loads)
 constexpr int CH_POLY = 4;                         // every CH_POLY-th pair of exponentials goes to the FMA units
 constexpr int CH_FIXED = 1, CH_SNAP = 3, CH_WHOLE = 8;
-constexpr int CH_SOFTMAX_REGS = 208, CH_HELPER_REGS = 88;
-static_assert(256 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS <= 384 * 168, "the split draws on what the block was launched with");
+constexpr int CH_SOFTMAX_REGS = 208, CH_HELPER_REGS = 88, CH_LAUNCH_REGS = 168;
+static_assert(CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS <= CH_THREADS * CH_LAUNCH_REGS,
+              "the split draws on what the block was launched with");
 
-// Barriers.
-enum { CH_Q_FULL = 0, CH_Q_FREE = 1, CH_S_FULL = 2, CH_P_READY = 4, CH_O_DONE = 8, CH_FULL = 10, CH_FREE = CH_FULL + CH_SLOTS,
+// Barriers: Q arrived / free; [2 half + buffer] scores done, weights written, product with the values done; [slot] tile arrived / free,
+// values looked after; [half] products ended early.
+enum { CH_Q_FULL = 0, CH_Q_FREE = 1, CH_S_FULL = 2, CH_P_READY = 6, CH_O_DONE = 10, CH_FULL = 14, CH_FREE = CH_FULL + CH_SLOTS,
        CH_V_OK = CH_FREE + CH_SLOTS, CH_DRAINED = CH_V_OK + CH_SLOTS, CH_BARS = CH_DRAINED + 2 };
 
 struct ChunkTile { int key0, there, edge; };      // first key, a bit per 16 keys whose page is there, some row does not see all of it
@@ -71,6 +74,16 @@ __device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
 __device__ __forceinline__ bool chunk_edge(const PagedArgs& A, const PagedItem& it, int key0, int there) {
   const int p_last = it.p0 + it.n_tok - 1;
   return key0 + CH_KEYS - 1 > it.p0 || there != 0xFF || (A.window > 0 && key0 <= p_last - A.window && key0 + CH_KEYS > A.sinks);
+}
+
+// Steps of a segment that half h takes: those whose first key is in front of the end of what its last row sees.
+__device__ __forceinline__ int chunk_steps(const PagedArgs& A, const PagedSegment& s, int h, int tm) {
+  const int n_tok = min(tm, s.item.n_tok - h * tm);
+  if (n_tok <= 0) return 0;
+  const int end = min(s.item.p0 + h * tm + n_tok, A.cap);
+  int steps = 2 * (s.k1 - s.k0);
+  while (steps > 0 && paged_tile(s.item, s.k0 + ((steps - 1) >> 1)) * CH_KEYS + ((steps - 1) & 1) * CH_STEP >= end) --steps;
+  return steps;
 }
 
 template <bool BF16>
@@ -141,73 +154,73 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
 
 __device__ __forceinline__ int chunk_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-// Warps 9 and 10: the products of half 0, of half 1.  What a half's next scores wait for is short: its weights, the rest of the product
-// with the values, the product with the keys; everything else is waited for before the weights are.
+// Two warps: the products of half 0, of half 1.
 template <bool BF16>
 __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int h, uint32_t q32, uint32_t ring, uint32_t bar, uint32_t tmem_,
                                const ChunkTile* s_info, int* s_trouble) {
-  constexpr uint32_t QK = mma_idesc<BF16>(128, false), PV = mma_idesc<BF16>(128, true);
+  constexpr uint32_t QK = mma_idesc<BF16>(CH_STEP, false), PV = mma_idesc<BF16>(128, true);
   const int tm = A.group >> 1;
   const uint32_t t_s = (uint32_t)chunk_uniform((int)tmem_ + 128 * h), t_o = t_s + 256, one = elect_one();
   const uint64_t q = desc_k_major((uint32_t)chunk_uniform((int)(q32 + h * CH_SLOT)));
-  int slot = 0, tile = 0;                                    // the next K's slot; tiles
-  uint32_t phases = 0, segments = 0, v_ok = 0, p_phase = 0;  // a bit per slot: parity of its next use
+  int tile = 0;                                              // tile x is in slots 2 (x & 1) and the next, their phase is x >> 1
+  uint32_t segments = 0, v_ok = 0, p_phase = 0;              // a bit per V slot / buffer: parity of its next use
   PagedSegment s;
   bool ok = true;
   auto wait = [&](int b, uint32_t parity) { ok = ok && bar_wait_warp(bar + 8 * b, parity); };
-  auto wait_slot = [&](int x) { wait(CH_FULL + x, phases >> x & 1); phases ^= 1u << x; };
-  auto after = [&](int x, int n) { x += n; return x >= CH_SLOTS ? x - CH_SLOTS : x; };
-  auto scores = [&](int k_slot) {                            // S = Q . K^T
-    const uint64_t k = desc_k_major(ring + k_slot * CH_SLOT);
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {                         // 16 channels: 32 bytes along the swizzled row, the second panel after four
-      const uint64_t off = ((uint64_t)(kk >> 2) * CH_PANEL + (uint64_t)(kk & 3) * 32u) >> 4;
-      mma_ss(one, t_s, q + off, k + off, QK, kk > 0 ? 1u : 0u);
+  auto wait_k = [&](int x) { wait(CH_FULL + 2 * (x & 1), x >> 1 & 1); };
+  auto wait_v = [&](int x) {
+    wait(CH_FULL + 2 * (x & 1) + 1, x >> 1 & 1);
+    if (ok && chunk_uniform(s_info[x % CH_INFO].edge) != 0) {
+      wait(CH_V_OK + 2 * (x & 1) + 1, v_ok >> (x & 1) & 1);
+      v_ok ^= 1u << (x & 1);
     }
-    mma_commit(one, bar + 8 * (CH_S_FULL + h));
   };
   while (ok && chunk_uniform(walk.next(A, s))) {
     const int n = chunk_uniform(s.k1 - s.k0);
     if (n == 0) continue;
-    const bool mine = h == 0 || chunk_uniform(s.item.n_tok > tm);
+    const int steps = chunk_uniform(chunk_steps(A, s, h, tm));
     wait(CH_Q_FULL, segments++ & 1);
-    wait_slot(slot);
-    if (!ok) break;
-    tmem_fence_after();
-    if (mine) scores(slot);
-    mma_commit(one, bar + 8 * (CH_FREE + slot));             // (nothing to wait for: arrives at once)
-    if (n == 1) mma_commit(one, bar + 8 * CH_Q_FREE);
-    for (int j = 0; j < n; ++j, ++tile) {                    // `slot`: K of tile j, then its V, then K of tile j + 1
-      const int v_slot = after(slot, 1), k_slot = after(slot, 2);
-      const bool more = j + 1 < n;
-      wait_slot(v_slot);
-      if (ok && chunk_uniform(s_info[tile % CH_INFO].edge) != 0) {
-        wait(CH_V_OK + v_slot, v_ok >> v_slot & 1);
-        v_ok ^= 1u << v_slot;
+    auto scores = [&](int t) {                               // S = Q . K^T of step t, into buffer t & 1
+      const int x = tile + (t >> 1);
+      if ((t & 1) == 0) wait_k(x);
+      if (!ok) return;
+      tmem_fence_after();
+      const uint64_t k = desc_k_major(ring + 2 * (x & 1) * CH_SLOT + (t & 1) * (CH_STEP * 128));
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {                       // 16 channels: 32 bytes along the swizzled row, the second panel after four
+        const uint64_t off = ((uint64_t)(kk >> 2) * CH_PANEL + (uint64_t)(kk & 3) * 32u) >> 4;
+        mma_ss(one, t_s + CH_STEP * (t & 1), q + off, k + off, QK, kk > 0 ? 1u : 0u);
       }
-      if (more) wait_slot(k_slot);
+      mma_commit(one, bar + 8 * (CH_S_FULL + 2 * h + (t & 1)));
+      if ((t & 1) == 1 || t == steps - 1) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1)));
+      if (t == steps - 1) mma_commit(one, bar + 8 * CH_Q_FREE);
+    };
+    if (steps > 0) scores(0);
+    if (steps > 1) scores(1);
+    for (int t = 0; ok && t < steps; ++t) {
+      const int x = tile + (t >> 1), b = t & 1;
+      if (b == 0) wait_v(x);
+      wait(CH_P_READY + 2 * h + b, p_phase >> b & 1);
+      p_phase ^= 1u << b;
       if (!ok) break;
-      if (mine) {
-        const uint64_t v = desc_mn_major(ring + v_slot * CH_SLOT, CH_PANEL);
+      tmem_fence_after();
+      const uint64_t v = desc_mn_major(ring + (2 * (x & 1) + 1) * CH_SLOT + b * (CH_STEP * 128), CH_PANEL);
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          wait(CH_P_READY + 2 * h + part, p_phase);
-          if (!ok) break;
-          tmem_fence_after();
-#pragma unroll
-          for (int kk = 4 * part; kk < 4 * part + 4; ++kk)   // 16 keys: 8 columns of P, two groups of eight rows of V
-            mma_ts(one, t_o, t_s + 8 * kk, v + kk * (2048 >> 4), PV, j > 0 || kk > 0 ? 1u : 0u);
-        }
-        p_phase ^= 1u;
-        if (!ok) break;
-        mma_commit(one, bar + 8 * (CH_O_DONE + h));
-        if (more) scores(k_slot);
-      }
-      mma_commit(one, bar + 8 * (CH_FREE + v_slot));
-      if (more) mma_commit(one, bar + 8 * (CH_FREE + k_slot));
-      if (j + 2 == n) mma_commit(one, bar + 8 * CH_Q_FREE);
-      slot = k_slot;
+      for (int kk = 0; kk < 4; ++kk)                         // 16 keys: 8 columns of P, two groups of eight rows of V
+        mma_ts(one, t_o, t_s + CH_STEP * b + 8 * kk, v + kk * (2048 >> 4), PV, t > 0 || kk > 0 ? 1u : 0u);
+      mma_commit(one, bar + 8 * (CH_O_DONE + 2 * h + b));
+      if (b == 1 || t == steps - 1) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1) + 1));
+      if (t + 2 < steps) scores(t + 2);
     }
+    // tiles that this half sees nothing of: their slots go back as they come
+    if (steps == 0) mma_commit(one, bar + 8 * CH_Q_FREE);
+    for (int x = tile + ((steps + 1) >> 1); ok && x < tile + n; ++x) {
+      wait_k(x);
+      if (ok) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1)));
+      wait_v(x);
+      if (ok) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1) + 1));
+    }
+    tile += n;
   }
   if (!ok) {                                                 // wait (again bounded) for the products in flight
     *s_trouble = 1;
@@ -216,7 +229,7 @@ __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int 
   }
 }
 
-// Warp 11: values in masked places.
+// One warp: values in masked places.
 template <bool BF16>
 __device__ void chunk_values(const PagedArgs& A, PagedWalk<CH_KEYS> walk, unsigned char* ring_ptr, uint32_t bar, const ChunkTile* s_info,
                              int* s_again, int* s_trouble) {
@@ -279,53 +292,47 @@ template <bool BF16>
 __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint32_t bar, uint32_t tmem, const ChunkTile* s_info,
                               const int* s_again, int* s_trouble, int cta, unsigned char* stage) {
   constexpr float RAISE = PagedWeights<BF16>::RAISE, LIFT = PagedWeights<BF16>::LIFT;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = warp >> 2, row = (warp & 3) * 32 + lane, tm = A.group >> 1;
-  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = warp >> 2, quad = warp & 3, row = quad * 32 + lane, tm = A.group >> 1;
+  const uint32_t lanes = (uint32_t)(quad * 32) << 16;
   const uint32_t t_s = tmem + 128 * h + lanes, t_o = tmem + 256 + 128 * h + lanes;
-  unsigned done = 0, tile = 0, segments = 0;                 // tiles of this half; tiles; segments
+  unsigned tile = 0, segments = 0;
+  uint32_t s_phase = 0;                                      // a bit per buffer: parity of its next use
+  // The product of buffer b's last step.  (A barrier a buffer: the one of the step before that is done when the scores that
+  // came after it are, so no phase can be mistaken for another.)
+  auto product_done = [&](int b) { return bar_wait_warp(bar + 8 * (CH_O_DONE + 2 * h + b), (s_phase >> b & 1) ^ 1u); };
   PagedSegment s;
   bool ok = true;
   while (ok && walk.next(A, s)) {
     const int tok = row / A.g, n_tok = min(tm, s.item.n_tok - h * tm);      // new tokens of this half
     const bool live = tok < n_tok && row < tm * A.g;
     const int item_row = h * tm * A.g + row;
-    if (s.k0 == s.k1) {                                      // an item without keys
-      if (live) {
-        const PagedRow d = paged_row<CH_ROWS>(A, s, item_row, cta);
-        for (int c = 0; c < 32; ++c) {
-          if (d.rec != nullptr) *reinterpret_cast<float4*>(d.rec + 4 + 4 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
-          else *reinterpret_cast<uint2*>(d.out + 4 * c) = make_uint2(0u, 0u);
-        }
-        if (d.rec != nullptr) *reinterpret_cast<float4*>(d.rec) = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      }
-      continue;
-    }
-    const int n = s.k1 - s.k0;
-    if (n_tok <= 0) { tile += n; ++segments; continue; }     // the item has one half
+    const int n = s.k1 - s.k0, steps = chunk_steps(A, s, h, tm);
     const int pos = live ? s.item.p0 + h * tm + tok : -1;
-    // the tokens of this warp's live rows, for whether a tile needs masks
-    const int tok_w = ((warp & 3) * 32) / A.g, tok_e = min(((warp & 3) * 32 + 31) / A.g, n_tok - 1);
+    // the tokens of this warp's live rows, for whether a step needs masks
+    const int tok_w = (quad * 32) / A.g, tok_e = min((quad * 32 + 31) / A.g, n_tok - 1);
     const int pos_w = s.item.p0 + h * tm + tok_w, pos_e = s.item.p0 + h * tm + tok_e;
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < n; ++j, ++tile, ++done) {
-      ok = bar_wait_warp(bar + 8 * (CH_S_FULL + h), done & 1);
+    for (int t = 0; t < steps; ++t) {
+      const int b = t & 1;
+      ok = bar_wait_warp(bar + 8 * (CH_S_FULL + 2 * h + b), s_phase >> b & 1);
+      s_phase ^= 1u << b;
       if (!ok) break;
       tmem_fence_after();
-      const ChunkTile info = s_info[tile % CH_INFO];
-      uint32_t v[128];
-      tmem_ld128(t_s, v);
-      if (info.key0 + CH_KEYS - 1 > pos_w || info.there != 0xFF || (A.window > 0 && info.key0 <= pos_e - A.window && info.key0 + CH_KEYS > A.sinks)) {
-        // keys the row sees: below `over`, and, under a window, from `from` on or below the sinks (relative to the tile), where the
+      const ChunkTile info = s_info[(tile + (t >> 1)) % CH_INFO];
+      uint32_t v[64];
+      tmem_ld64(t_s + CH_STEP * b, v);
+      const int key0 = info.key0 + CH_STEP * b, pages = info.there >> (4 * b) & 15;
+      if (key0 + CH_STEP - 1 > pos_w || pages != 15 || (A.window > 0 && key0 <= pos_e - A.window && key0 + CH_STEP > A.sinks)) {
+        // keys the row sees: below `over`, and, under a window, from `from` on or below the sinks (relative to the step), where the
         // page is there; a bit each
-        const int over = min(pos + 1, s.item.hi) - info.key0, from = A.window > 0 ? pos - A.window + 1 - info.key0 : -0x3fffffff;
-        const int sink = A.sinks - info.key0;
+        const int over = min(pos + 1, s.item.hi) - key0, from = A.window > 0 ? pos - A.window + 1 - key0 : -0x3fffffff, sink = A.sinks - key0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           auto below = [&](int x) {                          // bits of keys 32 c + i < x
             const int n = min(max(x - 32 * c, 0), 32);
             return n == 0 ? 0u : 0xFFFFFFFFu >> (32 - n);
           };
-          const uint32_t there = (info.there >> (2 * c) & 1 ? 0xFFFFu : 0u) | (info.there >> (2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
+          const uint32_t there = (pages >> (2 * c) & 1 ? 0xFFFFu : 0u) | (pages >> (2 * c + 1) & 1 ? 0xFFFF0000u : 0u);
           const uint32_t seen = below(over) & (~below(from) | below(sink)) & there;
 #pragma unroll
           for (int i = 0; i < 32; ++i)
@@ -334,15 +341,15 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; i += 8)
+      for (int i = 0; i < CH_STEP; i += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
       const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * A.scale_log2;
       if (__any_sync(0xffffffffu, high > m + RAISE)) {
         const float to = fmaxf(m, high), f = to == -INFINITY ? 1.f : exp2_approx(m - to);   // (m = -inf: 0)
         m = to; l *= f;
-        if (j > 0) {                                         // the accumulator, once the product before is done
-          ok = bar_wait_warp(bar + 8 * (CH_O_DONE + h), (done - 1) & 1);
+        if (t > 0) {                                         // the accumulator, once the product of the step before is done
+          ok = product_done(b ^ 1);
           if (!ok) break;
           tmem_fence_after();
 #pragma unroll 1
@@ -358,45 +365,38 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
       const float base = (m == -INFINITY ? 0.f : m) - LIFT;
       const uint64_t scale2 = two(A.scale_log2, A.scale_log2), base2 = two(-base, -base);
       uint64_t sum[2] = {0, 0};
-      auto weights = [&](int first, int end) {
 #pragma unroll
-        for (int i = first; i < end; i += 2) {
-          uint64_t x = fma2(two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, base2);
-          float lo, hi;
-          if ((i >> 1) % CH_POLY == CH_POLY - 1) {
-            x = exp2_poly2(x);
-            split(x, lo, hi);
-          } else {
-            split(x, lo, hi);
-            lo = exp2_approx(lo); hi = exp2_approx(hi);
-            x = two(lo, hi);
-          }
-          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
-          v[i >> 1] = paged_pack<BF16>(lo, hi);
+      for (int i = 0; i < CH_STEP; i += 2) {
+        uint64_t x = fma2(two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, base2);
+        float lo, hi;
+        if ((i >> 1) % CH_POLY == CH_POLY - 1) {
+          x = exp2_poly2(x);
+          split(x, lo, hi);
+        } else {
+          split(x, lo, hi);
+          lo = exp2_approx(lo); hi = exp2_approx(hi);
+          x = two(lo, hi);
         }
-      };
-      auto ready = [&](int part) {
-        tmem_wait_st();
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(bar + 8 * (CH_P_READY + 2 * h + part));
-      };
-      weights(0, 64);                                        // 64 keys: their product starts while the rest is worked out
-      tmem_st32(t_s, v);
-      weights(64, 80);
-      ready(0);
-      weights(80, 128);
-      tmem_st32(t_s + 32, v + 32);
-      ready(1);
-      float a, b, c, d;
-      split(sum[0], a, b); split(sum[1], c, d);
-      l += (a + b) + (c + d);
+        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
+        v[i >> 1] = paged_pack<BF16>(lo, hi);
+      }
+      tmem_st32(t_s + CH_STEP * b, v);
+      tmem_wait_st();
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar + 8 * (CH_P_READY + 2 * h + b));
+      float e0, e1, e2, e3;
+      split(sum[0], e0, e1); split(sum[1], e2, e3);
+      l += (e0 + e1) + (e2 + e3);
     }
     if (!ok) break;
-    ok = bar_wait_warp(bar + 8 * (CH_O_DONE + h), (done - 1) & 1);
-    if (!ok) break;
-    tmem_fence_after();
-    if (s_again[segments & 3] == (int)segments + 1) {
+    if (n_tok <= 0) { tile += n; segments += n > 0; continue; }             // the item has one half
+    if (steps > 0) {
+      ok = product_done((steps - 1) & 1);
+      if (!ok) break;
+      tmem_fence_after();
+    }
+    if (steps > 0 && s_again[segments & 3] == (int)segments + 1) {
       const PagedSegment copy = s;
       for (int r = 0; r < 32; ++r)
         if (__shfl_sync(0xffffffffu, live ? 1 : 0, r) != 0) paged_slow_row<BF16, CH_KEYS, CH_ROWS>(A, copy, item_row - lane + r, cta);
@@ -406,27 +406,29 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
       PagedRow d = {nullptr, nullptr};
       if (live) d = paged_row<CH_ROWS>(A, s, item_row, cta);
       const bool records = A.rec != nullptr || s.k0 != 0 || s.k1 != s.item.n;
-      const float w = records ? 1.f : paged_over(l);
+      const float w = steps == 0 ? 0.f : records ? 1.f : paged_over(l);
       if (d.rec != nullptr) *reinterpret_cast<float4*>(d.rec) = make_float4((m - LIFT) * PAGED_LN2, l, 0.f, 0.f);
       const uint64_t to = !live ? 0ull : records ? reinterpret_cast<uint64_t>(d.rec + 4) : reinterpret_cast<uint64_t>(d.out);
       uint4* mine = reinterpret_cast<uint4*>(stage) + lane * 8;
 #pragma unroll 1
       for (int c = 0; c < (records ? 4 : 2); ++c) {
         uint4 y[8];
-        if (records) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (records && e == 1) break;
           uint32_t x[32];
-          tmem_ld32(t_o + 32 * c, x);
+          if (steps > 0) tmem_ld32(t_o + (records ? 32 * c : 64 * c + 32 * e), x);
+          else
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        } else {
+            for (int i = 0; i < 32; ++i) x[i] = 0u;          // (no step wrote the accumulator)
+          if (records) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t x[32];
-            tmem_ld32(t_o + 64 * c + 32 * e, x);
+            for (int i = 0; i < 8; ++i) y[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              auto pair = [&](int k) { return paged_pack<BF16>(__uint_as_float(x[8 * i + k]) * w, __uint_as_float(x[8 * i + k + 1]) * w); };
-              y[4 * e + i] = make_uint4(pair(0), pair(2), pair(4), pair(6));
+              auto two16 = [&](int k) { return paged_pack<BF16>(__uint_as_float(x[8 * i + k]) * w, __uint_as_float(x[8 * i + k + 1]) * w); };
+              y[4 * e + i] = make_uint4(two16(0), two16(2), two16(4), two16(6));
             }
           }
         }
@@ -444,7 +446,8 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
       }
     }
     tmem_fence_before();
-    ++segments;
+    tile += n;
+    segments += n > 0;
   }
   if (!ok) *s_trouble = 1;
 }
@@ -453,7 +456,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(CH_THREADS, 1)
 paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v) {
-  extern __shared__ unsigned char ch_raw[];
+  extern __shared__ __align__(1024) unsigned char ch_raw[];
   __shared__ __align__(8) uint64_t s_bar[CH_BARS];
   __shared__ ChunkTile s_info[CH_INFO];
   __shared__ PagedPlaceScratch s_place;
@@ -461,13 +464,12 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   __shared__ int s_again[4];                                 // segment (its number + 1) whose rows are done again
   __shared__ int s_trouble;
   const int tid = threadIdx.x, warp = tid >> 5, cta = blockIdx.x;
-  const uint32_t q32 = (smem_addr(ch_raw) + 1023u) & ~1023u, ring = q32 + 2 * CH_SLOT, bar = smem_addr(s_bar);
+  const uint32_t q32 = smem_addr(ch_raw), ring = q32 + 2 * CH_SLOT, bar = smem_addr(s_bar);
   if (tid == 0) {
     bar_init(bar + 8 * CH_Q_FULL, 1); bar_init(bar + 8 * CH_Q_FREE, 2);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bar_init(bar + 8 * (CH_S_FULL + h), 1); bar_init(bar + 8 * (CH_P_READY + 2 * h), 4); bar_init(bar + 8 * (CH_P_READY + 2 * h + 1), 4); bar_init(bar + 8 * (CH_O_DONE + h), 1); bar_init(bar + 8 * (CH_DRAINED + h), 1);
-    }
+    for (int i = 0; i < 4; ++i) { bar_init(bar + 8 * (CH_S_FULL + i), 1); bar_init(bar + 8 * (CH_P_READY + i), 4); bar_init(bar + 8 * (CH_O_DONE + i), 1); }
+    bar_init(bar + 8 * CH_DRAINED, 1); bar_init(bar + 8 * (CH_DRAINED + 1), 1);
 #pragma unroll
     for (int i = 0; i < CH_SLOTS; ++i) {
       bar_init(bar + 8 * (CH_FULL + i), 1); bar_init(bar + 8 * (CH_FREE + i), 3); bar_init(bar + 8 * (CH_V_OK + i), 1);
@@ -477,7 +479,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   }
   if (tid < 4) s_again[tid] = 0;
   if (tid == 32) { tma_prefetch_map(&tm_q); tma_prefetch_map(&tm_k); tma_prefetch_map(&tm_v); }
-  if (warp == 9) {
+  if (warp == CH_SOFTMAX_WARPS + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -489,20 +491,21 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   tmem_fence_after();
   const uint32_t tmem = s_tmem;
   const PagedWalk<CH_KEYS> walk(A, from, to);
-  if (warp >= 8) {
+  unsigned char* ring_ptr = ch_raw + 2 * CH_SLOT;
+  if (warp >= CH_SOFTMAX_WARPS) {
+    const int role = warp - CH_SOFTMAX_WARPS;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_HELPER_REGS));
-    if (warp == 8) chunk_load<BF16>(A, &tm_q, &tm_k, &tm_v, walk, q32, ring, bar, s_info, &s_trouble);
-    else if (warp < 11) chunk_products<BF16>(A, walk, warp - 9, q32, ring, bar, tmem, s_info, &s_trouble);
-    else chunk_values<BF16>(A, walk, ch_raw + (ring - smem_addr(ch_raw)), bar, s_info, s_again, &s_trouble);
+    if (role == 0) chunk_load<BF16>(A, &tm_q, &tm_k, &tm_v, walk, q32, ring, bar, s_info, &s_trouble);
+    else if (role < 3) chunk_products<BF16>(A, walk, role - 1, q32, ring, bar, tmem, s_info, &s_trouble);
+    else chunk_values<BF16>(A, walk, ring_ptr, bar, s_info, s_again, &s_trouble);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CH_SOFTMAX_REGS));
-    chunk_softmax<BF16>(A, walk, bar, tmem, s_info, s_again, &s_trouble, cta,
-                        ch_raw + (ring - smem_addr(ch_raw)) + CH_SLOTS * CH_SLOT + warp * CH_STAGE);
+    chunk_softmax<BF16>(A, walk, bar, tmem, s_info, s_again, &s_trouble, cta, ring_ptr + CH_SLOTS * CH_SLOT + warp * CH_STAGE);
   }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == CH_SOFTMAX_WARPS + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   paged_zero_padding(A, CH_THREADS);
   if (tid == 0) A.status[cta] = s_trouble;
 }
@@ -531,7 +534,7 @@ int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, c
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
     if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
     // (the register split waits for ever if the block was launched with fewer than it hands out)
-    if (attr.numRegs * CH_THREADS < 256 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS) return RDKV_ERR_LAUNCH;
+    if (attr.numRegs * CH_THREADS < CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS) return RDKV_ERR_LAUNCH;
     kernel<<<PAGED_CHUNK_CTAS, CH_THREADS, CH_SMEM, st>>>(A, tm_q, tm_k, tm_v);
     const int rc = launch_status();
     if (rc != RDKV_OK) return rc;

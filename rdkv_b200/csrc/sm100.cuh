@@ -118,21 +118,29 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
       : "r"(taddr)
       : "memory");
 }
-// 128 columns.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t* v) {
+// 64 columns.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t* v) {
   asm volatile(
-      "{\n"
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
       "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, "
-      "%46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, "
-      "%72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, "
-      "%98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, "
-      "%120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n"
+      "%46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n"
       "tcgen05.wait::ld.sync.aligned;\n"
-      "}\n"
-      : RDKV_R8(v, 0), RDKV_R8(v, 8), RDKV_R8(v, 16), RDKV_R8(v, 24), RDKV_R8(v, 32), RDKV_R8(v, 40), RDKV_R8(v, 48), RDKV_R8(v, 56),
-        RDKV_R8(v, 64), RDKV_R8(v, 72), RDKV_R8(v, 80), RDKV_R8(v, 88), RDKV_R8(v, 96), RDKV_R8(v, 104), RDKV_R8(v, 112), RDKV_R8(v, 120)
+      : RDKV_R8(v, 0), RDKV_R8(v, 8), RDKV_R8(v, 16), RDKV_R8(v, 24), RDKV_R8(v, 32), RDKV_R8(v, 40), RDKV_R8(v, 48), RDKV_R8(v, 56)
       : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : RDKV_R8(v, 0), RDKV_R8(v, 8)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
+      ::"r"(taddr), RDKV_S8(v, 0), RDKV_S8(v, 8)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {

@@ -403,12 +403,20 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
     } else {
       // a row a thread in tensor memory, a row eight lanes on the way out: 128 bytes of every row pass through shared memory, their
       // 16-byte chunks swapped about by row (32 rows of 16 bytes each would be 32 lines an instruction)
-      PagedRow d = {nullptr, nullptr};
-      if (live) d = paged_row<CH_ROWS>(A, s, item_row, cta);
-      const bool records = A.rec != nullptr || s.k0 != 0 || s.k1 != s.item.n;
+      const bool whole = s.k0 == 0 && s.k1 == s.item.n, records = A.rec != nullptr || !whole;
       const float w = steps == 0 ? 0.f : records ? 1.f : paged_over(l);
-      if (d.rec != nullptr) *reinterpret_cast<float4*>(d.rec) = make_float4((m - LIFT) * PAGED_LN2, l, 0.f, 0.f);
-      const uint64_t to = !live ? 0ull : records ? reinterpret_cast<uint64_t>(d.rec + 4) : reinterpret_cast<uint64_t>(d.out);
+      const int64_t at_tok = s.item.tok0 + h * tm + tok, at_head = s.head * A.g + row - tok * A.g;
+      uint64_t to = 0ull;
+      if (live) {
+        if (records) {
+          float* rec = whole ? A.rec + (at_tok * A.H_q + at_head) * RDKV_PARTIAL_STRIDE
+                             : A.part + ((int64_t)(2 * cta + (s.k0 > 0 ? 0 : 1)) * CH_ROWS + item_row) * RDKV_PARTIAL_STRIDE;
+          *reinterpret_cast<float4*>(rec) = make_float4((m - LIFT) * PAGED_LN2, l, 0.f, 0.f);
+          to = reinterpret_cast<uint64_t>(rec + 4);
+        } else {
+          to = reinterpret_cast<uint64_t>(A.out + at_tok * A.o_tok + at_head * A.o_head);
+        }
+      }
       uint4* mine = reinterpret_cast<uint4*>(stage) + lane * 8;
 #pragma unroll 1
       for (int c = 0; c < (records ? 4 : 2); ++c) {
@@ -438,9 +446,12 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
 #pragma unroll
         for (int i = 0; i < 8; ++i) {                        // four rows at a time
           const int r = 4 * i + (lane >> 3);
-          const uint64_t at = __shfl_sync(0xffffffffu, to, r);
-          const uint4 x = reinterpret_cast<const uint4*>(stage)[r * 8 + ((lane & 7) ^ (r & 7))];
-          if (at != 0ull) *reinterpret_cast<uint4*>(at + 128 * c + 16 * (lane & 7)) = x;
+          y[i] = reinterpret_cast<const uint4*>(stage)[r * 8 + ((lane & 7) ^ (r & 7))];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint64_t at = __shfl_sync(0xffffffffu, to, 4 * i + (lane >> 3));
+          if (at != 0ull) store_global(at + 128 * c + 16 * (lane & 7), y[i]);
         }
         __syncwarp();
       }

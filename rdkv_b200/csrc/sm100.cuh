@@ -16,6 +16,10 @@ __device__ __forceinline__ float exp2_approx(float x) {          // 2^x, one ins
   return y;
 }
 
+__device__ __forceinline__ void store_global(uint64_t addr, const uint4& v) {
+  asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // ── mbarrier ────────────────────────────────────────────────────────────────
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));

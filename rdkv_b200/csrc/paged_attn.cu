@@ -432,36 +432,41 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
   if (tid == 0) A.status[cta] = s_trouble;
 }
 
+template <bool BF16>
+static int decode_cluster(const PagedArgs& A, unsigned ctas, unsigned size, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  constexpr auto kernel = paged_decode_kernel<BF16, true>;
+  cudaError_t e = allow_dynamic_smem_once<paged_decode_kernel<BF16, true>>(DEC_SMEM);
+  if (e == cudaSuccess && size > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+  cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = DEC_SMEM;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, A, tm_k, tm_v);
+  if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
+  return launch_status();
+}
+
+template <bool BF16>
+static int decode_line(const PagedArgs& A, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  const cudaError_t e = allow_dynamic_smem_once<paged_decode_kernel<BF16, false>>(DEC_SMEM);
+  if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
+  paged_decode_kernel<BF16, false><<<PAGED_DECODE_CTAS, DEC_THREADS, DEC_SMEM, st>>>(A, tm_k, tm_v);
+  const int rc = launch_status();
+  if (rc != RDKV_OK) return rc;
+  return paged_launch_join(paged_join_kernel<BF16, DEC_ROWS, PAGED_DECODE_CTAS>, A, dim3(PAGED_DECODE_CTAS - 1, DEC_ROWS / PAGED_JOIN_WARPS), st);
+}
+
 int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   // Few items: a cluster each, as long as eight CTAs an item fit the GPU at once.  (One request of 1061 tokens, 8 heads: see above.)
   const int64_t items = (int64_t)A.S * A.H_kv;
   if (items > 0 && items * 8 <= PAGED_DECODE_CTAS) {
     const int size = items * 16 <= PAGED_DECODE_CTAS ? 16 : 8;
-    auto go = [&](auto kernel) -> int {
-      cudaError_t e = allow_dynamic_smem(kernel, DEC_SMEM);
-      if (e == cudaSuccess && size > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = (unsigned)size; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cudaLaunchConfig_t cfg = {};
-      cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
-      cfg.gridDim = dim3((unsigned)(items * size)); cfg.blockDim = dim3(DEC_THREADS); cfg.dynamicSmemBytes = DEC_SMEM;
-      if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, A, tm_k, tm_v);
-      if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
-      return launch_status();
-    };
-    return bf16 ? go(paged_decode_kernel<true, true>) : go(paged_decode_kernel<false, true>);
+    return bf16 ? decode_cluster<true>(A, (unsigned)(items * size), (unsigned)size, tm_k, tm_v, st)
+                : decode_cluster<false>(A, (unsigned)(items * size), (unsigned)size, tm_k, tm_v, st);
   }
-  auto go = [&](auto kernel, auto join) -> int {
-    const cudaError_t e = allow_dynamic_smem(kernel, DEC_SMEM);
-    if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
-    kernel<<<PAGED_DECODE_CTAS, DEC_THREADS, DEC_SMEM, st>>>(A, tm_k, tm_v);
-    const int rc = launch_status();
-    if (rc != RDKV_OK) return rc;
-    return paged_launch_join(join, A, dim3(PAGED_DECODE_CTAS - 1, DEC_ROWS / PAGED_JOIN_WARPS), st);
-  };
-  if (bf16) return go(paged_decode_kernel<true, false>, paged_join_kernel<true, DEC_ROWS, PAGED_DECODE_CTAS>);
-  return go(paged_decode_kernel<false, false>, paged_join_kernel<false, DEC_ROWS, PAGED_DECODE_CTAS>);
+  return bf16 ? decode_line<true>(A, tm_k, tm_v, st) : decode_line<false>(A, tm_k, tm_v, st);
 }
 
 }  // namespace rdkv

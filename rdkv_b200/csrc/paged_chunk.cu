@@ -536,23 +536,29 @@ static bool chunk_q_map(CUtensorMap* tm, const PagedArgs& A, bool bf16) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <bool BF16>
+static int chunk_launch(const PagedArgs& A, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
+  constexpr auto kernel = paged_chunk_kernel<BF16>;
+  // (the register split waits for ever if the block was launched with fewer than it hands out)
+  static const int regs = [] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
+  }();
+  const cudaError_t e = allow_dynamic_smem_once<paged_chunk_kernel<BF16>>(CH_SMEM);
+  if (e != cudaSuccess || regs * CH_THREADS < CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS) {
+    g_last_cuda_error = (int)e;
+    return RDKV_ERR_LAUNCH;
+  }
+  kernel<<<PAGED_CHUNK_CTAS, CH_THREADS, CH_SMEM, st>>>(A, tm_q, tm_k, tm_v);
+  const int rc = launch_status();
+  if (rc != RDKV_OK) return rc;
+  return paged_launch_join(paged_join_kernel<BF16, CH_ROWS, PAGED_CHUNK_CTAS>, A, dim3(PAGED_CHUNK_CTAS - 1, 16), st);
+}
+
 int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   CUtensorMap tm_q;
   if (!chunk_q_map(&tm_q, A, bf16)) return RDKV_ERR_BAD_SHAPE;
-  auto go = [&](auto kernel, auto join) -> int {
-    cudaError_t e = allow_dynamic_smem(kernel, CH_SMEM);
-    cudaFuncAttributes attr;
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
-    if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
-    // (the register split waits for ever if the block was launched with fewer than it hands out)
-    if (attr.numRegs * CH_THREADS < CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS) return RDKV_ERR_LAUNCH;
-    kernel<<<PAGED_CHUNK_CTAS, CH_THREADS, CH_SMEM, st>>>(A, tm_q, tm_k, tm_v);
-    const int rc = launch_status();
-    if (rc != RDKV_OK) return rc;
-    return paged_launch_join(join, A, dim3(PAGED_CHUNK_CTAS - 1, 16), st);
-  };
-  if (bf16) return go(paged_chunk_kernel<true>, paged_join_kernel<true, CH_ROWS, PAGED_CHUNK_CTAS>);
-  return go(paged_chunk_kernel<false>, paged_join_kernel<false, CH_ROWS, PAGED_CHUNK_CTAS>);
+  return bf16 ? chunk_launch<true>(A, tm_q, tm_k, tm_v, st) : chunk_launch<false>(A, tm_q, tm_k, tm_v, st);
 }
 
 }  // namespace rdkv

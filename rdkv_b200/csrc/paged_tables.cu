@@ -160,7 +160,7 @@ extern "C" int rdkv_paged_tables(const int32_t* ctx_lens, const int32_t* new_len
   A.free_start = free_start; A.S = n_requests; A.width = width; A.n_free = n_free; A.page = page_size; A.n_tokens = n_tokens;
   A.slot_map = slot_map; A.positions = positions; A.q_start = q_start; A.kv_lens = kv_lens; A.free_next = free_next; A.missing = missing;
   const size_t smem = sizeof(int32_t) * 2 * (size_t)(n_requests + 1);
-  cudaError_t e = allow_dynamic_smem(paged_tables_kernel, sizeof(int32_t) * 2 * (TABLES_MAX_REQUESTS + 1));
+  const cudaError_t e = allow_dynamic_smem_once<paged_tables_kernel>(sizeof(int32_t) * 2 * (TABLES_MAX_REQUESTS + 1));
   if (e != cudaSuccess) { g_last_cuda_error = (int)e; return RDKV_ERR_LAUNCH; }
   const int64_t items = std::max<int64_t>(n_tokens, n_requests + 1);
   const unsigned grid = (unsigned)std::min<int64_t>(148, (items + TABLES_THREADS - 1) / TABLES_THREADS);

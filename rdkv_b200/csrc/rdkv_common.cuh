@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "rdkv_b200.h"
 
 namespace rdkv {
@@ -23,6 +25,20 @@ extern thread_local int g_last_cuda_error;
 template <class Kernel>
 inline cudaError_t allow_dynamic_smem(Kernel kernel, size_t most) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+}
+
+// The same, asked for once per device (`most` is a constant of the kernel, so once is enough; at most 64 devices).
+template <auto Kernel>
+inline cudaError_t allow_dynamic_smem_once(size_t most) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  e = allow_dynamic_smem(Kernel, most);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 inline int launch_status() {

@@ -611,14 +611,20 @@ int rdkv_knapsack_batched_static(const float* scores, int64_t row_stride, int n_
  * No counterpart in the reference.  Pages of page_size tokens, [n_pages][H_kv][page_size][128] in any strides
  * (elements) whose rows are contiguous; a request's pages are listed in its row of block_tables. */
 
-/* Rotates q [n_tokens][H_q][128] and k [n_tokens][H_kv][128] (dtype: all of one type) by the tokens' positions
- * on 1 to 4 axes into q_out / k_out (which may be q / k): axis a owns sections[a] (HOST array, sum 64) of the 64
- * frequencies, angle = positions[a*axis_stride + t] * inv_freq[j] (int32, or int64 with positions_64; taken in 64 bits). */
-int rdkv_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out, int64_t q_out_tok_stride,
-                   int64_t q_out_head_stride, int H_q, const void* k, int64_t k_tok_stride, int64_t k_head_stride,
-                   void* k_out, int64_t k_out_tok_stride, int64_t k_out_head_stride, int H_kv, int dtype, int n_tokens,
-                   const void* positions, int64_t axis_stride, int positions_64, const float* inv_freq,
-                   const int* sections, int n_axes, void* stream);
+/* Rotates q [n_tokens][H_q][128] and k [n_tokens][H_kv][128] (all of one type) by the tokens' positions on 1 to 4 axes into
+ * q_out / k_out (which may be q / k): axis a owns sections[a] (sum 64) of the 64 frequencies, angle =
+ * positions[a*axis_stride + t] * inv_freq[j] (int32, or int64 with positions_64; taken in 64 bits).  Strides in elements.
+ * args: HOST memory, read during the call. */
+typedef struct {
+  int64_t q_tok_stride, q_head_stride, q_out_tok_stride, q_out_head_stride;
+  int64_t k_tok_stride, k_head_stride, k_out_tok_stride, k_out_head_stride;
+  int64_t axis_stride;
+  int32_t H_q, H_kv, dtype, n_tokens, positions_64, n_axes;
+  int32_t sections[4];
+} rdkv_rope_axes_args;
+int rdkv_sizeof_rope_axes_args(void);
+int rdkv_rope_axes(const rdkv_rope_axes_args* args, const void* q, void* q_out, const void* k, void* k_out,
+                   const void* positions, const float* inv_freq, void* stream);
 
 /* Block tables and slot maps of a step: request i holds ctx_lens[i] tokens in its first ceil(ctx/page_size) pages and gets
  * new_lens[i] more.  The pages it lacks are taken from free_pages [n_free], in request order from entry *free_start
@@ -633,30 +639,42 @@ int rdkv_paged_tables(const int32_t* ctx_lens, const int32_t* new_lens, int n_re
 
 /* Writes k / v [n_tokens][H_kv][128] to the slots of slot_map (outside [0, n_pages*page_size): not written).  n_axes > 0:
  * the keys, and q into q_out (H_q > 0), are rotated as by rdkv_rope_axes. */
-int rdkv_paged_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
-                      int64_t v_head_stride, int H_kv, int dtype, int n_tokens, void* k_pages, int64_t k_page_stride,
-                      int64_t k_page_head_stride, int64_t k_page_row_stride, void* v_pages, int64_t v_page_stride,
-                      int64_t v_page_head_stride, int64_t v_page_row_stride, int n_pages, int page_size,
-                      const int64_t* slot_map, const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
-                      int64_t q_out_tok_stride, int64_t q_out_head_stride, int H_q, const void* positions,
-                      int64_t axis_stride, int positions_64, const float* inv_freq, const int* sections, int n_axes,
+typedef struct {
+  int64_t k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  int64_t k_page_stride, k_page_head_stride, k_page_row_stride, v_page_stride, v_page_head_stride, v_page_row_stride;
+  int64_t q_tok_stride, q_head_stride, q_out_tok_stride, q_out_head_stride;
+  int64_t axis_stride;
+  int32_t H_q, H_kv, dtype, n_tokens, n_pages, page_size, positions_64, n_axes;
+  int32_t sections[4];
+} rdkv_paged_append_args;
+int rdkv_sizeof_paged_append_args(void);
+int rdkv_paged_append(const rdkv_paged_append_args* args, const void* k, const void* v, void* k_pages, void* v_pages,
+                      const int64_t* slot_map, const void* q, void* q_out, const void* positions, const float* inv_freq,
                       void* stream);
 
 /* Attention of the new tokens of n_requests requests over their pages (fp16 / bf16; page_size a power of two, 16 to 1024;
  * up to 16 query heads a KV head; bases on 16 bytes, strides of whole 16 bytes).  Query row q_start[i]+j is request i's
- * token kv_lens[i]-n_i+j (n_i = q_start[i+1]-q_start[i], of which the first max_new are answered); it sees the tokens up to
- * itself, under window > 0 only the last `window` of them and the first `sinks`, and none whose page number is
- * outside [0, n_pages).  Either out [n_tokens][H_q][128] (rows behind q_start[n_requests]: zeroed with zero_padding, else left)
- * or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace: rdkv_paged_attention_workspace() bytes (16-byte
- * aligned; of one call at a time), contents arbitrary. */
+ * token kv_lens[i]-n_i+j (n_i = q_start[i+1]-q_start[i]); it sees the tokens up to itself, under window > 0 only the last
+ * `window` of them and the first `sinks`, and none whose page number is outside [0, n_pages).  max_new: the longest chunk
+ * (a hint: it chooses the kernel).  Either out [n_tokens][H_q][128] (rows behind q_start[n_requests]: zeroed with
+ * zero_padding, else left) or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace:
+ * rdkv_paged_attention_workspace() bytes (16-byte aligned; of one call at a time), contents arbitrary.  Its first
+ * rdkv_paged_attention_status_words() int32 say after the call whether a device-side wait ran out (not 0), in which
+ * case the results are invalid. */
+typedef struct {
+  int64_t q_tok_stride, q_head_stride;
+  int64_t k_page_stride, k_head_stride, k_row_stride, v_page_stride, v_head_stride, v_row_stride;
+  int64_t table_stride;
+  int32_t dtype, n_tokens, H_q, H_kv, n_pages, page_size, width, n_requests, max_new, window, sinks;
+  float scale;
+} rdkv_paged_attention_args;
+int rdkv_sizeof_paged_attention_args(void);
+int rdkv_paged_attention_status_words(void);
 int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, int H_q, int H_kv, int max_new);
-int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype, int n_tokens, int H_q,
-                         const void* k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
-                         const void* v_pages, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
-                         int n_pages, int H_kv, int page_size, const int32_t* block_tables, int64_t table_stride,
-                         int width, const int32_t* q_start, const int32_t* kv_lens, int n_requests, int max_new,
-                         int window, int sinks, float scale, void* out, int64_t out_tok_stride, int64_t out_head_stride,
-                         int zero_padding, float* out_partial, void* workspace, int64_t workspace_bytes, void* stream);
+int rdkv_paged_attention(const rdkv_paged_attention_args* args, const void* q, const void* k_pages, const void* v_pages,
+                         const int32_t* block_tables, const int32_t* q_start, const int32_t* kv_lens, void* out,
+                         int64_t out_tok_stride, int64_t out_head_stride, int zero_padding, float* out_partial,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -103,6 +103,32 @@ class UnpackJob(C.Structure):
     ]
 
 
+def _fields(*groups):
+    return [(n, t) for t, names in groups for n in names.split()]
+
+
+class RopeAxesArgs(C.Structure):
+    """Mirror of ``rdkv_rope_axes_args``; field order and types must match the header."""
+    _fields_ = _fields((C.c_int64, "q_tok_stride q_head_stride q_out_tok_stride q_out_head_stride k_tok_stride k_head_stride "
+                                   "k_out_tok_stride k_out_head_stride axis_stride"),
+                       (C.c_int32, "H_q H_kv dtype n_tokens positions_64 n_axes")) + [("sections", C.c_int32 * 4)]
+
+
+class PagedAppendArgs(C.Structure):
+    """Mirror of ``rdkv_paged_append_args``; field order and types must match the header."""
+    _fields_ = _fields((C.c_int64, "k_tok_stride k_head_stride v_tok_stride v_head_stride k_page_stride k_page_head_stride k_page_row_stride "
+                                   "v_page_stride v_page_head_stride v_page_row_stride q_tok_stride q_head_stride q_out_tok_stride "
+                                   "q_out_head_stride axis_stride"),
+                       (C.c_int32, "H_q H_kv dtype n_tokens n_pages page_size positions_64 n_axes")) + [("sections", C.c_int32 * 4)]
+
+
+class PagedAttentionArgs(C.Structure):
+    """Mirror of ``rdkv_paged_attention_args``; field order and types must match the header."""
+    _fields_ = _fields((C.c_int64, "q_tok_stride q_head_stride k_page_stride k_head_stride k_row_stride v_page_stride v_head_stride "
+                                   "v_row_stride table_stride"),
+                       (C.c_int32, "dtype n_tokens H_q H_kv n_pages page_size width n_requests max_new window sinks"), (C.c_float, "scale"))
+
+
 _i, _i64, _p, _f = C.c_int, C.c_int64, C.c_void_p, C.c_float
 
 _PROTOTYPES = {
@@ -125,13 +151,15 @@ _PROTOTYPES = {
     "rdkv_decode_attn": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_decode_attn_tail": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_rope": ([_p, _i, _i, _i64, _p, _i, _i, _i64, _p, _p, _i, _p], _i),
-    "rdkv_rope_axes": ([_p, _i64, _i64, _p, _i64, _i64, _i, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _p, _i64, _i, _p, _p, _i, _p], _i),
+    "rdkv_sizeof_rope_axes_args": ([], _i),
+    "rdkv_rope_axes": ([_p, _p, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_paged_tables": ([_p, _p, _i, _p, _i64, _i, _p, _i, _p, _i, _i64, _p, _p, _p, _p, _p, _p, _p], _i),
-    "rdkv_paged_append": ([_p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _p,
-                           _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i64, _i, _p, _p, _i, _p], _i),
+    "rdkv_sizeof_paged_append_args": ([], _i),
+    "rdkv_paged_append": ([_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p], _i),
+    "rdkv_sizeof_paged_attention_args": ([], _i),
+    "rdkv_paged_attention_status_words": ([], _i),
     "rdkv_paged_attention_workspace": ([_i, _i, _i, _i, _i], _i64),
-    "rdkv_paged_attention": ([_p, _i64, _i64, _i, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i, _i, _i, _p, _i64, _i,
-                              _p, _p, _i, _i, _i, _i, _f, _p, _i64, _i64, _i, _p, _p, _i64, _p], _i),
+    "rdkv_paged_attention": ([_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _p, _p, _i64, _p], _i),
     "rdkv_decode_attn_persistent": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_tail_attn_partial": ([_p, _i, _i64, _i, _i, _p, _p, _i, _i64, _i64, _i64, _i, _p, _i, _p, _p], _i),
     "rdkv_lse_combine": ([_p, _i64, _i, _i64, _i64, _p, _p, _p, _p], _i),
@@ -196,6 +224,9 @@ def lib() -> C.CDLL:
             raise RuntimeError("rdkv_b200: rdkv_pack_meta_job layout mismatch between header and binding")
         if handle.rdkv_sizeof_unpack_job() != C.sizeof(UnpackJob):
             raise RuntimeError("rdkv_b200: rdkv_unpack_job layout mismatch between header and binding")
+        for name, mirror in (("rope_axes", RopeAxesArgs), ("paged_append", PagedAppendArgs), ("paged_attention", PagedAttentionArgs)):
+            if getattr(handle, f"rdkv_sizeof_{name}_args")() != C.sizeof(mirror):
+                raise RuntimeError(f"rdkv_b200: rdkv_{name}_args layout mismatch between header and binding")
         _lib = handle
     return _lib
 

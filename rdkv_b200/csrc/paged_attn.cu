@@ -429,14 +429,21 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
   }
   __syncthreads();
   paged_zero_padding(A, DEC_THREADS);
-  if (tid == 0) A.status[cta] = s_trouble;
+  paged_report(A, s_trouble);
+}
+
+// Clusters of 16 are more than every GPU promises: asked for once per device.
+template <auto Kernel>
+static cudaError_t allow_big_clusters_once() {
+  static std::atomic<uint64_t> done{0};
+  return once_per_device(done, [] { return cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
 }
 
 template <bool BF16>
 static int decode_cluster(const PagedArgs& A, unsigned ctas, unsigned size, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   constexpr auto kernel = paged_decode_kernel<BF16, true>;
   cudaError_t e = allow_dynamic_smem_once<paged_decode_kernel<BF16, true>>(DEC_SMEM);
-  if (e == cudaSuccess && size > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && size > 8) e = allow_big_clusters_once<paged_decode_kernel<BF16, true>>();
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -483,45 +490,47 @@ extern "C" int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, 
                                              : paged_workspace_bytes(PAGED_CHUNK_CTAS, PAGED_CHUNK_ROWS);
 }
 
-extern "C" int rdkv_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype, int n_tokens, int H_q,
-                                    const void* k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
-                                    const void* v_pages, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
-                                    int n_pages, int H_kv, int page_size, const int32_t* block_tables, int64_t table_stride,
-                                    int width, const int32_t* q_start, const int32_t* kv_lens, int n_requests, int max_new,
-                                    int window, int sinks, float scale, void* out, int64_t out_tok_stride, int64_t out_head_stride,
-                                    int zero_padding, float* out_partial, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (n_tokens < 0 || n_requests < 0 || H_q <= 0 || H_kv <= 0 || n_pages < 0 || width < 0 || window < 0 || sinks < 0 || max_new < 0 || !(scale > 0.f))
+extern "C" int rdkv_sizeof_paged_attention_args(void) { return (int)sizeof(rdkv_paged_attention_args); }
+extern "C" int rdkv_paged_attention_status_words(void) { return PAGED_STATUS_WORDS; }
+
+extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const void* q, const void* k_pages, const void* v_pages,
+                                    const int32_t* block_tables, const int32_t* q_start, const int32_t* kv_lens, void* out,
+                                    int64_t out_tok_stride, int64_t out_head_stride, int zero_padding, float* out_partial,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+  if (args == nullptr) return RDKV_ERR_BAD_ARG;
+  const rdkv_paged_attention_args& g = *args;
+  if (g.n_tokens < 0 || g.n_requests < 0 || g.H_q <= 0 || g.H_kv <= 0 || g.n_pages < 0 || g.width < 0 || g.window < 0 || g.sinks < 0 ||
+      g.max_new < 0 || !(g.scale > 0.f))
     return RDKV_ERR_BAD_ARG;
-  if (dtype != RDKV_F16 && dtype != RDKV_BF16) return RDKV_ERR_BAD_ARG;
-  if (H_q % H_kv != 0 || H_q / H_kv > MAX_GROUP) return RDKV_ERR_BAD_SHAPE;
-  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) return RDKV_ERR_BAD_SHAPE;
-  if (n_tokens == 0) return RDKV_OK;
+  if (g.dtype != RDKV_F16 && g.dtype != RDKV_BF16) return RDKV_ERR_BAD_ARG;
+  if (g.H_q % g.H_kv != 0 || g.H_q / g.H_kv > MAX_GROUP) return RDKV_ERR_BAD_SHAPE;
+  if (g.page_size < 16 || g.page_size > 1024 || (g.page_size & (g.page_size - 1)) != 0) return RDKV_ERR_BAD_SHAPE;
+  if (g.n_tokens == 0) return RDKV_OK;
   if (q == nullptr || q_start == nullptr || (out == nullptr) == (out_partial == nullptr)) return RDKV_ERR_BAD_ARG;
-  if (n_requests > 0 && (kv_lens == nullptr || (width > 0 && block_tables == nullptr))) return RDKV_ERR_BAD_ARG;
-  if (n_pages > 0 && (k_pages == nullptr || v_pages == nullptr)) return RDKV_ERR_BAD_ARG;
+  if (g.n_requests > 0 && (kv_lens == nullptr || (g.width > 0 && block_tables == nullptr))) return RDKV_ERR_BAD_ARG;
+  if (g.n_pages > 0 && (k_pages == nullptr || v_pages == nullptr)) return RDKV_ERR_BAD_ARG;
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
-      workspace_bytes < rdkv_paged_attention_workspace(n_requests, n_tokens, H_q, H_kv, max_new))
+      workspace_bytes < rdkv_paged_attention_workspace(g.n_requests, g.n_tokens, g.H_q, g.H_kv, g.max_new))
     return RDKV_ERR_BAD_ARG;
   PagedArgs A = {};
   A.q = (const uint16_t*)q; A.k = (const uint16_t*)k_pages; A.v = (const uint16_t*)v_pages;
-  A.q_tok = q_tok_stride; A.q_head = q_head_stride;
-  A.k_page = k_page_stride; A.k_head = k_head_stride; A.k_row = k_row_stride;
-  A.v_page = v_page_stride; A.v_head = v_head_stride; A.v_row = v_row_stride;
-  A.n_pages = n_pages; A.page = page_size; A.H_q = H_q; A.H_kv = H_kv; A.g = H_q / H_kv;
-  for (A.page_log2 = 0; (1 << A.page_log2) < page_size; ++A.page_log2) {}
-  A.table = block_tables; A.table_stride = table_stride; A.width = width;
-  A.cap = (int)std::min<int64_t>((int64_t)width * page_size, 0x7fff0000);
-  A.q_start = q_start; A.kv_lens = kv_lens; A.S = n_requests; A.T = n_tokens;
-  A.window = std::min(window, 1 << 30); A.sinks = std::min(sinks, 1 << 30); A.scale_log2 = scale * PAGED_LOG2E;
+  A.q_tok = g.q_tok_stride; A.q_head = g.q_head_stride;
+  A.k_page = g.k_page_stride; A.k_head = g.k_head_stride; A.k_row = g.k_row_stride;
+  A.v_page = g.v_page_stride; A.v_head = g.v_head_stride; A.v_row = g.v_row_stride;
+  A.n_pages = g.n_pages; A.page = g.page_size; A.H_q = g.H_q; A.H_kv = g.H_kv; A.g = g.H_q / g.H_kv;
+  for (A.page_log2 = 0; (1 << A.page_log2) < g.page_size; ++A.page_log2) {}
+  A.table = block_tables; A.table_stride = g.table_stride; A.width = g.width;
+  A.cap = (int)std::min<int64_t>((int64_t)g.width * g.page_size, 0x7fff0000);
+  A.q_start = q_start; A.kv_lens = kv_lens; A.S = g.n_requests; A.T = g.n_tokens;
+  A.window = std::min(g.window, 1 << 30); A.sinks = std::min(g.sinks, 1 << 30); A.scale_log2 = g.scale * PAGED_LOG2E;
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
-  const bool bf = dtype == RDKV_BF16;
-  const bool few = paged_few_rows(max_new, A.g);
+  const bool bf = g.dtype == RDKV_BF16, few = paged_few_rows(g.max_new, A.g);
   A.group = few ? PAGED_DECODE_ROWS / A.g : 2 * (128 / A.g);
   paged_workspace(&A, workspace, few ? PAGED_DECODE_CTAS : PAGED_CHUNK_CTAS);
   CUtensorMap tm_k, tm_v;
-  const int box = std::min(page_size, few ? PAGED_DECODE_KEYS : PAGED_CHUNK_KEYS);
-  if (!paged_map(&tm_k, k_pages, bf, k_page_stride, k_head_stride, k_row_stride, n_pages, H_kv, page_size, box) ||
-      !paged_map(&tm_v, v_pages, bf, v_page_stride, v_head_stride, v_row_stride, n_pages, H_kv, page_size, box))
+  const int box = std::min(g.page_size, few ? PAGED_DECODE_KEYS : PAGED_CHUNK_KEYS);
+  if (!paged_map(&tm_k, k_pages, bf, g.k_page_stride, g.k_head_stride, g.k_row_stride, g.n_pages, g.H_kv, g.page_size, box) ||
+      !paged_map(&tm_v, v_pages, bf, g.v_page_stride, g.v_head_stride, g.v_row_stride, g.n_pages, g.H_kv, g.page_size, box))
     return RDKV_ERR_BAD_SHAPE;
   return few ? paged_decode_launch(A, bf, tm_k, tm_v, (cudaStream_t)stream) : paged_chunk_launch(A, bf, tm_k, tm_v, (cudaStream_t)stream);
 }

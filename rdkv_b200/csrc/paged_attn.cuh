@@ -65,6 +65,8 @@ int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, 
 int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st);
 constexpr int PAGED_CHUNK_ROWS = 256, PAGED_CHUNK_CTAS = PAGED_SMS, PAGED_CHUNK_KEYS = 128;
 constexpr int PAGED_DECODE_ROWS = 16, PAGED_DECODE_CTAS = 2 * PAGED_SMS, PAGED_DECODE_KEYS = 64;
+constexpr int PAGED_STATUS_WORDS = 2 * PAGED_SMS;   // one a CTA, of the larger grid
+static_assert(PAGED_STATUS_WORDS % 4 == 0 && PAGED_STATUS_WORDS >= PAGED_DECODE_CTAS && PAGED_STATUS_WORDS >= PAGED_CHUNK_CTAS);
 
 // A pair of 16-bit values: bits 15 and 31 of the result say which of them is not finite (its exponent is all ones: one more carries over).
 template <bool BF16>
@@ -377,6 +379,13 @@ __device__ __forceinline__ void paged_zero_padding(const PagedArgs& A, int n_thr
   }
 }
 
+// The CTA's status word (the first CTA also writes those of CTAs that the launch does not have).
+__device__ __forceinline__ void paged_report(const PagedArgs& A, int trouble) {
+  if (threadIdx.x == 0) A.status[blockIdx.x] = trouble;
+  if (blockIdx.x == 0)
+    for (int i = gridDim.x + threadIdx.x; i < PAGED_STATUS_WORDS; i += blockDim.x) A.status[i] = 0;
+}
+
 // Joins the records of items that a cut went through.  Block (c, y): if the cut in front of CTA c is the first one inside an
 // item, rows y, y + gridDim.y * 8, ... of that item, a warp each.  Its loads are three round trips: the places, the parts' m
 // and l together with the first parts' sums, the rest.
@@ -480,12 +489,12 @@ inline bool paged_map(CUtensorMap* tm, const void* base, bool bf16, int64_t page
 
 // Workspace of a launch of G CTAs whose items have up to `rows` rows.
 inline int64_t paged_workspace_bytes(int G, int rows) {
-  return (int64_t)(G + 1) * 32 + (((int64_t)G * 4 + 15) / 16) * 16 + (int64_t)2 * G * rows * RDKV_PARTIAL_STRIDE * 4;
+  return PAGED_STATUS_WORDS * 4 + (int64_t)(G + 1) * 32 + (int64_t)2 * G * rows * RDKV_PARTIAL_STRIDE * 4;
 }
 inline void paged_workspace(PagedArgs* A, void* workspace, int G) {
   char* p = static_cast<char*>(workspace);
+  A->status = reinterpret_cast<int*>(p); p += PAGED_STATUS_WORDS * 4;
   A->place = reinterpret_cast<int4*>(p); p += (int64_t)(G + 1) * 32;
-  A->status = reinterpret_cast<int*>(p); p += (((int64_t)G * 4 + 15) / 16) * 16;
   A->part = reinterpret_cast<float*>(p);
 }
 

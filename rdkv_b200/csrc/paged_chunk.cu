@@ -518,7 +518,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   tmem_fence_after();
   if (warp == CH_SOFTMAX_WARPS + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   paged_zero_padding(A, CH_THREADS);
-  if (tid == 0) A.status[cta] = s_trouble;
+  paged_report(A, s_trouble);
 }
 
 // A map over query rows [T][H_q][128] (strides in elements) whose boxes are 64 channels of g heads of `tokens` tokens.

@@ -27,18 +27,23 @@ inline cudaError_t allow_dynamic_smem(Kernel kernel, size_t most) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
 }
 
-// The same, asked for once per device (`most` is a constant of the kernel, so once is enough; at most 64 devices).
-template <auto Kernel>
-inline cudaError_t allow_dynamic_smem_once(size_t most) {
-  static std::atomic<uint64_t> done{0};
+// Calls `set` (something that stays with the current device) unless it succeeded there before; at most 64 devices are kept in mind.
+template <class Set>
+inline cudaError_t once_per_device(std::atomic<uint64_t>& done, Set set) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const uint64_t bit = (uint64_t)1 << (dev & 63);
   if (dev < 64 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
-  e = allow_dynamic_smem(Kernel, most);
+  e = set();
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
   return e;
+}
+// allow_dynamic_smem, once per device (`most` is a constant of the kernel).
+template <auto Kernel>
+inline cudaError_t allow_dynamic_smem_once(size_t most) {
+  static std::atomic<uint64_t> done{0};
+  return once_per_device(done, [&] { return allow_dynamic_smem(Kernel, most); });
 }
 
 inline int launch_status() {

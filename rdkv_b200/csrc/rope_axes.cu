@@ -136,7 +136,7 @@ rope_axes_kernel(const AxesArgs A) {
 
 // `sections` [n_axes] on the host; false if they are not 1 to 4 runs that cover the 64 frequencies.
 static bool axes_sections(AxesArgs* A, const int* sections, int n_axes) {
-  if (n_axes < 1 || n_axes > AXES_MAX || sections == nullptr) return false;
+  if (n_axes < 1 || n_axes > AXES_MAX) return false;
   int end = 0;
   for (int a = 0; a < n_axes; ++a) {
     if (sections[a] < 0 || sections[a] > 64) return false;
@@ -175,51 +175,51 @@ static bool axes_aligned(int dtype, std::initializer_list<const void*> bases, st
 
 using namespace rdkv;
 
-extern "C" int rdkv_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out, int64_t q_out_tok_stride,
-                              int64_t q_out_head_stride, int H_q, const void* k, int64_t k_tok_stride, int64_t k_head_stride,
-                              void* k_out, int64_t k_out_tok_stride, int64_t k_out_head_stride, int H_kv, int dtype, int n_tokens,
-                              const void* positions, int64_t axis_stride, int positions_64, const float* inv_freq,
-                              const int* sections, int n_axes, void* stream) {
-  if (n_tokens < 0 || H_q < 0 || H_kv < 0 || dtype < RDKV_F16 || dtype > RDKV_F32) return RDKV_ERR_BAD_ARG;
-  if (n_tokens > 0 && ((H_q > 0 && (q == nullptr || q_out == nullptr)) || (H_kv > 0 && (k == nullptr || k_out == nullptr)) ||
-                       positions == nullptr || inv_freq == nullptr))
+extern "C" int rdkv_sizeof_rope_axes_args(void) { return (int)sizeof(rdkv_rope_axes_args); }
+extern "C" int rdkv_sizeof_paged_append_args(void) { return (int)sizeof(rdkv_paged_append_args); }
+
+extern "C" int rdkv_rope_axes(const rdkv_rope_axes_args* args, const void* q, void* q_out, const void* k, void* k_out,
+                              const void* positions, const float* inv_freq, void* stream) {
+  if (args == nullptr) return RDKV_ERR_BAD_ARG;
+  const rdkv_rope_axes_args& g = *args;
+  if (g.n_tokens < 0 || g.H_q < 0 || g.H_kv < 0 || g.dtype < RDKV_F16 || g.dtype > RDKV_F32) return RDKV_ERR_BAD_ARG;
+  if (g.n_tokens > 0 && ((g.H_q > 0 && (q == nullptr || q_out == nullptr)) || (g.H_kv > 0 && (k == nullptr || k_out == nullptr)) ||
+                         positions == nullptr || inv_freq == nullptr))
     return RDKV_ERR_BAD_ARG;
   AxesArgs A = {};
-  if (!axes_sections(&A, sections, n_axes)) return RDKV_ERR_BAD_SHAPE;
+  if (!axes_sections(&A, g.sections, g.n_axes)) return RDKV_ERR_BAD_SHAPE;
   A.q = q; A.k = k; A.q_out = q_out; A.k_out = k_out;
-  A.q_tok = q_tok_stride; A.q_head = q_head_stride; A.k_tok = k_tok_stride; A.k_head = k_head_stride;
-  A.qo_tok = q_out_tok_stride; A.qo_head = q_out_head_stride; A.ko_tok = k_out_tok_stride; A.ko_head = k_out_head_stride;
-  A.positions = positions; A.pos_axis = axis_stride; A.pos64 = positions_64; A.inv_freq = inv_freq;
-  A.T = n_tokens; A.H_q = H_q; A.H_kv = H_kv;
-  A.aligned = axes_aligned(dtype, {q, k, q_out, k_out}, {A.q_tok, A.q_head, A.k_tok, A.k_head, A.qo_tok, A.qo_head, A.ko_tok, A.ko_head});
-  return axes_launch(A, dtype, false, (cudaStream_t)stream);
+  A.q_tok = g.q_tok_stride; A.q_head = g.q_head_stride; A.k_tok = g.k_tok_stride; A.k_head = g.k_head_stride;
+  A.qo_tok = g.q_out_tok_stride; A.qo_head = g.q_out_head_stride; A.ko_tok = g.k_out_tok_stride; A.ko_head = g.k_out_head_stride;
+  A.positions = positions; A.pos_axis = g.axis_stride; A.pos64 = g.positions_64; A.inv_freq = inv_freq;
+  A.T = g.n_tokens; A.H_q = g.H_q; A.H_kv = g.H_kv;
+  A.aligned = axes_aligned(g.dtype, {q, k, q_out, k_out}, {A.q_tok, A.q_head, A.k_tok, A.k_head, A.qo_tok, A.qo_head, A.ko_tok, A.ko_head});
+  return axes_launch(A, g.dtype, false, (cudaStream_t)stream);
 }
 
-extern "C" int rdkv_paged_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
-                                 int64_t v_head_stride, int H_kv, int dtype, int n_tokens, void* k_pages, int64_t k_page_stride,
-                                 int64_t k_page_head_stride, int64_t k_page_row_stride, void* v_pages, int64_t v_page_stride,
-                                 int64_t v_page_head_stride, int64_t v_page_row_stride, int n_pages, int page_size,
-                                 const int64_t* slot_map, const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
-                                 int64_t q_out_tok_stride, int64_t q_out_head_stride, int H_q, const void* positions,
-                                 int64_t axis_stride, int positions_64, const float* inv_freq, const int* sections, int n_axes,
-                                 void* stream) {
-  if (n_tokens < 0 || H_q < 0 || H_kv <= 0 || dtype < RDKV_F16 || dtype > RDKV_F32 || n_pages < 0 || page_size <= 0)
+extern "C" int rdkv_paged_append(const rdkv_paged_append_args* args, const void* k, const void* v, void* k_pages, void* v_pages,
+                                 const int64_t* slot_map, const void* q, void* q_out, const void* positions,
+                                 const float* inv_freq, void* stream) {
+  if (args == nullptr) return RDKV_ERR_BAD_ARG;
+  const rdkv_paged_append_args& g = *args;
+  if (g.n_tokens < 0 || g.H_q < 0 || g.H_kv <= 0 || g.dtype < RDKV_F16 || g.dtype > RDKV_F32 || g.n_pages < 0 || g.page_size <= 0)
     return RDKV_ERR_BAD_ARG;
-  if (n_tokens > 0 && (k == nullptr || v == nullptr || slot_map == nullptr || (n_pages > 0 && (k_pages == nullptr || v_pages == nullptr)) ||
-                       (H_q > 0 && (q == nullptr || q_out == nullptr)) || (n_axes > 0 && (positions == nullptr || inv_freq == nullptr))))
+  if (g.n_tokens > 0 &&
+      (k == nullptr || v == nullptr || slot_map == nullptr || (g.n_pages > 0 && (k_pages == nullptr || v_pages == nullptr)) ||
+       (g.H_q > 0 && (q == nullptr || q_out == nullptr)) || (g.n_axes > 0 && (positions == nullptr || inv_freq == nullptr))))
     return RDKV_ERR_BAD_ARG;
   AxesArgs A = {};
-  if (n_axes != 0 && !axes_sections(&A, sections, n_axes)) return RDKV_ERR_BAD_SHAPE;
+  if (g.n_axes != 0 && !axes_sections(&A, g.sections, g.n_axes)) return RDKV_ERR_BAD_SHAPE;
   A.q = q; A.k = k; A.v = v; A.q_out = q_out; A.k_out = k_pages; A.v_pages = v_pages;
-  A.q_tok = q_tok_stride; A.q_head = q_head_stride; A.k_tok = k_tok_stride; A.k_head = k_head_stride; A.v_tok = v_tok_stride;
-  A.v_head = v_head_stride; A.qo_tok = q_out_tok_stride; A.qo_head = q_out_head_stride;
-  A.kp_page = k_page_stride; A.kp_head = k_page_head_stride; A.kp_row = k_page_row_stride;
-  A.vp_page = v_page_stride; A.vp_head = v_page_head_stride; A.vp_row = v_page_row_stride;
-  A.slots = slot_map; A.n_slots = (int64_t)n_pages * page_size; A.page = page_size;
-  A.positions = positions; A.pos_axis = axis_stride; A.pos64 = positions_64; A.inv_freq = inv_freq;
-  A.T = n_tokens; A.H_q = H_q; A.H_kv = H_kv;
-  A.aligned = axes_aligned(dtype, {q, k, v, q_out, k_pages, v_pages},
+  A.q_tok = g.q_tok_stride; A.q_head = g.q_head_stride; A.k_tok = g.k_tok_stride; A.k_head = g.k_head_stride; A.v_tok = g.v_tok_stride;
+  A.v_head = g.v_head_stride; A.qo_tok = g.q_out_tok_stride; A.qo_head = g.q_out_head_stride;
+  A.kp_page = g.k_page_stride; A.kp_head = g.k_page_head_stride; A.kp_row = g.k_page_row_stride;
+  A.vp_page = g.v_page_stride; A.vp_head = g.v_page_head_stride; A.vp_row = g.v_page_row_stride;
+  A.slots = slot_map; A.n_slots = (int64_t)g.n_pages * g.page_size; A.page = g.page_size;
+  A.positions = positions; A.pos_axis = g.axis_stride; A.pos64 = g.positions_64; A.inv_freq = inv_freq;
+  A.T = g.n_tokens; A.H_q = g.H_q; A.H_kv = g.H_kv;
+  A.aligned = axes_aligned(g.dtype, {q, k, v, q_out, k_pages, v_pages},
                            {A.q_tok, A.q_head, A.k_tok, A.k_head, A.v_tok, A.v_head, A.qo_tok, A.qo_head, A.kp_page, A.kp_head, A.kp_row,
                             A.vp_page, A.vp_head, A.vp_row});
-  return axes_launch(A, dtype, true, (cudaStream_t)stream);
+  return axes_launch(A, g.dtype, true, (cudaStream_t)stream);
 }

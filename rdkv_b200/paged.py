@@ -19,12 +19,14 @@ the call), so calls on different streams and captured graphs do not share any.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import NamedTuple, Optional, Sequence
 
 import torch
 from torch import Tensor
 
-from ._lib import HEAD_DIM, PARTIAL_STRIDE, CallCache, check, lib, q_dtype_tag, raw_stream, require_cuda
+from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, check, lib, q_dtype_tag, raw_stream,
+                   require_cuda)
 from .rope import axes_check
 
 MAX_REQUESTS = 16384
@@ -137,8 +139,6 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     [T]: slot of every token; a slot below zero or behind the last page is not written.  The slots of a call must
     differ from one another.  q [T,H_q,128] of the same dtype goes to ``q_out`` (default: a new tensor; may be q
     itself), which is returned; k is not changed.  positions [T] or [axes,T], inv_freq and sections: see ``rope_axes``."""
-    if q is not None and q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), k_pages.shape, k_pages.stride(),
            k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype, v_pages.get_device(), slot_map.shape,
            slot_map.stride(), slot_map.dtype, slot_map.get_device(), None if sections is None else tuple(sections),
@@ -149,11 +149,13 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     call = _APPEND_CALLS.get(key)
     if call is None:
         call = _APPEND_CALLS.remember(key, _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sections, q_out))
-    ks, vs, kps, vps, qs, qos, ax, sec, index = call
+    args, _, index = call
+    if q is not None and q_out is None:
+        q_out = q.new_empty(q.shape)
     status = lib().rdkv_paged_append(
-        k.data_ptr(), *ks, v.data_ptr(), *vs, k_pages.data_ptr(), *kps, v_pages.data_ptr(), *vps, slot_map.data_ptr(),
-        None if q is None else q.data_ptr(), *qs, None if q is None else q_out.data_ptr(), *qos,
-        None if positions is None else positions.data_ptr(), *ax, None if positions is None else inv_freq.data_ptr(), *sec, raw_stream(index))
+        args, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slot_map.data_ptr(), None if q is None else q.data_ptr(),
+        None if q is None else q_out.data_ptr(), None if positions is None else positions.data_ptr(),
+        None if positions is None else inv_freq.data_ptr(), raw_stream(index))
     if status:
         check(status, "rdkv_paged_append")
     return q_out
@@ -175,8 +177,8 @@ def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sect
     tag = q_dtype_tag(k)
     if (positions is None) != (inv_freq is None) or (positions is None and (q is not None or sections is not None)):
         raise ValueError("q and sections need positions and inv_freq; positions needs inv_freq")
-    axes = (0, 0, None, 0) if positions is None else axes_check(positions, inv_freq, sections, T, dev)
-    qs, qos = (0, 0), (0, 0, 0)
+    axes = {} if positions is None else axes_check(positions, inv_freq, sections, T, dev)
+    qs, qos, H_q = (0, 0), (0, 0), 0
     if q is None:
         if q_out is not None:
             raise ValueError("q_out needs q")
@@ -184,17 +186,23 @@ def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sect
         require_cuda(q, "q")
         if q.dim() != 3 or q.shape[0] != T or q.shape[2] != HEAD_DIM or q.dtype != k.dtype or q.stride(2) != 1:
             raise ValueError(f"q must be [{T},H_q,{HEAD_DIM}] {k.dtype} with contiguous rows, got {tuple(q.shape)} {q.dtype}")
-        if q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
+        if q_out is not None and (q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1):
             raise ValueError("q_out must have q's shape and dtype and contiguous rows")
-        qs, qos = q.stride()[:2], (*q_out.stride()[:2], q.shape[1])
+        H_q = q.shape[1]
+        qs, qos = q.stride(), (H_q * HEAD_DIM, HEAD_DIM) if q_out is None else q_out.stride()
     _same_device(dev, v=v, k_pages=k_pages, v_pages=v_pages, slot_map=slot_map, q=q, q_out=q_out)
-    return (k.stride()[:2], (*v.stride()[:2], H_kv, tag, T), k_pages.stride()[:3], (*v_pages.stride()[:3], n_pages, page_size), qs, qos,
-            axes[:2], axes[2:], dev.index)
+    ks, vs, kp, vp = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
+    args = PagedAppendArgs(
+        k_tok_stride=ks[0], k_head_stride=ks[1], v_tok_stride=vs[0], v_head_stride=vs[1], k_page_stride=kp[0], k_page_head_stride=kp[1],
+        k_page_row_stride=kp[2], v_page_stride=vp[0], v_page_head_stride=vp[1], v_page_row_stride=vp[2], q_tok_stride=qs[0],
+        q_head_stride=qs[1], q_out_tok_stride=qos[0], q_out_head_stride=qos[1], H_q=H_q, H_kv=H_kv, dtype=tag, n_tokens=T, n_pages=n_pages,
+        page_size=page_size, **axes)
+    return C.addressof(args), args, dev.index
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: Tensor, q_start: Tensor, kv_lens: Tensor, *,
                     max_new: Optional[int] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
-                    out: Optional[Tensor] = None, out_partial: Optional[Tensor] = None) -> Tensor:
+                    out: Optional[Tensor] = None, out_partial: Optional[Tensor] = None, check_status: bool = False) -> Tensor:
     """Attention of a batch's new tokens over the pages of their requests.
 
     q [T,H_q,128] (fp16 / bf16, the pages' dtype, after rotation); k_pages, v_pages [n_pages,H_kv,page_size,128] with
@@ -205,8 +213,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     and the request's first ``sinks``.  Tokens whose page is missing (an entry outside the pages) are not seen, and what
     stands in masked places does not matter, whatever it is.  A token that sees nothing gets zeros.
 
-    max_new: the longest chunk of the batch, or a bound of it (default T); requests with more new tokens than that
-    get no result for the rest.  scale: of the scores, default 1/sqrt(128).
+    max_new: the longest chunk of the batch (default T), which chooses the kernel: a hint, results do not depend on it.
+    scale: of the scores, positive, default 1/sqrt(128).  check_status: wait for the kernels and raise if one of their
+    bounded waits ran out, in which case the results are invalid; without it the call returns at once.
     Returns ``out`` [T,H_q,128] in q's dtype.  Tokens behind the last request's are padding: zero in an ``out`` that the
     call allocates, left as they were in one that it is given.  ``out_partial`` float32 [T*H_q,132] receives
     un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
@@ -217,17 +226,19 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     call = _ATTENTION_CALLS.get(key)
     if call is None:
         call = _ATTENTION_CALLS.remember(key, _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_new, window, sinks, scale))
-    qs, ks, vs, shape, table, numbers, n_ws, index, tail = call
-    if not qs or q.data_ptr() & 15:                        # (rows that no 16-byte copy can fetch)
+    args, direct, n_ws, index, fields = call
+    if not direct or q.data_ptr() & 15:                    # (rows that no 16-byte copy can fetch)
         q = q.clone(memory_format=torch.contiguous_format)
-        qs = (*q.stride()[:2], *tail)
+        fields = PagedAttentionArgs.from_buffer_copy(fields)
+        fields.q_tok_stride, fields.q_head_stride = q.stride()[:2]
+        args = C.addressof(fields)
     k_ptr, v_ptr = k_pages.data_ptr(), v_pages.data_ptr()
     if (k_ptr | v_ptr) & 15:
         raise ValueError("k_pages and v_pages must start on 16 bytes")
     if out_partial is None:
         zero = 0
         if out is None:
-            out, zero = torch.empty_like(q, memory_format=torch.contiguous_format), 1
+            out, zero = q.new_empty(q.shape), 1
         else:
             require_cuda(out, "out")
             if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() % 16
@@ -243,11 +254,12 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
             raise ValueError(f"out_partial must be contiguous float32 [{q.shape[0] * q.shape[1]},{PARTIAL_STRIDE}] on {q.device}")
         os, out_ptr, rec_ptr, zero = (0, 0), None, out_partial.data_ptr(), 0
     ws = kv_lens.new_empty(n_ws)
-    status = lib().rdkv_paged_attention(
-        q.data_ptr(), *qs, k_ptr, *ks, v_ptr, *vs, *shape, block_tables.data_ptr(), *table, q_start.data_ptr(), kv_lens.data_ptr(), *numbers,
-        out_ptr, os[0], os[1], zero, rec_ptr, ws.data_ptr(), 4 * n_ws, raw_stream(index))
+    status = lib().rdkv_paged_attention(args, q.data_ptr(), k_ptr, v_ptr, block_tables.data_ptr(), q_start.data_ptr(), kv_lens.data_ptr(),
+                                        out_ptr, os[0], os[1], zero, rec_ptr, ws.data_ptr(), 4 * n_ws, raw_stream(index))
     if status:
         check(status, "rdkv_paged_attention")
+    if check_status and n_ws > 0 and bool(ws[:lib().rdkv_paged_attention_status_words()].any().item()):
+        raise RuntimeError("rdkv_paged_attention: a device-side wait ran out; the results are invalid")
     return out if out_partial is None else out_partial
 
 
@@ -282,8 +294,11 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
     if any(x % 8 for x in ks + vs):
         raise ValueError("k_pages and v_pages must have strides of whole 16 bytes")
     _same_device(q.device, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, q_start=q_start, kv_lens=kv_lens)
-    tail = (q_dtype_tag(q), T, H_q)
-    qs = () if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 else (*q.stride()[:2], *tail)
+    direct = q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0
     n_ws = -(-lib().rdkv_paged_attention_workspace(S, T, H_q, H_kv, max_new) // 4)
-    return (qs, ks, vs, (n_pages, H_kv, page_size), (block_tables.stride(0), block_tables.shape[1]), (S, max_new, int(window), int(sinks), scale),
-            n_ws, q.device.index, tail)
+    args = PagedAttentionArgs(
+        q_tok_stride=q.stride(0), q_head_stride=q.stride(1), k_page_stride=ks[0], k_head_stride=ks[1], k_row_stride=ks[2], v_page_stride=vs[0],
+        v_head_stride=vs[1], v_row_stride=vs[2], table_stride=block_tables.stride(0), dtype=q_dtype_tag(q), n_tokens=T, H_q=H_q, H_kv=H_kv,
+        n_pages=n_pages, page_size=page_size, width=block_tables.shape[1], n_requests=S, max_new=max_new, window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30),
+        scale=scale)
+    return C.addressof(args), direct, n_ws, q.device.index, args

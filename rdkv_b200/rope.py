@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import HEAD_DIM, CallCache, check, lib, ptr, q_dtype_tag, raw_stream, require_cuda, stream_ptr
+from ._lib import HEAD_DIM, CallCache, RopeAxesArgs, check, lib, ptr, q_dtype_tag, raw_stream, require_cuda, stream_ptr
 
 
 def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
@@ -40,7 +40,7 @@ _AXES_TAG = {torch.int32: 0, torch.int64: 1}
 
 
 def axes_check(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[int]], T: int, dev):
-    """(axis stride, 64-bit positions, C array of the sections, axes) of a call, as the library takes them."""
+    """The fields of a call's arguments that say how it rotates, by name."""
     half = HEAD_DIM // 2
     require_cuda(positions, "positions"); require_cuda(inv_freq, "inv_freq")
     n_axes = 1 if positions.dim() == 1 else positions.shape[0]
@@ -58,7 +58,8 @@ def axes_check(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[
         sections = (half,)
     if any(int(n) != n or n < 0 for n in sections) or sum(sections) != half or len(sections) != n_axes:
         raise ValueError(f"sections must be {n_axes} whole numbers (one an axis) that add up to {half}, got {tuple(sections)}")
-    return (0 if n_axes == 1 else positions.stride(0), _AXES_TAG[positions.dtype], (C.c_int * n_axes)(*(int(n) for n in sections)), n_axes)
+    return dict(axis_stride=0 if n_axes == 1 else positions.stride(0), positions_64=_AXES_TAG[positions.dtype], n_axes=n_axes,
+                sections=(C.c_int32 * 4)(*(int(n) for n in sections)))
 
 
 _ROPE_CALLS = CallCache()
@@ -74,32 +75,40 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     lose nothing (below 2^24).  sections: how many of the 64 frequencies each axis owns, in order (text
     with one axis: all of them).  Returns (q_out, k_out): new tensors, or the given ones, which may be q and k
     themselves."""
-    if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if k_out is None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), positions.shape, positions.stride(),
            positions.dtype, positions.get_device(), inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.get_device(),
-           None if sections is None else tuple(sections), q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device(), k_out.shape,
-           k_out.stride(), k_out.dtype, k_out.get_device())
+           None if sections is None else tuple(sections), None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device()),
+           None if k_out is None else (k_out.shape, k_out.stride(), k_out.dtype, k_out.get_device()))
     call = _ROPE_CALLS.get(key)
     if call is None:
-        for name, t in (("q", q), ("k", k)):
-            require_cuda(t, name)
-            if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
-                raise ValueError(f"{name} must be [T,heads,{HEAD_DIM}] with contiguous rows, got {tuple(t.shape)}")
-        T, dev = q.shape[0], q.device
-        if k.shape[0] != T or k.dtype != q.dtype or k.device != dev:
-            raise ValueError("q and k must have the same tokens, dtype and device")
-        for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
-            if t.shape != x.shape or t.dtype != x.dtype or t.device != dev or t.stride(2) != 1:
-                raise ValueError(f"{name} must have the shape, dtype and device of its input and contiguous rows")
-        axes = axes_check(positions, inv_freq, sections, T, dev)
-        call = _ROPE_CALLS.remember(key, (q.stride()[:2], (*q_out.stride()[:2], q.shape[1]), k.stride()[:2],
-                                          (*k_out.stride()[:2], k.shape[1], q_dtype_tag(q), T), axes[:2], axes[2:], dev.index))
-    qs, qos, ks, kos, ax, sec, index = call
-    status = lib().rdkv_rope_axes(q.data_ptr(), *qs, q_out.data_ptr(), *qos, k.data_ptr(), *ks, k_out.data_ptr(), *kos, positions.data_ptr(),
-                                  *ax, inv_freq.data_ptr(), *sec, raw_stream(index))
+        call = _ROPE_CALLS.remember(key, _rope_check(q, k, positions, inv_freq, sections, q_out, k_out))
+    args, _, index = call
+    if q_out is None:
+        q_out = q.new_empty(q.shape)
+    if k_out is None:
+        k_out = k.new_empty(k.shape)
+    status = lib().rdkv_rope_axes(args, q.data_ptr(), q_out.data_ptr(), k.data_ptr(), k_out.data_ptr(), positions.data_ptr(),
+                                  inv_freq.data_ptr(), raw_stream(index))
     if status:
         check(status, "rdkv_rope_axes")
     return q_out, k_out
+
+
+def _rope_check(q, k, positions, inv_freq, sections, q_out, k_out):
+    for name, t in (("q", q), ("k", k)):
+        require_cuda(t, name)
+        if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
+            raise ValueError(f"{name} must be [T,heads,{HEAD_DIM}] with contiguous rows, got {tuple(t.shape)}")
+    T, dev = q.shape[0], q.device
+    if k.shape[0] != T or k.dtype != q.dtype or k.device != dev:
+        raise ValueError("q and k must have the same tokens, dtype and device")
+    for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != dev or t.stride(2) != 1):
+            raise ValueError(f"{name} must have the shape, dtype and device of its input and contiguous rows")
+    (q0, q1), (k0, k1) = q.stride()[:2], k.stride()[:2]
+    qo = (q.shape[1] * HEAD_DIM, HEAD_DIM) if q_out is None else q_out.stride()
+    ko = (k.shape[1] * HEAD_DIM, HEAD_DIM) if k_out is None else k_out.stride()
+    args = RopeAxesArgs(q_tok_stride=q0, q_head_stride=q1, q_out_tok_stride=qo[0], q_out_head_stride=qo[1], k_tok_stride=k0, k_head_stride=k1,
+                        k_out_tok_stride=ko[0], k_out_head_stride=ko[1], H_q=q.shape[1], H_kv=k.shape[1], dtype=q_dtype_tag(q), n_tokens=T,
+                        **axes_check(positions, inv_freq, sections, T, dev))
+    return C.addressof(args), args, dev.index

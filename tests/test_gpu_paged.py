@@ -167,7 +167,7 @@ def run(lens, new, H_kv, g, page, dtype, seed=0, window=0, sinks=0, pad=0, max_n
     T = sum(new) + pad
     q = randn(T, H_kv * g, 128, seed=seed + 1, dtype=dtype) * 1.5
     most = max(new, default=0) if max_new == "true" else max_new
-    got = paged_attention(q, k, v, table, starts(new), ints(lens), max_new=most, window=window, sinks=sinks, **kw)
+    got = paged_attention(q, k, v, table, starts(new), ints(lens), max_new=most, window=window, sinks=sinks, check_status=True, **kw)
     check(got, R.attention(q, k, v, table, starts(new), ints(lens), window, sinks, kw.get("scale")), f"{lens} {new}")
     return q, k, v, table, got
 
@@ -192,7 +192,7 @@ def test_chunks(dtype, page, H_kv, g):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 0), (128, 64), (500, 200), (10000, 5), (33, 10000)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 0), (128, 64), (500, 200), (10000, 5), (33, 10000), (2 ** 40, 2 ** 40)])
 @pytest.mark.parametrize("g,page", [(4, 16), (3, 128)])
 def test_window_and_sinks(dtype, window, sinks, g, page):
     lens = [1, 17, 900, 600, 1301, 300]

@@ -11,19 +11,23 @@ def _lib():
 
 
 def _attention(**change):
-    a = dict(q=1 << 12, q_tok=1024, q_head=128, dtype=0, T=4, H_q=8, k=1 << 12, k_page=1, k_head=1, k_row=128, v=1 << 12, v_page=1, v_head=1,
-             v_row=128, n_pages=2, H_kv=2, page=16, table=1 << 12, stride=4, width=4, q_start=1 << 12, lens=1 << 12, S=1, max_new=4, window=0,
-             sinks=0, scale=1.0, out=1 << 12, o_tok=1024, o_head=128, pad=0, rec=None, ws=1 << 12, ws_bytes=1 << 40, stream=None)
-    assert set(change) <= set(a)
-    return _lib().rdkv_paged_attention(*{**a, **change}.values())
+    from rdkv_b200._lib import PagedAttentionArgs
+    p = 1 << 12
+    fields = dict(q_tok_stride=1024, q_head_stride=128, k_page_stride=1, k_head_stride=1, k_row_stride=128, v_page_stride=1, v_head_stride=1,
+                  v_row_stride=128, table_stride=4, dtype=0, n_tokens=4, H_q=8, H_kv=2, n_pages=2, page_size=16, width=4, n_requests=1, max_new=4,
+                  window=0, sinks=0, scale=1.0)
+    rest = dict(q=p, k=p, v=p, table=p, q_start=p, lens=p, out=p, o_tok=1024, o_head=128, pad=0, rec=None, ws=p, ws_bytes=1 << 40, stream=None)
+    assert set(change) <= set(fields) | set(rest)
+    args = PagedAttentionArgs(**{n: change.get(n, x) for n, x in fields.items()})
+    return _lib().rdkv_paged_attention(C.addressof(args), *(change.get(n, x) for n, x in rest.items()))
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(T=-1), 1), (dict(S=-1), 1), (dict(H_q=0), 1), (dict(H_kv=0), 1), (dict(dtype=2), 1), (dict(dtype=7), 1), (dict(window=-1), 1),
-    (dict(sinks=-1), 1), (dict(max_new=-1), 1), (dict(width=-1), 1), (dict(n_pages=-1), 1), (dict(H_kv=3), 2), (dict(H_q=34), 2), (dict(page=8), 2),
-    (dict(page=24), 2), (dict(page=2048), 2), (dict(q=None), 1), (dict(q_start=None), 1), (dict(lens=None), 1), (dict(table=None), 1),
+    (dict(n_tokens=-1), 1), (dict(n_requests=-1), 1), (dict(H_q=0), 1), (dict(H_kv=0), 1), (dict(dtype=2), 1), (dict(dtype=7), 1), (dict(window=-1), 1),
+    (dict(sinks=-1), 1), (dict(max_new=-1), 1), (dict(width=-1), 1), (dict(n_pages=-1), 1), (dict(H_kv=3), 2), (dict(H_q=34), 2), (dict(page_size=8), 2),
+    (dict(page_size=24), 2), (dict(page_size=2048), 2), (dict(q=None), 1), (dict(q_start=None), 1), (dict(lens=None), 1), (dict(table=None), 1),
     (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(rec=1 << 12), 1), (dict(scale=0.0), 1), (dict(scale=-1.0), 1), (dict(scale=float('nan')), 1), (dict(ws=None), 1), (dict(ws=(1 << 12) + 8), 1), (dict(ws_bytes=100), 1),
-    (dict(T=0, q=None), 0)])
+    (dict(n_tokens=0, q=None), 0)])
 def test_attention_refusals(change, status):
     assert _attention(**change) == status
 
@@ -44,19 +48,31 @@ def test_tables_refusals():
 
 
 def test_rotation_and_append_refusals():
+    from rdkv_b200._lib import PagedAppendArgs, RopeAxesArgs
     lib, p = _lib(), 1 << 12
-    sec = lambda *n: (C.c_int * len(n))(*n)
-    rope = lambda *, dtype=0, T=2, q=p, k=p, pos=p, inv=p, sections=sec(64), axes=1: lib.rdkv_rope_axes(
-        q, 512, 128, p, 512, 128, 4, k, 128, 128, p, 128, 128, 1, dtype, T, pos, 2, 0, inv, sections, axes, None)
-    assert rope(dtype=3) == 1 and rope(T=-1) == 1 and rope(q=None) == 1 and rope(k=None) == 1 and rope(pos=None) == 1 and rope(inv=None) == 1
-    assert rope(sections=None) == 2 and rope(axes=0) == 2 and rope(axes=5) == 2 and rope(sections=sec(63)) == 2
-    assert rope(sections=sec(70, -6), axes=2) == 2 and rope(T=0) == 0
-    append = lambda *, dtype=0, T=2, H_kv=1, k=p, v=p, kp=p, vp=p, page=16, slots=p, q=p, q_out=p, H_q=4, pos=p, inv=p, sections=sec(64), axes=1: \
-        lib.rdkv_paged_append(k, 128, 128, v, 128, 128, H_kv, dtype, T, kp, 2048, 2048, 128, vp, 2048, 2048, 128, 3, page, slots, q, 512, 128,
-                              q_out, 512, 128, H_q, pos, 2, 0, inv, sections, axes, None)
-    assert append(dtype=-1) == 1 and append(T=-1) == 1 and append(H_kv=0) == 1 and append(k=None) == 1 and append(v=None) == 1
-    assert append(kp=None) == 1 and append(vp=None) == 1 and append(page=0) == 1 and append(slots=None) == 1 and append(q=None) == 1
-    assert append(q_out=None) == 1 and append(pos=None) == 1 and append(inv=None) == 1 and append(sections=sec(60)) == 2 and append(T=0) == 0
+
+    def call(mirror, function, fields, rest, change):
+        assert set(change) <= set(fields) | set(rest)
+        fields = {n: change.get(n, x) for n, x in fields.items()}
+        fields["sections"] = (C.c_int32 * 4)(*fields["sections"])
+        args = mirror(**fields)
+        return function(C.addressof(args), *(change.get(n, x) for n, x in rest.items()), None)
+
+    def rope(**change):
+        return call(RopeAxesArgs, lib.rdkv_rope_axes, dict(H_q=4, H_kv=1, dtype=0, n_tokens=2, n_axes=1, sections=(64,)),
+                    dict(q=p, q_out=p, k=p, k_out=p, pos=p, inv=p), change)
+    assert rope(dtype=3) == 1 and rope(n_tokens=-1) == 1 and rope(q=None) == 1 and rope(k=None) == 1 and rope(pos=None) == 1 and rope(inv=None) == 1
+    assert rope(q_out=None) == 1 and rope(k_out=None) == 1 and rope(n_axes=0) == 2 and rope(n_axes=5) == 2 and rope(sections=(63,)) == 2
+    assert rope(sections=(70, -6), n_axes=2) == 2 and rope(n_tokens=0) == 0 and lib.rdkv_rope_axes(None, p, p, p, p, p, p, None) == 1
+
+    def append(**change):
+        return call(PagedAppendArgs, lib.rdkv_paged_append,
+                    dict(H_q=4, H_kv=1, dtype=0, n_tokens=2, n_pages=3, page_size=16, n_axes=1, sections=(64,)),
+                    dict(k=p, v=p, kp=p, vp=p, slots=p, q=p, q_out=p, pos=p, inv=p), change)
+    assert append(dtype=-1) == 1 and append(n_tokens=-1) == 1 and append(H_kv=0) == 1 and append(k=None) == 1 and append(v=None) == 1
+    assert append(kp=None) == 1 and append(vp=None) == 1 and append(page_size=0) == 1 and append(slots=None) == 1 and append(q=None) == 1
+    assert append(q_out=None) == 1 and append(pos=None) == 1 and append(inv=None) == 1 and append(sections=(60,)) == 2 and append(n_tokens=0) == 0
+    assert lib.rdkv_paged_append(None, p, p, p, p, p, p, p, p, p, None) == 1
 
 
 def test_host_tensors_are_refused():

@@ -115,7 +115,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     } else {
       let_next_kernel_start();
       PagedPlace from, to;
-      paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP, DEC_WHOLE>(A, cta, PAGED_DECODE_CTAS, s_place, from, to);   // (its barriers order the set-up too)
+      paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP, DEC_WHOLE, PAGED_DECODE_CTAS>(A, cta, s_place, from, to);   // (its barriers order the set-up too)
       return DecWalk<false>(A, from, to);
     }
   };
@@ -526,6 +526,9 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
   const bool bf = g.dtype == RDKV_BF16, few = paged_few_rows(g.max_new, A.g);
   A.group = few ? PAGED_DECODE_ROWS / A.g : 2 * (128 / A.g);
+  // a head's line of units has to fit 31 bits: (groups of new tokens) x (tiles of the longest request the table has room for)
+  const int64_t groups = (int64_t)g.n_tokens / A.group + g.n_requests + 1, tiles = A.cap / (few ? PAGED_DECODE_KEYS : PAGED_CHUNK_KEYS) + 4;
+  if (groups * tiles > 0x7fffffffLL) return RDKV_ERR_TOO_LARGE;
   paged_workspace(&A, workspace, few ? PAGED_DECODE_CTAS : PAGED_CHUNK_CTAS);
   CUtensorMap tm_k, tm_v;
   const int box = std::min(g.page_size, few ? PAGED_DECODE_KEYS : PAGED_CHUNK_KEYS);

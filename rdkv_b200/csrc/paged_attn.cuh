@@ -121,30 +121,29 @@ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& A, const PagedR
 __device__ __forceinline__ int paged_tile(const PagedItem& it, int k) { return k < it.t_sink ? k : it.t_lo + k - it.t_sink; }
 
 // ── the line of units ───────────────────────────────────────────────────────
-struct PagedPlace { int i, head, group, tile; };  // i = S: the end
+struct PagedPlace { int i, head, group, tile; };  // head = H_kv: the end
 
-struct PagedPlaceScratch { uint64_t part[32]; uint32_t most[32]; uint64_t at[2]; uint32_t width[2]; int request[2]; int4 found[2], item; };
+struct PagedPlaceScratch { uint32_t part[32], most[32], groups[32]; uint32_t at[2]; int request[2]; int4 found[2], item; };
 
-// Where the parts of CTA c of G start and end.  All threads of the block (NT, whole warps) call it.  FIXED: cost of an item besides its
-// tiles; a cut that would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.  With no more
-// items than CTAs, and none more than WHOLE units over its share, every CTA gets a whole item: a cut costs both its sides
-// an item's records, written and read again.
-template <int KEYS, int NT, int FIXED, int SNAP, int WHOLE>
-__device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, PagedPlaceScratch& s, PagedPlace& from, PagedPlace& to) {
+// Where the part of CTA c of G starts and ends.  All threads of the block (NT, whole warps) call it.  The line goes through
+// the heads, in a head through the requests, in a request through its groups.  FIXED: cost of an item besides its tiles; a cut that
+// would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.  With no more items than CTAs, and
+// none more than WHOLE units over its share, every CTA gets a whole item: a cut costs both its sides an item's records,
+// written and read again.  The launcher has seen to it that a head's units fit 31 bits.  (Every launch pays for this code from
+// a cold instruction cache: in 64 bits, with two divisions more, it took 7400 cycles.)
+template <int KEYS, int NT, int FIXED, int SNAP, int WHOLE, int G>
+__device__ __forceinline__ void paged_place(const PagedArgs& A, int c, PagedPlaceScratch& s, PagedPlace& from, PagedPlace& to) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // units of a head of request i, its groups, its costliest item
-  auto units = [&](int i, int& groups, uint32_t& most) -> uint32_t {
+  auto units = [&](int i, uint32_t& groups_, uint32_t& most) -> uint32_t {
     PagedRequest r = {0, 0, 0};
     if (i < A.S) r = paged_request(A, i);
-    groups = paged_groups(A, r);
+    const int groups = paged_groups(A, r);
+    groups_ = (uint32_t)groups;
     uint32_t sum = 0;
     most = 0;
-    if (groups <= 4)
-      for (int x = 0; x < groups; ++x) {
-        const uint32_t cost = paged_item<KEYS>(A, r, x).n + FIXED;
-        sum += cost; most = max(most, cost);
-      }
-    unsigned many = __ballot_sync(0xffffffffu, groups > 4);   // long chunks: the warp's lanes take their groups
+    if (groups == 1) sum = most = paged_item<KEYS>(A, r, 0).n + FIXED;
+    unsigned many = __ballot_sync(0xffffffffu, groups > 1);   // chunks: the warp's lanes take their groups
     while (many != 0) {
       const int from_lane = __ffs(many) - 1;
       many &= many - 1;
@@ -153,6 +152,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
       o.len = __shfl_sync(0xffffffffu, r.len, from_lane);
       const int n = paged_groups(A, o);
       uint32_t mine = 0, top = 0;
+#pragma unroll 1
       for (int x = lane; x < n; x += 32) {
         const uint32_t cost = paged_item<KEYS>(A, o, x).n + FIXED;
         mine += cost; top = max(top, cost);
@@ -163,96 +163,99 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
     }
     return sum;
   };
-  auto block_scan = [&](uint64_t x, uint64_t& before, uint64_t& all) {   // exclusive sum over the block's threads
-    uint64_t incl = x;
+  auto warp_scan = [&](uint32_t x) {                          // inclusive
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const uint64_t y = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += y;
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
     }
+    return x;
+  };
+  auto block_scan = [&](uint32_t x, uint32_t& all) {          // exclusive
+    const uint32_t incl = warp_scan(x);
     __syncthreads();
     if (lane == 31) s.part[warp] = incl;
     __syncthreads();
-    before = incl - x; all = 0;
+    uint32_t before = incl - x;
+    all = 0;
 #pragma unroll
     for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) before += s.part[w];
-      all += s.part[w];
+      const uint32_t y = s.part[w];
+      before += w < warp ? y : 0u;
+      all += y;
     }
+    return before;
   };
-  if (tid < 2) s.request[tid] = A.S;
-  // units in the low 40 bits, items above them
-  constexpr int BITS = 40;
-  constexpr uint64_t LOW = ((uint64_t)1 << BITS) - 1;
-  uint64_t total = 0, before = 0, all = 0, mine = 0;
-  uint32_t most = 0;
+  if (tid < 2) s.request[tid] = -1;
+  uint32_t total = 0, mine = 0, groups = 0, n_groups = 0, most = 0, before = 0, all = 0;
   for (int base = 0; base < A.S; base += NT) {
-    int groups;
     uint32_t top;
     mine = units(base + tid, groups, top);
-    mine |= (uint64_t)groups << BITS;
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) s.most[warp] = top;
-    block_scan(mine, before, all);
+    const uint32_t sum = __reduce_add_sync(0xffffffffu, groups);
+    if (base > 0) __syncthreads();                            // (the round before has been read)
+    if (lane == 0) { s.most[warp] = top; s.groups[warp] = sum; }
+    before = block_scan(mine, all);
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) most = max(most, s.most[w]);
+    for (int w = 0; w < NT / 32; ++w) { most = max(most, s.most[w]); n_groups += s.groups[w]; }
     total += all;
   }
-  const uint64_t n_items = (total >> BITS) * (uint64_t)A.H_kv, n_units = (total & LOW) * (uint64_t)A.H_kv;
-  const bool whole = n_items <= (uint64_t)G && most <= (uint32_t)(n_units / (uint64_t)G) + WHOLE;
-  auto pick = [&](uint64_t x) { return whole ? x >> BITS : x & LOW; };
-  const uint64_t cut[2] = {whole ? (uint64_t)c : (uint64_t)c * n_units / (uint64_t)G, whole ? (uint64_t)c + 1 : (uint64_t)(c + 1) * n_units / (uint64_t)G};
-  uint64_t run = 0;
+  const bool whole = (uint64_t)n_groups * A.H_kv <= (uint64_t)G && most <= (uint32_t)((uint64_t)total * A.H_kv / G) + WHOLE;
+  // cut e: its head, and its place in the head's line
+  int head[2];
+  uint32_t cut[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (whole) {
+      head[e] = n_groups > 0 ? min((c + e) / (int)n_groups, A.H_kv) : A.H_kv;
+      cut[e] = (uint32_t)(c + e - head[e] * (int)n_groups);
+    } else {
+      const int x = (c + e) * A.H_kv;
+      head[e] = x / G;
+      cut[e] = (uint32_t)((uint64_t)(x - head[e] * G) * total / G);
+    }
+  }
+  if (whole) { total = n_groups; if (A.S <= NT) { mine = groups; before = block_scan(mine, all); } }
+  uint32_t run = 0;
   for (int base = 0; base < A.S; base += NT) {
     if (A.S > NT) {
-      int groups;
       uint32_t top;
       mine = units(base + tid, groups, top);
-      mine |= (uint64_t)groups << BITS;
-      block_scan(mine, before, all);
+      if (whole) mine = groups;
+      before = block_scan(mine, all);
     }
-    const uint64_t a = (pick(run) + pick(before)) * A.H_kv, b = a + pick(mine) * A.H_kv;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (cut[e] >= a && cut[e] < b) { s.request[e] = base + tid; s.at[e] = cut[e] - a; s.width[e] = (uint32_t)pick(mine); }
+      if (head[e] < A.H_kv && cut[e] - (run + before) < mine) { s.request[e] = base + tid; s.at[e] = cut[e] - (run + before); }
     run += all;
   }
   __syncthreads();
-  if (warp < 2) {                                 // warp e: the head, group and tile of cut e
+  if (warp < 2) {                                 // warp e: the group and tile of cut e
     const int i = s.request[warp];
-    int4 found = make_int4(A.S, 0, 0, 0);
-    if (i < A.S) {
+    if (i >= 0) {
       const PagedRequest r = paged_request(A, i);
-      const int groups = paged_groups(A, r);
-      const uint32_t width = s.width[warp];
-      const uint64_t at = s.at[warp];
-      const int head = at >> 32 == 0 ? (int)((uint32_t)at / width) : (int)(at / width);
-      uint32_t left = (uint32_t)(at - (uint64_t)head * width);
-      for (int x0 = 0; x0 < groups; x0 += 32) {
-        const PagedItem it = paged_item<KEYS>(A, r, min(x0 + lane, groups - 1));
-        const int n = it.n;
-        const uint32_t cost = x0 + lane < groups ? (whole ? 1 : n + FIXED) : 0;
-        uint32_t incl = cost;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const uint32_t y = __shfl_up_sync(0xffffffffu, incl, d);
-          if (lane >= d) incl += y;
-        }
-        const uint32_t sum = __shfl_sync(0xffffffffu, incl, 31);
-        if (left < sum) {
-          if (left >= incl - cost && left < incl) {
-            int tile = max(0, (int)(left - (incl - cost)) - FIXED);
+      const int n_mine = paged_groups(A, r);
+      uint32_t left = s.at[warp];
+#pragma unroll 1
+      for (int x0 = 0;; x0 += 32) {
+        const PagedItem it = paged_item<KEYS>(A, r, min(x0 + lane, n_mine - 1));
+        const uint32_t cost = x0 + lane < n_mine ? (whole ? 1u : (uint32_t)(it.n + FIXED)) : 0u;
+        const uint32_t incl = warp_scan(cost), sum = __shfl_sync(0xffffffffu, incl, 31);
+        if (left < sum || x0 + 32 >= n_mine) {
+          const uint32_t off = left - (incl - cost);
+          if (off < cost) {
+            int tile = whole ? 0 : max(0, (int)off - FIXED);
             if (tile < SNAP) tile = 0;
-            else if (n - tile < SNAP) tile = n;
-            s.found[warp] = make_int4(i, head, x0 + lane, tile);
-            if (warp == 0) s.item = make_int4(n, it.n_tok * A.g, it.tok0, 0);
+            else if (it.n - tile < SNAP) tile = it.n;
+            s.found[warp] = make_int4(i, warp == 0 ? head[0] : head[1], x0 + lane, tile);
+            if (warp == 0) s.item = make_int4(it.n, it.n_tok * A.g, it.tok0, 0);
           }
           break;
         }
         left -= sum;
       }
     } else if (lane == 0) {
-      s.found[warp] = found;
+      s.found[warp] = make_int4(0, A.H_kv, 0, 0);
       if (warp == 0) s.item = make_int4(0, 0, 0, 0);
     }
   }
@@ -262,7 +265,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, int G, Pa
   to = {t.x, t.y, t.z, t.w};
   if (tid == 0) {
     A.place[2 * c] = f; A.place[2 * c + 1] = s.item;
-    if (c == G - 1) A.place[2 * G] = make_int4(A.S, 0, 0, 0);
+    if (c == G - 1) A.place[2 * G] = make_int4(0, A.H_kv, 0, 0);
   }
 }
 
@@ -283,13 +286,17 @@ struct PagedWalk {
   }
   __device__ __forceinline__ void load(const PagedArgs& A) {
     groups = 0;
-    if (at.i < A.S) { r = paged_request(A, at.i); groups = paged_groups(A, r); }
+    if (at.head < A.H_kv) { r = paged_request(A, at.i); groups = paged_groups(A, r); }
+  }
+  __device__ __forceinline__ void next_request(const PagedArgs& A) {
+    at.group = at.tile = 0;
+    if (++at.i == A.S) { at.i = 0; ++at.head; }
+    load(A);
   }
   __device__ __forceinline__ bool next(const PagedArgs& A, PagedSegment& s) {
-    while (!done && at.i < A.S) {
-      if (at.i > to.i) { done = true; break; }
-      if (groups == 0) { ++at.i; at.head = at.group = at.tile = 0; load(A); continue; }
-      const bool last = at.i == to.i && at.head == to.head && at.group == to.group;
+    while (!done && at.head < A.H_kv) {
+      if (groups == 0) { next_request(A); continue; }
+      const bool last = at.head == to.head && at.i == to.i && at.group == to.group;
       s.request = r; s.i = at.i; s.head = at.head; s.group = at.group;
       s.item = paged_item<KEYS>(A, r, at.group);
       s.k0 = at.tile;
@@ -297,10 +304,7 @@ struct PagedWalk {
       const bool some = s.k0 < s.k1 || (s.item.n == 0 && s.k0 == 0 && !last);
       at.tile = 0;
       if (last) done = true;
-      else if (++at.group == groups) {
-        at.group = 0;
-        if (++at.head == A.H_kv) { at.head = 0; ++at.i; load(A); }
-      }
+      else if (++at.group == groups) next_request(A);
       if (some) return true;
     }
     return false;
@@ -399,7 +403,7 @@ paged_join_kernel(const PagedArgs A) {
   wait_for_previous_kernel();
   const int4 at = A.place[2 * c], item = A.place[2 * c + 1], prev = A.place[2 * c - 2];
   int4 a = A.place[2 * min(c + tid, G)], b = A.place[2 * min(c + tid + 1, G)];
-  if (at.x >= A.S || at.w == 0 || at.w >= item.x) return;
+  if (at.y >= A.H_kv || at.w == 0 || at.w >= item.x) return;
   if (prev.x == at.x && prev.y == at.y && prev.z == at.z && prev.w > 0) return;   // an earlier cut is in this item
   // the CTAs from c on that start inside the item (a run), and which of them have tiles of it
   int n_parts = 1;

@@ -465,10 +465,14 @@ static int decode_line(const PagedArgs& A, const CUtensorMap& tm_k, const CUtens
   return paged_launch_join(paged_join_kernel<BF16, DEC_ROWS, PAGED_DECODE_CTAS>, A, dim3(PAGED_DECODE_CTAS - 1, DEC_ROWS / PAGED_JOIN_WARPS), st);
 }
 
+// Items that the decode kernel gives a cluster of eight CTAs or more each.
+static bool paged_few_items(int64_t n_requests, int H_kv) { return n_requests * H_kv * 8 <= PAGED_DECODE_CTAS; }
+
 int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
-  // Few items: a cluster each, as long as eight CTAs an item fit the GPU at once.  (One request of 1061 tokens, 8 heads: see above.)
+  // Few items: a cluster each, as long as eight CTAs an item fit the GPU at once.  (One request of 1061 tokens, 8 heads: 17.3 us on the
+  // line of units with its second launch, 8.6 in clusters of 16.)
   const int64_t items = (int64_t)A.S * A.H_kv;
-  if (items > 0 && items * 8 <= PAGED_DECODE_CTAS) {
+  if (items > 0 && paged_few_items(A.S, A.H_kv)) {
     const int size = items * 16 <= PAGED_DECODE_CTAS ? 16 : 8;
     return bf16 ? decode_cluster<true>(A, (unsigned)(items * size), (unsigned)size, tm_k, tm_v, st)
                 : decode_cluster<false>(A, (unsigned)(items * size), (unsigned)size, tm_k, tm_v, st);
@@ -480,13 +484,19 @@ int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, 
 
 using namespace rdkv;
 
-// Rows of a request's longest chunk under one KV head decide the kernel: up to 16 fill one tile of the decode kernel.
-static bool paged_few_rows(int max_new, int g) { return (int64_t)max_new * g <= PAGED_DECODE_ROWS; }
+// Rows of a request's longest chunk under one KV head decide the kernel: up to 16 fill one tile of the decode kernel, up to 24 (two
+// tiles, which read the keys twice, the second time from L2) are still faster there unless clusters would take the two in
+// turn.  (8 KV heads, us, decode kernel / chunk kernel: 16 requests x 4000 tokens, 20 rows 40 / 52; 64 x 4000, 20 rows 106 / 120 and 32 rows
+// 141 / 123; 200 x 1000, 20 rows 101 / 133; one request of 30000, 32 rows 72 / 45.)
+static bool paged_few_rows(int n_requests, int H_kv, int max_new, int g) {
+  const int64_t rows = (int64_t)max_new * g;
+  return rows <= PAGED_DECODE_ROWS || (rows <= PAGED_DECODE_ROWS + 8 && !paged_few_items(n_requests, H_kv));
+}
 
 extern "C" int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, int H_q, int H_kv, int max_new) {
   if (n_requests < 0 || n_tokens < 0 || H_q <= 0 || H_kv <= 0 || max_new < 0) return -1;
   if (n_tokens == 0) return 0;
-  return paged_few_rows(max_new, H_q / H_kv) ? paged_workspace_bytes(PAGED_DECODE_CTAS, PAGED_DECODE_ROWS)
+  return paged_few_rows(n_requests, H_kv, max_new, H_q / H_kv) ? paged_workspace_bytes(PAGED_DECODE_CTAS, PAGED_DECODE_ROWS)
                                              : paged_workspace_bytes(PAGED_CHUNK_CTAS, PAGED_CHUNK_ROWS);
 }
 
@@ -524,7 +534,7 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
   A.q_start = q_start; A.kv_lens = kv_lens; A.S = g.n_requests; A.T = g.n_tokens;
   A.window = std::min(g.window, 1 << 30); A.sinks = std::min(g.sinks, 1 << 30); A.scale_log2 = g.scale * PAGED_LOG2E;
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
-  const bool bf = g.dtype == RDKV_BF16, few = paged_few_rows(g.max_new, A.g);
+  const bool bf = g.dtype == RDKV_BF16, few = paged_few_rows(g.n_requests, g.H_kv, g.max_new, A.g);
   A.group = few ? PAGED_DECODE_ROWS / A.g : 2 * (128 / A.g);
   // a head's line of units has to fit 31 bits: (groups of new tokens) x (tiles of the longest request the table has room for)
   const int64_t groups = (int64_t)g.n_tokens / A.group + g.n_requests + 1, tiles = A.cap / (few ? PAGED_DECODE_KEYS : PAGED_CHUNK_KEYS) + 4;

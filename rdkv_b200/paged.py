@@ -55,6 +55,14 @@ def _same_device(dev, **tensors: Optional[Tensor]) -> None:
             raise ValueError(f"{name} must live on {dev}, got {t.device}")
 
 
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the bytes from the first element to the last of two tensors meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    end = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) for t in (a, b)]
+    return a.data_ptr() < end[1] and b.data_ptr() < end[0]
+
+
 def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor, free_pages: Tensor, page_size: int, n_tokens: int,
                        *, free_start: Optional[Tensor] = None, out: Optional[PagedPlan] = None) -> PagedPlan:
     """Gives the requests of a step the pages they lack and every new token its slot; one launch.
@@ -68,7 +76,8 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
 
     A page that is not to be had (the free list is used up: entry -1; the table is too narrow: no entry) leaves its
     tokens without a slot (-1): :func:`append_kv` does not write them and :func:`paged_attention` does not see them.
-    ``missing`` counts such pages.  ``out``: a plan of the same S and n_tokens to write into (for captured steps)."""
+    ``missing`` counts such pages.  ``out``: a plan of the same S and n_tokens to write into; it must not share memory with the
+    arguments (a step's ``kv_lens`` are the next one's ``ctx_lens``: take two plans in turn, or copy)."""
     n_tokens, page_size = int(n_tokens), int(page_size)
     key = (ctx_lens.shape, ctx_lens.stride(), ctx_lens.dtype, ctx_lens.get_device(), new_lens.shape, new_lens.stride(), new_lens.dtype,
            new_lens.get_device(), block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.get_device(), free_pages.shape,
@@ -106,8 +115,11 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
         if out.slot_map.dtype != torch.int64 or tuple(out.slot_map.shape) != (n_tokens,) or not out.slot_map.is_contiguous():
             raise ValueError(f"out.slot_map must be a contiguous int64 tensor of {n_tokens} elements")
         _same_device(ctx_lens.device, **{f"out.{n}": t for n, t in out._asdict().items()})
-        if free_start is not None and out.free_next.data_ptr() == free_start.data_ptr():
-            raise ValueError("out.free_next must not be free_start itself (other blocks of the launch still read it)")
+        for name, t in out._asdict().items():
+            for other, x in (("ctx_lens", ctx_lens), ("new_lens", new_lens), ("free_pages", free_pages), ("free_start", free_start),
+                             ("block_tables", block_tables)):
+                if x is not None and _overlap(t, x):
+                    raise ValueError(f"out.{name} shares memory with {other}, which other blocks of the launch still read")
     slot_map, positions, q_start, kv_lens, free_next, missing = out
     status = lib().rdkv_paged_tables(
         ctx_lens.data_ptr(), new_lens.data_ptr(), S, block_tables.data_ptr(), *table, free_pages.data_ptr(), n_free,
@@ -217,7 +229,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     scale: of the scores, positive, default 1/sqrt(128).  check_status: wait for the kernels and raise if one of their
     bounded waits ran out, in which case the results are invalid; without it the call returns at once.
     Returns ``out`` [T,H_q,128] in q's dtype.  Tokens behind the last request's are padding: zero in an ``out`` that the
-    call allocates, left as they were in one that it is given.  ``out_partial`` float32 [T*H_q,132] receives
+    call allocates, left as they were in one that it is given (which must not be q itself).  ``out_partial`` float32 [T*H_q,132] receives
     un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape,
            v_pages.stride(), v_pages.dtype, v_pages.get_device(), block_tables.shape, block_tables.stride(), block_tables.dtype,
@@ -244,6 +256,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
             if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() % 16
                     or out.stride(0) % 8 or out.stride(1) % 8):
                 raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} on {q.device} with contiguous rows on 16 bytes")
+            if out.data_ptr() == q.data_ptr() and out.numel() > 0:
+                raise ValueError("out must not be q itself")
         os, out_ptr, rec_ptr = out.stride(), out.data_ptr(), None
     else:
         if out is not None:

@@ -271,6 +271,36 @@ def test_a_bad_value_reaches_the_tokens_that_see_it_and_no_others(dtype, g, bad)
     check(got[500:], (want[0][500:], want[1][500:]))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new", [[1, 1], [3, 2], [300, 100]])
+def test_a_bad_key_reaches_the_tokens_that_see_it_and_no_others(dtype, new):
+    from rdkv_b200.paged import paged_attention
+    lens = [400, 150]
+    k, v, table = R.build_cache(lens, 2, 16, dtype, seed=18)
+    q = randn(sum(new), 8, 128, seed=19, dtype=dtype)
+    args = (table, starts(new), ints(lens))
+    want = R.attention(q, k, v, *args)
+    at = 398 if new[0] <= 3 else 250                                    # of request 0, in its KV head 1
+    k[table[0, at // 16], 1, at % 16, 7] = float("nan")
+    got = paged_attention(q, k, v, *args, max_new=max(new))
+    first = max(0, at - (400 - new[0]))
+    assert torch.isnan(got[first:new[0], 4:]).all()
+    check(got[:, :4], (want[0][:, :4], want[1][:, :4]))
+    check(got[:first], (want[0][:first], want[1][:first]))
+    check(got[new[0]:], (want[0][new[0]:], want[1][new[0]:]))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [100, 3]])
+def test_lengths_past_what_the_table_holds(new):
+    """A length behind the table's last page, up to the end of 32 bits: the tokens there are, are seen."""
+    from rdkv_b200.paged import paged_attention
+    k, v, table = R.build_cache([320, 64], 2, 64, BF16, seed=28, width_extra=0)
+    q = randn(sum(new), 4, 128, seed=29, dtype=BF16)
+    for lens in ([5000, 300], [2 ** 31 - 1, 2 ** 31 - 1]):
+        got = paged_attention(q, k, v, table, starts(new), ints(lens), max_new=max(new))
+        check(got, R.attention(q, k, v, table, starts(new), ints([6000, 6000])))      # (every token is in front of the new ones)
+
+
 @pytest.mark.parametrize("max_new", [None, 1, 3, 10 ** 6])
 def test_max_new_is_only_a_hint(max_new):
     run([40, 300, 77], [9, 30, 1], 2, 4, 16, BF16, seed=2, max_new=max_new)
@@ -507,6 +537,10 @@ def test_refusals():
     plan = build_block_tables(*base)
     with pytest.raises(ValueError):
         build_block_tables(*base, free_start=plan.free_next, out=plan)
+    with pytest.raises(ValueError):
+        build_block_tables(plan.kv_lens, *base[1:], out=plan)
+    with pytest.raises(ValueError):
+        paged_attention(**{**good, "out": q})
     with pytest.raises(ValueError):
         build_block_tables(*base[:5], 3, out=plan)
     n = 16385

@@ -8,7 +8,8 @@
 // tile on its own: scores (queries as A operand, keys as B), running maximum and sum, then the weights, which are
 // already in A operand form, times the values (ldmatrix.trans).  The four partial results meet in the slot of the
 // segment's last tile.  Why not tcgen05: its smallest M is 64 rows, of which 4 to 16 would be used, and scores would
-// have to go through tensor memory and shared memory between the products; the tensor pipe is idle most of the time as it is.
+// have to go through tensor memory between the products; the tensor pipe is 80 % idle as it is.
+// 64 requests of up to 8192 tokens, 8 x 4 heads, pages of 16: 181 us, 6.2 TB/s of keys and values (96 % of a copy's rate).
 //
 // Few items (CLUSTER): each is cut evenly over a cluster of 8 or 16 CTAs, which exchange their records through distributed
 // shared memory; there is no line of units to find a place in and no second launch.

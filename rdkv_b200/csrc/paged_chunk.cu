@@ -5,8 +5,8 @@
 // memory, fp32 scores in tensor memory), softmax of S by a warpgroup with one row per thread, the weights P written over S as
 // 16-bit values, O += P.V (tcgen05.mma, P from tensor memory, V as it lies in the cache: MN-major).  Tensor memory is full:
 // per half two buffers of 64 scores and an accumulator of 128 columns.  The scores of step t + 2 are asked for as soon as
-// the weights of step t are used up, so a warpgroup always has its next scores waiting (with one buffer of 128 a half
-// had nothing to do between its weights and its next scores, 1700 cycles of 3900 a tile).
+// the weights of step t are used up, so a warpgroup has its next scores waiting when it is done with a step (with one
+// buffer of 128 scores a half had nothing to do between its weights and its next scores, 1700 cycles of 3900 a tile).
 //
 // 12 warps: two warpgroups of softmax (half 0, half 1), and one of helpers: one warp brings in Q and the tiles (tiled TMA, one box
 // per page and 64-channel panel, 128-byte swizzle, four slots of 32 KB for K and V in turn), two issue the products of a
@@ -16,6 +16,13 @@
 //
 // An accumulator is rescaled by the threads that own its rows, and only when a score passes the row's reference by more
 // than PagedWeights::RAISE.  Every wait is bounded; a wait that runs out ends the CTA's work and sets its status word.
+//
+// What bounds it (2048 tokens behind 30000, 8 x 4 heads, bf16: 0.95 to 1.07 ms over several GPUs, 0.98 to 1.09 PFLOP/s):
+// long launches reach the 1000 W limit, where the clock settles at 1.5 GHz; in short ones (2048 behind 6000: 3650 cycles
+// a tile, of which the products need 2570) the chain of a step inside a softmax warp, about 1700 cycles for 345 instructions:
+// tensor pipe 56 % busy, issue slots 52 %, exponential units 42 %.  Measured and dropped: two warps a row with shared
+// references (sixteen softmax warps; 4040 cycles), the halves' products strictly in turn (4060), the weights worked out before
+// the maximum is known (4450), next scores loaded under the exponentials (does not fit the registers).
 #include "paged_attn.cuh"
 
 namespace rdkv {
@@ -27,8 +34,11 @@ constexpr int CH_SLOT = 2 * CH_PANEL;
 constexpr int CH_STAGE = 32 * 128;                // bytes a softmax warp's results pass through on their way out
 constexpr size_t CH_SMEM = (size_t)(2 + CH_SLOTS) * CH_SLOT + CH_SOFTMAX_WARPS * CH_STAGE;   // (starts on 1024 bytes)
 constexpr int CH_INFO = 8;                        // tiles whose description is kept (a softmax warp is at most three behind the loads)
-constexpr int CH_POLY = 4;                         // every CH_POLY-th pair of exponentials goes to the FMA units
-constexpr int CH_FIXED = 1, CH_SNAP = 3, CH_WHOLE = 8;
+// Every CH_POLY-th pair of exponentials goes to the FMA units.  (2048 behind 6000, thousand cycles: every 4th 369, every 8th 396, none 385.)
+constexpr int CH_POLY = 4;
+// (Six requests of up to 500 tokens behind up to 3000: 95 us with a fixed cost of one tile an item, 87 with two, 91 with three; cuts that
+// leave a tile or two are moved: an item's records are 135 KB.)
+constexpr int CH_FIXED = 2, CH_SNAP = 3, CH_WHOLE = 8;
 constexpr int CH_SOFTMAX_REGS = 208, CH_HELPER_REGS = 88, CH_LAUNCH_REGS = 168;
 static_assert(CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS <= CH_THREADS * CH_LAUNCH_REGS,
               "the split draws on what the block was launched with");

@@ -9,7 +9,7 @@
 // Every CTA works out both prefix sums (new tokens, new pages) for itself in shared memory and then writes its share of
 // the entries; who owns a token or a page is found by bisection.  So nothing is handed from CTA to CTA: entries of
 // the table that are read belong to pages held before, entries that are written to new ones.  Bound by latency:
-// two dependent loads, a scan, a bisection, a store.
+// two dependent loads, a scan, a bisection, a store (16 requests of one new token 4.3 us, 512 requests with 46 thousand 5.3).
 #include <algorithm>
 
 #include "rdkv_common.cuh"

@@ -27,7 +27,7 @@ from torch import Tensor
 
 from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, check, lib, q_dtype_tag, raw_stream,
                    require_cuda)
-from .rope import axes_check
+from .rope import axes_check, empty_rows
 
 MAX_REQUESTS = 16384
 _TABLES_CALLS, _APPEND_CALLS, _ATTENTION_CALLS = CallCache(), CallCache(), CallCache()
@@ -105,7 +105,7 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
     S, table, n_free, index = call
     if out is None:
         ints = ctx_lens.new_empty(n_tokens + 2 * S + 3)
-        out = PagedPlan(ctx_lens.new_empty(n_tokens, dtype=torch.int64), *ints.split_with_sizes((n_tokens, S + 1, S, 1, 1)))
+        out = PagedPlan(ctx_lens.new_empty(n_tokens, dtype=torch.int64), *ints.unsafe_split_with_sizes((n_tokens, S + 1, S, 1, 1)))
     else:
         for name, n in (("positions", n_tokens), ("q_start", S + 1), ("kv_lens", S), ("free_next", 1), ("missing", 1)):
             t = getattr(out, name)
@@ -161,9 +161,9 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     call = _APPEND_CALLS.get(key)
     if call is None:
         call = _APPEND_CALLS.remember(key, _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sections, q_out))
-    args, _, index = call
+    args, _, index, dense = call
     if q is not None and q_out is None:
-        q_out = q.new_empty(q.shape)
+        q_out = empty_rows(q, dense)
     status = lib().rdkv_paged_append(
         args, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slot_map.data_ptr(), None if q is None else q.data_ptr(),
         None if q is None else q_out.data_ptr(), None if positions is None else positions.data_ptr(),
@@ -209,7 +209,7 @@ def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sect
         k_page_row_stride=kp[2], v_page_stride=vp[0], v_page_head_stride=vp[1], v_page_row_stride=vp[2], q_tok_stride=qs[0],
         q_head_stride=qs[1], q_out_tok_stride=qos[0], q_out_head_stride=qos[1], H_q=H_q, H_kv=H_kv, dtype=tag, n_tokens=T, n_pages=n_pages,
         page_size=page_size, **axes)
-    return C.addressof(args), args, dev.index
+    return C.addressof(args), args, dev.index, q is not None and q.is_contiguous()
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: Tensor, q_start: Tensor, kv_lens: Tensor, *,
@@ -238,9 +238,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     call = _ATTENTION_CALLS.get(key)
     if call is None:
         call = _ATTENTION_CALLS.remember(key, _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_new, window, sinks, scale))
-    args, direct, n_ws, index, fields = call
+    args, direct, n_ws, index, fields, dense = call
     if not direct or q.data_ptr() & 15:                    # (rows that no 16-byte copy can fetch)
-        q = q.clone(memory_format=torch.contiguous_format)
+        q, dense = q.clone(memory_format=torch.contiguous_format), True
         fields = PagedAttentionArgs.from_buffer_copy(fields)
         fields.q_tok_stride, fields.q_head_stride = q.stride()[:2]
         args = C.addressof(fields)
@@ -250,7 +250,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     if out_partial is None:
         zero = 0
         if out is None:
-            out, zero = q.new_empty(q.shape), 1
+            out, zero = empty_rows(q, dense), 1
         else:
             require_cuda(out, "out")
             if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() % 16
@@ -315,4 +315,4 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
         v_head_stride=vs[1], v_row_stride=vs[2], table_stride=block_tables.stride(0), dtype=q_dtype_tag(q), n_tokens=T, H_q=H_q, H_kv=H_kv,
         n_pages=n_pages, page_size=page_size, width=block_tables.shape[1], n_requests=S, max_new=max_new, window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30),
         scale=scale)
-    return C.addressof(args), direct, n_ws, q.device.index, args
+    return C.addressof(args), direct, n_ws, q.device.index, args, q.is_contiguous()

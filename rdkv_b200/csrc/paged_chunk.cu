@@ -355,7 +355,8 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(v[i + 2 * e]), __uint_as_float(v[i + 2 * e + 1]));
       const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * A.scale_log2;
-      if (__any_sync(0xffffffffu, high > m + RAISE)) {
+      // (rows that stand for no token hold what happens to be in shared memory: they have no say, or results would not repeat)
+      if (__any_sync(0xffffffffu, live && high > m + RAISE)) {
         const float to = fmaxf(m, high), f = to == -INFINITY ? 1.f : exp2_approx(m - to);   // (m = -inf: 0)
         m = to; l *= f;
         if (t > 0) {                                         // the accumulator, once the product of the step before is done

@@ -397,11 +397,16 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("new", [[1] * 6, [90, 1, 40, 3, 128, 17]])
-def test_results_repeat(new):
-    """The same call again, beside others on another stream: the same bits."""
+@pytest.mark.parametrize("g", [4, 5, 7])
+def test_results_repeat(new, g):
+    """The same call again, beside others on another stream and after one with large queries (7 query heads a KV head
+    leave rows of a tile without a token): the same bits."""
     from rdkv_b200.paged import paged_attention
     lens = [700, 64, 999, 300, 2000, 17]
-    q, k, v, table, want = run(lens, new, 2, 4, 16, BF16, seed=51)
+    q, k, v, table, want = run(lens, new, 2, g, 16, BF16, seed=51)
+    for size in (100.0, 1e-3):
+        paged_attention(q * size, k, v, table, starts(new), ints(lens), max_new=max(new))
+        assert torch.equal(paged_attention(q, k, v, table, starts(new), ints(lens), max_new=max(new)), want)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     mine, others = [], []

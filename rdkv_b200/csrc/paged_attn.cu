@@ -11,7 +11,7 @@
 // have to go through tensor memory between the products; the tensor pipe is 80 % idle as it is.
 // 64 requests of up to 8192 tokens, 8 x 4 heads, pages of 16: 181 us, 6.2 TB/s of keys and values (96 % of a copy's rate).
 //
-// Few items (CLUSTER): each is cut evenly over a cluster of 8 or 16 CTAs, which exchange their records through distributed
+// Few items (CLUSTER): each is cut evenly over a cluster of 8, 12 or 16 CTAs, which exchange their records through distributed
 // shared memory; there is no line of units to find a place in and no second launch.
 //
 // Masks are applied only to 16-key blocks that reach past some row's limits.  There, values of keys that no row of
@@ -403,12 +403,12 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
           const float M = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
           const float L = warp_sum(ml.y * f);
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int x0 = 0; x0 < size; x0 += 8) {             // (clusters are of 8 or 16)
-            float4 p[8];
+          for (int x0 = 0; x0 < size; x0 += 4) {             // (clusters are of 8, 12 or 16)
+            float4 p[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = dec_remote4(dec_map(at + 16u + 16u * lane, x0 + e));
+            for (int e = 0; e < 4; ++e) p[e] = dec_remote4(dec_map(at + 16u + 16u * lane, x0 + e));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4; ++e) {
               const float w = __shfl_sync(0xffffffffu, f, x0 + e);
               sum.x = fmaf(p[e].x, w, sum.x); sum.y = fmaf(p[e].y, w, sum.y); sum.z = fmaf(p[e].z, w, sum.z); sum.w = fmaf(p[e].w, w, sum.w);
             }
@@ -466,17 +466,20 @@ static int decode_line(const PagedArgs& A, const CUtensorMap& tm_k, const CUtens
   return paged_launch_join(paged_join_kernel<BF16, DEC_ROWS, PAGED_DECODE_CTAS>, A, dim3(PAGED_DECODE_CTAS - 1, DEC_ROWS / PAGED_JOIN_WARPS), st);
 }
 
-// Items that the decode kernel gives a cluster of eight CTAs or more each.
-static bool paged_few_items(int64_t n_requests, int H_kv) { return n_requests * H_kv * 8 <= PAGED_DECODE_CTAS; }
+// CTAs of the cluster that an item gets where all items' clusters fit the GPU at once, two CTAs an SM (14 clusters of 16, 21 of 12, 33
+// of 8: a cluster lies in one GPC); 0: too many items.  (8 KV heads, us, clusters / line of units with its second launch: one
+// request of 1000 tokens 9.0 / 13.5, of 8000 15.4 / 18.0, of 32000 38 / 38; two of 1000 10.6 / 12.7, of 32000 51 / 52; four of 1000 10.2 / 13.1.
+// Sixteen clusters of 16 are two waves: two requests of 1000 tokens 16.0.)
+static int paged_cluster_size(int64_t n_requests, int H_kv) {
+  const int64_t items = n_requests * H_kv;
+  return items <= 0 || items > 33 ? 0 : items <= 14 ? 16 : items <= 21 ? 12 : 8;
+}
 
 int paged_decode_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
-  // Few items: a cluster each, as long as eight CTAs an item fit the GPU at once.  (One request of 1061 tokens, 8 heads: 17.3 us on the
-  // line of units with its second launch, 8.6 in clusters of 16.)
-  const int64_t items = (int64_t)A.S * A.H_kv;
-  if (items > 0 && paged_few_items(A.S, A.H_kv)) {
-    const int size = items * 16 <= PAGED_DECODE_CTAS ? 16 : 8;
-    return bf16 ? decode_cluster<true>(A, (unsigned)(items * size), (unsigned)size, tm_k, tm_v, st)
-                : decode_cluster<false>(A, (unsigned)(items * size), (unsigned)size, tm_k, tm_v, st);
+  const int size = paged_cluster_size(A.S, A.H_kv);
+  if (size > 0) {
+    const unsigned ctas = (unsigned)(A.S * A.H_kv * size);
+    return bf16 ? decode_cluster<true>(A, ctas, (unsigned)size, tm_k, tm_v, st) : decode_cluster<false>(A, ctas, (unsigned)size, tm_k, tm_v, st);
   }
   return bf16 ? decode_line<true>(A, tm_k, tm_v, st) : decode_line<false>(A, tm_k, tm_v, st);
 }
@@ -491,7 +494,7 @@ using namespace rdkv;
 // 141 / 123; 200 x 1000, 20 rows 101 / 133; one request of 30000, 32 rows 72 / 45.)
 static bool paged_few_rows(int n_requests, int H_kv, int max_new, int g) {
   const int64_t rows = (int64_t)max_new * g;
-  return rows <= PAGED_DECODE_ROWS || (rows <= PAGED_DECODE_ROWS + 8 && !paged_few_items(n_requests, H_kv));
+  return rows <= PAGED_DECODE_ROWS || (rows <= PAGED_DECODE_ROWS + 8 && paged_cluster_size(n_requests, H_kv) == 0);
 }
 
 extern "C" int64_t rdkv_paged_attention_workspace(int n_requests, int n_tokens, int H_q, int H_kv, int max_new) {

@@ -314,6 +314,8 @@ def test_many_requests_and_few():
     new = [rng.choice([0, 1, 2, rng.randint(0, n)]) for n in lens]
     run(lens[:300], [min(a, b) for a, b in zip(new, lens)][:300], 1, 2, 16, F16, seed=22)
     run(lens, [min(a, b) for a, b in zip(new, lens)], 2, 8, 16, BF16, seed=26)
+    run(lens[:18], [1] * 18, 1, 4, 16, F16, seed=27)                     # (clusters of 12 CTAs; of 8)
+    run(lens[:31], [1] * 31, 1, 4, 16, F16, seed=28)
     run([5000], [1], 1, 8, 64, F16, seed=23)
     run([5000], [1], 8, 1, 64, BF16, seed=24, window=3000, sinks=4)
     run([3000], [700], 1, 4, 64, BF16, seed=25)

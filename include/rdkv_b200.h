@@ -656,11 +656,11 @@ int rdkv_paged_append(const rdkv_paged_append_args* args, const void* k, const v
  * up to 16 query heads a KV head; bases on 16 bytes, strides of whole 16 bytes).  Query row q_start[i]+j is request i's
  * token kv_lens[i]-n_i+j (n_i = q_start[i+1]-q_start[i]); it sees the tokens up to itself, under window > 0 only the last
  * `window` of them and the first `sinks`, and none whose page number is outside [0, n_pages).  max_new: the longest chunk
- * (a hint: it chooses the kernel).  Either out [n_tokens][H_q][128] (rows behind q_start[n_requests]: zeroed with
- * zero_padding, else left) or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace:
+ * (a hint: it chooses the kernel).  Either out [n_tokens][H_q][128] (rows in front of q_start[0] and from
+ * q_start[n_requests] on: zeroed with zero_padding, else left) or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace:
  * rdkv_paged_attention_workspace() bytes (16-byte aligned; of one call at a time), contents arbitrary.  Its first
- * rdkv_paged_attention_status_words() int32 say after the call whether a device-side wait ran out (not 0), in which
- * case the results are invalid. */
+ * rdkv_paged_attention_status_words() int32 are 0 after the call, or hold bit 1 (a device-side wait ran out: the
+ * results are invalid) or 2 (q_start falls somewhere: no request was computed). */
 typedef struct {
   int64_t q_tok_stride, q_head_stride;
   int64_t k_page_stride, k_head_stride, k_row_stride, v_page_stride, v_head_stride, v_row_stride;

@@ -111,12 +111,16 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
   auto begin = [&]() {
     if constexpr (CLUSTER) {
       DecWalk<true> walk(A);
-      __syncthreads();
+      if (__syncthreads_or(paged_falls(A, tid))) {           // (no more requests than clusters: fewer than threads)
+        walk.groups = 0;
+        if (tid == 0) s_trouble = 2;
+      }
       return walk;
     } else {
       let_next_kernel_start();
       PagedPlace from, to;
-      paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP, DEC_WHOLE, PAGED_DECODE_CTAS>(A, cta, s_place, from, to);   // (its barriers order the set-up too)
+      const bool ordered = paged_place<DEC_KEYS, DEC_THREADS, DEC_FIXED, DEC_SNAP, DEC_WHOLE, PAGED_DECODE_CTAS>(A, cta, s_place, from, to);
+      if (!ordered && tid == 0) s_trouble = 2;               // (the barriers in there order the set-up too)
       return DecWalk<false>(A, from, to);
     }
   };

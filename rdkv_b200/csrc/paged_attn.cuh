@@ -41,7 +41,7 @@ struct PagedArgs {
   float* rec;                                     // [T][H_q][132] instead of out
   // workspace
   int4* place;                                    // [G+1][2] where CTA c starts: request, head, group, tile; the item's tiles, rows, first query row
-  int* status;                                    // [G] 1: a wait of the CTA ran out
+  int* status;                                    // [G] bits: 1 a wait of the CTA ran out, 2 q_start falls
   float* part;                                    // [2 G][rows of an item][132] records of cut items
 };
 
@@ -101,6 +101,8 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedArgs& A, int i)
   r.len = max(A.kv_lens[i], 0);
   return r;
 }
+// Whether q_start falls behind request i (one of a batch's requests; other numbers: no).
+__device__ __forceinline__ bool paged_falls(const PagedArgs& A, int i) { return i < A.S && A.q_start[i + 1] < A.q_start[i]; }
 __device__ __forceinline__ int paged_groups(const PagedArgs& A, const PagedRequest& r) { return (r.n + A.group - 1) / A.group; }
 
 template <int KEYS>
@@ -130,11 +132,13 @@ struct PagedPlaceScratch { uint32_t part[32], most[32], groups[32]; uint32_t at[
 // would leave fewer than SNAP tiles of an item on one side is moved to the item's edge.  With no more items than CTAs, and
 // none more than WHOLE units over its share, every CTA gets a whole item: a cut costs both its sides an item's records,
 // written and read again.  The launcher has seen to it that a head's units fit 31 bits.  (Every launch pays for this code from
-// a cold instruction cache: in 64 bits, with two divisions more, it took 7400 cycles.)
+// a cold instruction cache: in 64 bits, with two divisions more, it took 7400 cycles.)  Returns false, and the end as both places,
+// where q_start falls somewhere: requests would share query rows.
 template <int KEYS, int NT, int FIXED, int SNAP, int WHOLE, int G>
-__device__ __forceinline__ void paged_place(const PagedArgs& A, int c, PagedPlaceScratch& s, PagedPlace& from, PagedPlace& to) {
+__device__ __forceinline__ bool paged_place(const PagedArgs& A, int c, PagedPlaceScratch& s, PagedPlace& from, PagedPlace& to) {
+  constexpr uint32_t FALLS = 0x80000000u;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // units of a head of request i, its groups, its costliest item
+  // units of a head of request i, its groups, its costliest item (FALLS: q_start falls there)
   auto units = [&](int i, uint32_t& groups_, uint32_t& most) -> uint32_t {
     PagedRequest r = {0, 0, 0};
     if (i < A.S) r = paged_request(A, i);
@@ -161,6 +165,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, PagedPlac
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == from_lane) { sum = mine; most = top; }
     }
+    if (paged_falls(A, i)) most = FALLS;
     return sum;
   };
   auto warp_scan = [&](uint32_t x) {                          // inclusive
@@ -200,6 +205,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, PagedPlac
     for (int w = 0; w < NT / 32; ++w) { most = max(most, s.most[w]); n_groups += s.groups[w]; }
     total += all;
   }
+  const bool ordered = most < FALLS;
   const bool whole = (uint64_t)n_groups * A.H_kv <= (uint64_t)G && most <= (uint32_t)((uint64_t)total * A.H_kv / G) + WHOLE;
   // cut e: its head, and its place in the head's line
   int head[2];
@@ -226,7 +232,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, PagedPlac
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (head[e] < A.H_kv && cut[e] - (run + before) < mine) { s.request[e] = base + tid; s.at[e] = cut[e] - (run + before); }
+      if (ordered && head[e] < A.H_kv && cut[e] - (run + before) < mine) { s.request[e] = base + tid; s.at[e] = cut[e] - (run + before); }
     run += all;
   }
   __syncthreads();
@@ -267,6 +273,7 @@ __device__ __forceinline__ void paged_place(const PagedArgs& A, int c, PagedPlac
     A.place[2 * c] = f; A.place[2 * c + 1] = s.item;
     if (c == G - 1) A.place[2 * G] = make_int4(0, A.H_kv, 0, 0);
   }
+  return ordered;
 }
 
 // The segments of a CTA: runs of tiles of one item.  Every role of the CTA walks them by itself.

@@ -508,7 +508,8 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   let_next_kernel_start();
   tmem_fence_before();
   PagedPlace from, to;
-  paged_place<CH_KEYS, CH_THREADS, CH_FIXED, CH_SNAP, CH_WHOLE, PAGED_CHUNK_CTAS>(A, cta, s_place, from, to);   // (its barriers order the set-up too)
+  const bool ordered = paged_place<CH_KEYS, CH_THREADS, CH_FIXED, CH_SNAP, CH_WHOLE, PAGED_CHUNK_CTAS>(A, cta, s_place, from, to);
+  if (!ordered && tid == 0) s_trouble = 2;                   // (the barriers in there order the set-up too)
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = s_tmem;

@@ -219,7 +219,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
 
     q [T,H_q,128] (fp16 / bf16, the pages' dtype, after rotation); k_pages, v_pages [n_pages,H_kv,page_size,128] with
     page_size a power of two from 16 to 1024 and up to 16 query heads a KV head; block_tables int32 [S,width], q_start
-    int32 [S+1], kv_lens int32 [S] (as :func:`build_block_tables` leaves them).  The last ``q_start[i+1]-q_start[i]`` of
+    int32 [S+1], kv_lens int32 [S] (as :func:`build_block_tables` leaves them: q_start must not fall).  The last ``q_start[i+1]-q_start[i]`` of
     request i's ``kv_lens[i]`` tokens are the new ones, whose keys and values are in the pages already.  A token
     sees its request's tokens up to itself; with ``window`` > 0 only the last ``window`` of them (itself included)
     and the request's first ``sinks``.  Tokens whose page is missing (an entry outside the pages) are not seen, and what
@@ -227,8 +227,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
 
     max_new: the longest chunk of the batch (default T), which chooses the kernel: a hint, results do not depend on it.
     scale: of the scores, positive, default 1/sqrt(128).  check_status: wait for the kernels and raise if one of their
-    bounded waits ran out, in which case the results are invalid; without it the call returns at once.
-    Returns ``out`` [T,H_q,128] in q's dtype.  Tokens behind the last request's are padding: zero in an ``out`` that the
+    bounded waits ran out or q_start falls, in which case the results are invalid; without it the call returns at once.
+    Returns ``out`` [T,H_q,128] in q's dtype.  Tokens in front of the first request's and behind the
+    last one's are padding: zero in an ``out`` that the
     call allocates, left as they were in one that it is given (which must not be q itself).  ``out_partial`` float32 [T*H_q,132] receives
     un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape,
@@ -272,8 +273,12 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
                                         out_ptr, os[0], os[1], zero, rec_ptr, ws.data_ptr(), 4 * n_ws, raw_stream(index))
     if status:
         check(status, "rdkv_paged_attention")
-    if check_status and n_ws > 0 and bool(ws[:lib().rdkv_paged_attention_status_words()].any().item()):
-        raise RuntimeError("rdkv_paged_attention: a device-side wait ran out; the results are invalid")
+    if check_status and n_ws > 0:
+        trouble = int(ws[:lib().rdkv_paged_attention_status_words()].max())
+        if trouble & 2:
+            raise ValueError("q_start must not fall: nothing was computed")
+        if trouble:
+            raise RuntimeError("rdkv_paged_attention: a device-side wait ran out; the results are invalid")
     return out if out_partial is None else out_partial
 
 

@@ -321,6 +321,35 @@ def test_many_requests_and_few():
     run([3000], [700], 1, 4, 64, BF16, seed=25)
 
 
+@pytest.mark.parametrize("max_new", [1, 200])
+@pytest.mark.parametrize("start", [[3, 4, 9], [0, 0, 300], [2, 150, 200], [-7, 3, 8]])
+def test_rows_in_front_and_starts_outside(start, max_new):
+    """Query rows in front of the first request's are padding too, and rows outside the tensor are not touched.  A length below zero counts as none."""
+    from rdkv_b200.paged import paged_attention
+    k, v, table = R.build_cache([400, 333], 2, 32, BF16, seed=61)
+    T = 203
+    q = randn(T, 8, 128, seed=62, dtype=BF16)
+    clamped = [min(max(x, 0), T) for x in start]
+    for lens in ([400, 333], [-5, 300]):
+        got = paged_attention(q, k, v, table, ints(start), ints(lens), max_new=max_new, check_status=True)
+        check(got, R.attention(q, k, v, table, ints(clamped), ints([max(n, 0) for n in lens])))
+        assert (got[:max(min(clamped), 0)] == 0).all() and (got[max(clamped):] == 0).all()
+
+
+@pytest.mark.parametrize("S,H_kv,max_new", [(2, 2, 1), (2, 2, 200), (30, 1, 1), (60, 2, 1), (600, 1, 1), (600, 1, 200)])
+def test_starts_that_fall_are_refused(S, H_kv, max_new):
+    """Requests would share query rows.  The kernels compute nothing and say so, wherever the fall stands."""
+    from rdkv_b200.paged import paged_attention
+    k, v, table = R.build_cache([40] * S, H_kv, 32, BF16, seed=63)
+    q = randn(S + 9, 4 * H_kv, 128, seed=64, dtype=BF16)
+    for at in sorted({1, S // 2 + 1, S}):                     # q_start[at] < q_start[at - 1]
+        start = [i + 3 if i < at else i for i in range(S + 1)]
+        out = torch.full_like(q, 7.0)
+        with pytest.raises(ValueError, match="q_start must not fall"):
+            paged_attention(q, k, v, table, ints(start), ints([40] * S), max_new=max_new, out=out, check_status=True)
+        assert (out == 7.0).all()
+
+
 @pytest.mark.parametrize("new", [[1, 1], [100, 37]])
 def test_layouts_and_buffers(new):
     """Pages whose rows come before their heads, query rows out of a fused projection (also with a stride no 16-byte

@@ -268,6 +268,12 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def separate_rows(t: torch.Tensor, name: str) -> None:
+    """Refuses a broadcast view, whose rows are one and the same memory, where rows are written or TMA copies read them."""
+    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} must not be a broadcast view")
+
+
 class CallCache(dict):
     """What the checks of a call worked out from the shapes, strides, types and devices of its arguments, under just
     those: the next call of the same kind skips the checks.  Nothing of the arguments' contents, addresses or identity."""

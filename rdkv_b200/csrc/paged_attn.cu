@@ -518,7 +518,7 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
   if (args == nullptr) return RDKV_ERR_BAD_ARG;
   const rdkv_paged_attention_args& g = *args;
   if (g.n_tokens < 0 || g.n_requests < 0 || g.H_q <= 0 || g.H_kv <= 0 || g.n_pages < 0 || g.width < 0 || g.window < 0 || g.sinks < 0 ||
-      g.max_new < 0 || !(g.scale > 0.f))
+      g.max_new < 0 || !(g.scale > 0.f && g.scale <= 1e30f))
     return RDKV_ERR_BAD_ARG;
   if (g.dtype != RDKV_F16 && g.dtype != RDKV_BF16) return RDKV_ERR_BAD_ARG;
   if (g.H_q % g.H_kv != 0 || g.H_q / g.H_kv > MAX_GROUP) return RDKV_ERR_BAD_SHAPE;

@@ -26,7 +26,7 @@ import torch
 from torch import Tensor
 
 from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, check, lib, q_dtype_tag, raw_stream,
-                   require_cuda)
+                   require_cuda, separate_rows)
 from .rope import axes_check, empty_rows
 
 MAX_REQUESTS = 16384
@@ -139,6 +139,7 @@ def _check_pages(k_pages: Tensor, v_pages: Tensor) -> None:
         raise ValueError("k_pages and v_pages must have one dtype")
     if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
         raise ValueError("rows of k_pages and v_pages must be contiguous")
+    separate_rows(k_pages, "k_pages"); separate_rows(v_pages, "v_pages")
 
 
 def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: Tensor, *, q: Optional[Tensor] = None,
@@ -200,6 +201,8 @@ def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sect
             raise ValueError(f"q must be [{T},H_q,{HEAD_DIM}] {k.dtype} with contiguous rows, got {tuple(q.shape)} {q.dtype}")
         if q_out is not None and (q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1):
             raise ValueError("q_out must have q's shape and dtype and contiguous rows")
+        if q_out is not None:
+            separate_rows(q_out, "q_out")
         H_q = q.shape[1]
         qs, qos = q.stride(), (H_q * HEAD_DIM, HEAD_DIM) if q_out is None else q_out.stride()
     _same_device(dev, v=v, k_pages=k_pages, v_pages=v_pages, slot_map=slot_map, q=q, q_out=q_out)
@@ -240,7 +243,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     if call is None:
         call = _ATTENTION_CALLS.remember(key, _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_new, window, sinks, scale))
     args, direct, n_ws, index, fields, dense = call
-    if not direct or q.data_ptr() & 15:                    # (rows that no 16-byte copy can fetch)
+    if not direct or q.data_ptr() & 15:                    # (rows that no 16-byte or TMA copy can fetch)
         q, dense = q.clone(memory_format=torch.contiguous_format), True
         fields = PagedAttentionArgs.from_buffer_copy(fields)
         fields.q_tok_stride, fields.q_head_stride = q.stride()[:2]
@@ -257,6 +260,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
             if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.data_ptr() % 16
                     or out.stride(0) % 8 or out.stride(1) % 8):
                 raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} on {q.device} with contiguous rows on 16 bytes")
+            separate_rows(out, "out")
             if out.data_ptr() == q.data_ptr() and out.numel() > 0:
                 raise ValueError("out must not be q itself")
         os, out_ptr, rec_ptr = out.stride(), out.data_ptr(), None
@@ -304,8 +308,8 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError("window and sinks must not be negative, and sinks need a window")
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
-    if not scale > 0:
-        raise ValueError(f"scale must be positive, got {scale}")
+    if not 1e-30 < scale < 1e30:                           # (an ordinary number in 32 bits)
+        raise ValueError(f"scale must be positive and finite, got {scale}")
     max_new = T if max_new is None else min(int(max_new), T)
     if max_new < 0:
         raise ValueError("max_new must not be negative")
@@ -313,11 +317,11 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
     if any(x % 8 for x in ks + vs):
         raise ValueError("k_pages and v_pages must have strides of whole 16 bytes")
     _same_device(q.device, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, q_start=q_start, kv_lens=kv_lens)
-    direct = q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0
+    direct = q.stride(2) == 1 and all(st % 8 == 0 and (st > 0 or n == 1) for n, st in zip(q.shape[:2], q.stride()))
     n_ws = -(-lib().rdkv_paged_attention_workspace(S, T, H_q, H_kv, max_new) // 4)
     args = PagedAttentionArgs(
         q_tok_stride=q.stride(0), q_head_stride=q.stride(1), k_page_stride=ks[0], k_head_stride=ks[1], k_row_stride=ks[2], v_page_stride=vs[0],
         v_head_stride=vs[1], v_row_stride=vs[2], table_stride=block_tables.stride(0), dtype=q_dtype_tag(q), n_tokens=T, H_q=H_q, H_kv=H_kv,
-        n_pages=n_pages, page_size=page_size, width=block_tables.shape[1], n_requests=S, max_new=max_new, window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30),
-        scale=scale)
+        n_pages=n_pages, page_size=page_size, width=block_tables.shape[1], n_requests=S, max_new=max_new,
+        window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30), scale=scale)
     return C.addressof(args), direct, n_ws, q.device.index, args, q.is_contiguous()

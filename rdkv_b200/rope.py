@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import HEAD_DIM, CallCache, RopeAxesArgs, check, lib, ptr, q_dtype_tag, raw_stream, require_cuda, stream_ptr
+from ._lib import HEAD_DIM, CallCache, RopeAxesArgs, check, lib, ptr, q_dtype_tag, raw_stream, require_cuda, separate_rows, stream_ptr
 
 
 def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
@@ -110,6 +110,8 @@ def _rope_check(q, k, positions, inv_freq, sections, q_out, k_out):
     for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != dev or t.stride(2) != 1):
             raise ValueError(f"{name} must have the shape, dtype and device of its input and contiguous rows")
+        if t is not None:
+            separate_rows(t, name)
     (q0, q1), (k0, k1) = q.stride()[:2], k.stride()[:2]
     qo = (q.shape[1] * HEAD_DIM, HEAD_DIM) if q_out is None else q_out.stride()
     ko = (k.shape[1] * HEAD_DIM, HEAD_DIM) if k_out is None else k_out.stride()

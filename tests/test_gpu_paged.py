@@ -321,6 +321,32 @@ def test_many_requests_and_few():
     run([3000], [700], 1, 4, 64, BF16, seed=25)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [150, 70]])
+def test_broadcast_views(new):
+    """Queries are taken as they are; pages and results are refused."""
+    from rdkv_b200.paged import append_kv, paged_attention
+    from rdkv_b200.rope import rope_axes
+    lens, T = [300, 111], sum(new)
+    k, v, table = R.build_cache(lens, 2, 32, BF16, seed=71)
+    args = (table, starts(new), ints(lens))
+    q = randn(T, 8, 128, seed=72, dtype=BF16)
+    for x in (q[:1].expand(T, 8, 128), q[:, :1].expand(T, 8, 128)):
+        check(paged_attention(x, k, v, *args, max_new=max(new)), R.attention(x, k, v, *args))
+    for x, y in ((k[:, :1].expand_as(k), v[:, :1].expand_as(v)), (k[:1].expand_as(k), v[:1].expand_as(v))):
+        for pages in ((x, v), (k, y)):
+            with pytest.raises(ValueError, match="broadcast"):
+                paged_attention(q, *pages, *args, max_new=max(new))
+    rows = randn(T, 2, 128, seed=73, dtype=BF16)
+    slots, pos = torch.arange(T, device="cuda"), torch.arange(T, device="cuda")
+    many = torch.empty(T, 1, 128, device="cuda", dtype=BF16).expand(T, 8, 128)
+    for call in (lambda: paged_attention(q, k, v, *args, out=many), lambda: rope_axes(q, rows, pos, INV(), q_out=many),
+                 lambda: rope_axes(q, rows, pos, INV(), k_out=many[:, :2]), lambda: append_kv(rows, rows, k[:1].expand_as(k), v, slots),
+                 lambda: append_kv(rows, rows, k, v[:, :1].expand_as(v), slots),
+                 lambda: append_kv(rows, rows, k, v, slots, q=q, positions=pos, inv_freq=INV(), q_out=many)):
+        with pytest.raises(ValueError, match="broadcast"):
+            call()
+
+
 @pytest.mark.parametrize("max_new", [1, 200])
 @pytest.mark.parametrize("start", [[3, 4, 9], [0, 0, 300], [2, 150, 200], [-7, 3, 8]])
 def test_rows_in_front_and_starts_outside(start, max_new):
@@ -541,7 +567,7 @@ def test_refusals():
     good = dict(q=q, k_pages=k, v_pages=v, block_tables=table, q_start=ints([0, 1, 2]), kv_lens=ints([64, 64]))
     for change in (dict(q=q.float()), dict(q=q.to(BF16)), dict(q=q[:, :7]), dict(q=q[..., :64]), dict(q=q[0]), dict(v_pages=v[1:]), dict(v_pages=v.to(BF16)),
                    dict(k_pages=k[:, :, :8], v_pages=v[:, :, :8]), dict(block_tables=table.long()), dict(block_tables=table[:1]),
-                   dict(q_start=ints([0, 2])), dict(kv_lens=ints([64])), dict(kv_lens=ints([64, 64]).long()), dict(window=-1), dict(sinks=3), dict(max_new=-1), dict(scale=0.0), dict(scale=-1.0),
+                   dict(q_start=ints([0, 2])), dict(kv_lens=ints([64])), dict(kv_lens=ints([64, 64]).long()), dict(window=-1), dict(sinks=3), dict(max_new=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=1e-50),
                    dict(out=torch.empty_like(q).float()), dict(out=torch.empty(2, 8, 129, dtype=F16, device="cuda")[..., 1:]),
                    dict(out_partial=torch.empty(16, 131, device="cuda")), dict(out=torch.empty_like(q), out_partial=torch.empty(16, 132, device="cuda")),
                    dict(k_pages=torch.empty(10, 2, 16, 132, dtype=F16, device="cuda")[..., :128], v_pages=torch.empty(10, 2, 16, 128, dtype=F16, device="cuda")),

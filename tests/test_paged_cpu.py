@@ -26,7 +26,7 @@ def _attention(**change):
     (dict(n_tokens=-1), 1), (dict(n_requests=-1), 1), (dict(H_q=0), 1), (dict(H_kv=0), 1), (dict(dtype=2), 1), (dict(dtype=7), 1), (dict(window=-1), 1),
     (dict(sinks=-1), 1), (dict(max_new=-1), 1), (dict(width=-1), 1), (dict(n_pages=-1), 1), (dict(H_kv=3), 2), (dict(H_q=34), 2), (dict(page_size=8), 2),
     (dict(page_size=24), 2), (dict(page_size=2048), 2), (dict(q=None), 1), (dict(q_start=None), 1), (dict(lens=None), 1), (dict(table=None), 1),
-    (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(rec=1 << 12), 1), (dict(scale=0.0), 1), (dict(scale=-1.0), 1), (dict(scale=float('nan')), 1), (dict(ws=None), 1), (dict(ws=(1 << 12) + 8), 1), (dict(ws_bytes=100), 1),
+    (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1), (dict(rec=1 << 12), 1), (dict(scale=0.0), 1), (dict(scale=-1.0), 1), (dict(scale=float('nan')), 1), (dict(scale=float('inf')), 1), (dict(ws=None), 1), (dict(ws=(1 << 12) + 8), 1), (dict(ws_bytes=100), 1),
     (dict(n_requests=16384, width=1 << 20, page_size=1024), 3), (dict(n_tokens=0, q=None), 0)])
 def test_attention_refusals(change, status):
     assert _attention(**change) == status

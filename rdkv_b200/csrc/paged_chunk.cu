@@ -86,15 +86,31 @@ __device__ __forceinline__ bool chunk_edge(const PagedArgs& A, const PagedItem& 
   return key0 + CH_KEYS - 1 > it.p0 || there != 0xFF || (A.window > 0 && key0 <= p_last - A.window && key0 + CH_KEYS > A.sinks);
 }
 
-// Steps of a segment that half h takes: those whose first key is in front of the end of what its last row sees.
-__device__ __forceinline__ int chunk_steps(const PagedArgs& A, const PagedSegment& s, int h, int tm) {
-  const int n_tok = min(tm, s.item.n_tok - h * tm);
-  if (n_tok <= 0) return 0;
-  const int end = min(s.item.p0 + h * tm + n_tok, A.cap);
-  int steps = 2 * (s.k1 - s.k0);
-  while (steps > 0 && paged_tile(s.item, s.k0 + ((steps - 1) >> 1)) * CH_KEYS + ((steps - 1) & 1) * CH_STEP >= end) --steps;
-  return steps;
-}
+// Steps of a segment that half h takes: up to the end of what its last row sees, but under a window not the second step of the
+// last tile of sinks, where they end before it, nor the first of the window's first tile, where the window begins behind it (4000 tokens
+// behind 8000, window 1024 and 4 sinks: 18 steps an item for 19.5, 121.5 -> 117.6 us; four requests of 1000 tokens under a window of 256
+// 46.8 -> 40.1).  Every tile in front of the end keeps a step.
+template <bool WINDOW>
+struct ChunkSteps {
+  int n, end, skip_sinks, skip_front;             // steps taken; end of all; the two that may be left out (-1: none)
+  __device__ __forceinline__ ChunkSteps(const PagedArgs& A, const PagedSegment& s, int h, int tm) : n(0), end(0), skip_sinks(-1), skip_front(-1) {
+    const int n_tok = min(tm, s.item.n_tok - h * tm);
+    if (n_tok <= 0) return;
+    const int p0 = s.item.p0 + h * tm, last = min(p0 + n_tok, A.cap);
+    end = 2 * (s.k1 - s.k0);
+    while (end > 0 && paged_tile(s.item, s.k0 + ((end - 1) >> 1)) * CH_KEYS + ((end - 1) & 1) * CH_STEP >= last) --end;
+    n = end;
+    if (!WINDOW) return;
+    const int sinks = 2 * (s.item.t_sink - s.k0) - 1, front = sinks + 1, key0 = s.item.t_lo * CH_KEYS;
+    if (sinks > 0 && sinks < end && A.sinks <= (s.item.t_sink - 1) * CH_KEYS + CH_STEP) { skip_sinks = sinks; --n; }
+    if (front >= 0 && front + 1 < end && A.sinks <= key0 && p0 - A.window + 1 >= key0 + CH_STEP) { skip_front = front; --n; }
+  }
+  __device__ __forceinline__ int next(int t) const {         // (the two may be neighbours)
+    if (!WINDOW) return t + 1;
+    t += t + 1 == skip_sinks ? 2 : 1;
+    return t == skip_front ? t + 1 : t;
+  }
+};
 
 template <bool BF16>
 __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
@@ -165,7 +181,7 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
 __device__ __forceinline__ int chunk_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // Two warps: the products of half 0, of half 1.
-template <bool BF16>
+template <bool BF16, bool WINDOW>
 __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int h, uint32_t q32, uint32_t ring, uint32_t bar, uint32_t tmem_,
                                const ChunkTile* s_info, int* s_trouble) {
   constexpr uint32_t QK = mma_idesc<BF16>(CH_STEP, false), PV = mma_idesc<BF16>(128, true);
@@ -188,43 +204,48 @@ __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int 
   while (ok && chunk_uniform(walk.next(A, s))) {
     const int n = chunk_uniform(s.k1 - s.k0);
     if (n == 0) continue;
-    const int steps = chunk_uniform(chunk_steps(A, s, h, tm));
+    ChunkSteps<WINDOW> st(A, s, h, tm);
+    st.skip_sinks = chunk_uniform(st.skip_sinks); st.skip_front = chunk_uniform(st.skip_front);
+    const int steps = chunk_uniform(st.n), end = chunk_uniform(st.end);
     wait(CH_Q_FULL, segments++ & 1);
-    auto scores = [&](int t) {                               // S = Q . K^T of step t, into buffer t & 1
-      const int x = tile + (t >> 1);
-      if ((t & 1) == 0) wait_k(x);
+    int asked = st.next(-1), taken = asked, k_tile = -1, v_tile = -1;   // the next step to ask for / to take; tiles waited for
+    auto scores = [&](int u) {                               // S = Q . K^T of the u-th step, into buffer u & 1
+      const int t = asked, x = tile + (t >> 1);
+      asked = st.next(t);
+      if (WINDOW ? t >> 1 != k_tile : (t & 1) == 0) { wait_k(x); k_tile = t >> 1; }
       if (!ok) return;
       tmem_fence_after();
       const uint64_t k = desc_k_major(ring + 2 * (x & 1) * CH_SLOT + (t & 1) * (CH_STEP * 128));
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {                       // 16 channels: 32 bytes along the swizzled row, the second panel after four
         const uint64_t off = ((uint64_t)(kk >> 2) * CH_PANEL + (uint64_t)(kk & 3) * 32u) >> 4;
-        mma_ss(one, t_s + CH_STEP * (t & 1), q + off, k + off, QK, kk > 0 ? 1u : 0u);
+        mma_ss(one, t_s + CH_STEP * (u & 1), q + off, k + off, QK, kk > 0 ? 1u : 0u);
       }
-      mma_commit(one, bar + 8 * (CH_S_FULL + 2 * h + (t & 1)));
-      if ((t & 1) == 1 || t == steps - 1) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1)));
-      if (t == steps - 1) mma_commit(one, bar + 8 * CH_Q_FREE);
+      mma_commit(one, bar + 8 * (CH_S_FULL + 2 * h + (u & 1)));
+      if (u == steps - 1 || (WINDOW ? asked >> 1 != t >> 1 : (t & 1) == 1)) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1)));
+      if (u == steps - 1) mma_commit(one, bar + 8 * CH_Q_FREE);
     };
     if (steps > 0) scores(0);
     if (steps > 1) scores(1);
-    for (int t = 0; ok && t < steps; ++t) {
-      const int x = tile + (t >> 1), b = t & 1;
-      if (b == 0) wait_v(x);
+    for (int u = 0; ok && u < steps; ++u) {
+      const int t = taken, x = tile + (t >> 1), b = u & 1;
+      taken = st.next(t);
+      if (WINDOW ? t >> 1 != v_tile : (t & 1) == 0) { wait_v(x); v_tile = t >> 1; }
       wait(CH_P_READY + 2 * h + b, p_phase >> b & 1);
       p_phase ^= 1u << b;
       if (!ok) break;
       tmem_fence_after();
-      const uint64_t v = desc_mn_major(ring + (2 * (x & 1) + 1) * CH_SLOT + b * (CH_STEP * 128), CH_PANEL);
+      const uint64_t v = desc_mn_major(ring + (2 * (x & 1) + 1) * CH_SLOT + (t & 1) * (CH_STEP * 128), CH_PANEL);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)                         // 16 keys: 8 columns of P, two groups of eight rows of V
-        mma_ts(one, t_o, t_s + CH_STEP * b + 8 * kk, v + kk * (2048 >> 4), PV, t > 0 || kk > 0 ? 1u : 0u);
+        mma_ts(one, t_o, t_s + CH_STEP * b + 8 * kk, v + kk * (2048 >> 4), PV, u > 0 || kk > 0 ? 1u : 0u);
       mma_commit(one, bar + 8 * (CH_O_DONE + 2 * h + b));
-      if (b == 1 || t == steps - 1) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1) + 1));
-      if (t + 2 < steps) scores(t + 2);
+      if (u == steps - 1 || (WINDOW ? taken >> 1 != t >> 1 : (t & 1) == 1)) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1) + 1));
+      if (u + 2 < steps) scores(u + 2);
     }
     // tiles that this half sees nothing of: their slots go back as they come
     if (steps == 0) mma_commit(one, bar + 8 * CH_Q_FREE);
-    for (int x = tile + ((steps + 1) >> 1); ok && x < tile + n; ++x) {
+    for (int x = tile + ((end + 1) >> 1); ok && x < tile + n; ++x) {
       wait_k(x);
       if (ok) mma_commit(one, bar + 8 * (CH_FREE + 2 * (x & 1)));
       wait_v(x);
@@ -240,7 +261,7 @@ __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int 
 }
 
 // One warp: values in masked places.
-template <bool BF16>
+template <bool BF16, bool WINDOW>
 __device__ void chunk_values(const PagedArgs& A, PagedWalk<CH_KEYS> walk, unsigned char* ring_ptr, uint32_t bar, const ChunkTile* s_info,
                              int* s_again, int* s_trouble) {
   const int lane = threadIdx.x & 31;
@@ -262,9 +283,9 @@ __device__ void chunk_values(const PagedArgs& A, PagedWalk<CH_KEYS> walk, unsign
           for (int g = 0; g < 8; ++g) {
             const int key0 = info.key0 + 16 * g;
             const bool gone = (info.there >> g & 1) == 0 || key0 >= s.item.hi;
-            if (!gone && key0 + 15 <= p_first && (A.window == 0 || key0 > p_last - A.window || key0 + 15 < A.sinks)) continue;
+            if (!gone && key0 + 15 <= p_first && (!WINDOW || key0 > p_last - A.window || key0 + 15 < A.sinks)) continue;
             uint4* at = reinterpret_cast<uint4*>(ring_ptr + slot * CH_SLOT + (16 * g + (lane >> 3)) * 128 + (lane & 7) * 16);
-            const int mine = key0 + (lane >> 3), low = A.window > 0 ? p_first - A.window : -1;   // (keys up to `low`, behind the sinks: no row's)
+            const int mine = key0 + (lane >> 3), low = WINDOW ? p_first - A.window : -1;   // (keys up to `low`, behind the sinks: no row's)
             if (gone || key0 + 15 >= s.item.hi || (key0 <= low && key0 + 15 >= A.sinks)) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -298,7 +319,7 @@ __device__ void chunk_values(const PagedArgs& A, PagedWalk<CH_KEYS> walk, unsign
   if (!ok) *s_trouble = 1;
 }
 
-template <bool BF16>
+template <bool BF16, bool WINDOW>
 __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint32_t bar, uint32_t tmem, const ChunkTile* s_info,
                               const int* s_again, int* s_trouble, int cta, unsigned char* stage) {
   constexpr float RAISE = PagedWeights<BF16>::RAISE, LIFT = PagedWeights<BF16>::LIFT;
@@ -316,14 +337,16 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
     const int tok = row / A.g, n_tok = min(tm, s.item.n_tok - h * tm);      // new tokens of this half
     const bool live = tok < n_tok && row < tm * A.g;
     const int item_row = h * tm * A.g + row;
-    const int n = s.k1 - s.k0, steps = chunk_steps(A, s, h, tm);
+    const int n = s.k1 - s.k0;
+    const ChunkSteps<WINDOW> st(A, s, h, tm);
+    const int steps = st.n;
     const int pos = live ? s.item.p0 + h * tm + tok : -1;
     // the tokens of this warp's live rows, for whether a step needs masks
     const int tok_w = (quad * 32) / A.g, tok_e = min((quad * 32 + 31) / A.g, n_tok - 1);
     const int pos_w = s.item.p0 + h * tm + tok_w, pos_e = s.item.p0 + h * tm + tok_e;
     float m = -INFINITY, l = 0.f;
-    for (int t = 0; t < steps; ++t) {
-      const int b = t & 1;
+    for (int u = 0, t = st.next(-1); u < steps; ++u, t = st.next(t)) {
+      const int b = u & 1, half = t & 1;
       ok = bar_wait_warp(bar + 8 * (CH_S_FULL + 2 * h + b), s_phase >> b & 1);
       s_phase ^= 1u << b;
       if (!ok) break;
@@ -331,11 +354,11 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
       const ChunkTile info = s_info[(tile + (t >> 1)) % CH_INFO];
       uint32_t v[64];
       tmem_ld64(t_s + CH_STEP * b, v);
-      const int key0 = info.key0 + CH_STEP * b, pages = info.there >> (4 * b) & 15;
-      if (key0 + CH_STEP - 1 > pos_w || pages != 15 || (A.window > 0 && key0 <= pos_e - A.window && key0 + CH_STEP > A.sinks)) {
+      const int key0 = info.key0 + CH_STEP * half, pages = info.there >> (4 * half) & 15;
+      if (key0 + CH_STEP - 1 > pos_w || pages != 15 || (WINDOW && key0 <= pos_e - A.window && key0 + CH_STEP > A.sinks)) {
         // keys the row sees: below `over`, and, under a window, from `from` on or below the sinks (relative to the step), where the
         // page is there; a bit each
-        const int over = min(pos + 1, s.item.hi) - key0, from = A.window > 0 ? pos - A.window + 1 - key0 : -0x3fffffff, sink = A.sinks - key0;
+        const int over = min(pos + 1, s.item.hi) - key0, from = WINDOW ? pos - A.window + 1 - key0 : -0x3fffffff, sink = A.sinks - key0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           auto below = [&](int x) {                          // bits of keys 32 c + i < x
@@ -359,7 +382,7 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
       if (__any_sync(0xffffffffu, live && high > m + RAISE)) {
         const float to = fmaxf(m, high), f = to == -INFINITY ? 1.f : exp2_approx(m - to);   // (m = -inf: 0)
         m = to; l *= f;
-        if (t > 0) {                                         // the accumulator, once the product of the step before is done
+        if (u > 0) {                                         // the accumulator, once the product of the step before is done
           ok = product_done(b ^ 1);
           if (!ok) break;
           tmem_fence_after();
@@ -474,7 +497,7 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
   if (!ok) *s_trouble = 1;
 }
 
-template <bool BF16>
+template <bool BF16, bool WINDOW>
 __global__ void __launch_bounds__(CH_THREADS, 1)
 paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v) {
@@ -519,11 +542,11 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
     const int role = warp - CH_SOFTMAX_WARPS;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_HELPER_REGS));
     if (role == 0) chunk_load<BF16>(A, &tm_q, &tm_k, &tm_v, walk, q32, ring, bar, s_info, &s_trouble);
-    else if (role < 3) chunk_products<BF16>(A, walk, role - 1, q32, ring, bar, tmem, s_info, &s_trouble);
-    else chunk_values<BF16>(A, walk, ring_ptr, bar, s_info, s_again, &s_trouble);
+    else if (role < 3) chunk_products<BF16, WINDOW>(A, walk, role - 1, q32, ring, bar, tmem, s_info, &s_trouble);
+    else chunk_values<BF16, WINDOW>(A, walk, ring_ptr, bar, s_info, s_again, &s_trouble);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CH_SOFTMAX_REGS));
-    chunk_softmax<BF16>(A, walk, bar, tmem, s_info, s_again, &s_trouble, cta, ring_ptr + CH_SLOTS * CH_SLOT + warp * CH_STAGE);
+    chunk_softmax<BF16, WINDOW>(A, walk, bar, tmem, s_info, s_again, &s_trouble, cta, ring_ptr + CH_SLOTS * CH_SLOT + warp * CH_STAGE);
   }
   tmem_fence_before();
   __syncthreads();
@@ -548,15 +571,15 @@ static bool chunk_q_map(CUtensorMap* tm, const PagedArgs& A, bool bf16) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool BF16>
+template <bool BF16, bool WINDOW>
 static int chunk_launch(const PagedArgs& A, const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
-  constexpr auto kernel = paged_chunk_kernel<BF16>;
+  constexpr auto kernel = paged_chunk_kernel<BF16, WINDOW>;
   // (the register split waits for ever if the block was launched with fewer than it hands out)
   static const int regs = [] {
     cudaFuncAttributes attr;
     return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
   }();
-  const cudaError_t e = allow_dynamic_smem_once<paged_chunk_kernel<BF16>>(CH_SMEM);
+  const cudaError_t e = allow_dynamic_smem_once<paged_chunk_kernel<BF16, WINDOW>>(CH_SMEM);
   if (e != cudaSuccess || regs * CH_THREADS < CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS) {
     g_last_cuda_error = (int)e;
     return RDKV_ERR_LAUNCH;
@@ -570,7 +593,9 @@ static int chunk_launch(const PagedArgs& A, const CUtensorMap& tm_q, const CUten
 int paged_chunk_launch(const PagedArgs& A, bool bf16, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t st) {
   CUtensorMap tm_q;
   if (!chunk_q_map(&tm_q, A, bf16)) return RDKV_ERR_BAD_SHAPE;
-  return bf16 ? chunk_launch<true>(A, tm_q, tm_k, tm_v, st) : chunk_launch<false>(A, tm_q, tm_k, tm_v, st);
+  // (the window's masks and left-out steps in a kernel of their own: in one they cost the others 3 %, 2048 behind 6000 226 -> 233 us)
+  if (A.window > 0) return bf16 ? chunk_launch<true, true>(A, tm_q, tm_k, tm_v, st) : chunk_launch<false, true>(A, tm_q, tm_k, tm_v, st);
+  return bf16 ? chunk_launch<true, false>(A, tm_q, tm_k, tm_v, st) : chunk_launch<false, false>(A, tm_q, tm_k, tm_v, st);
 }
 
 }  // namespace rdkv

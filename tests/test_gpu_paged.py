@@ -321,6 +321,14 @@ def test_many_requests_and_few():
     run([3000], [700], 1, 4, 64, BF16, seed=25)
 
 
+@pytest.mark.parametrize("sinks", [0, 1, 64, 65, 128, 129, 192, 193, 600])
+@pytest.mark.parametrize("window", [1, 63, 64, 65, 300])
+def test_windows_and_sinks_that_begin_and_end_in_either_half_of_a_tile(window, sinks):
+    """Half tiles that none of an item's rows see are left out, and nothing else is."""
+    for lead in (0, 31, 32, 63, 64, 65, 96, 127):
+        run([700 + lead, 1500], [200 + lead, 130], 1, 4, 32, BF16, seed=80 + lead, window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("new", [[1, 1], [150, 70]])
 def test_broadcast_views(new):
     """Queries are taken as they are; pages and results are refused."""

@@ -36,6 +36,7 @@ constexpr size_t CH_SMEM = (size_t)(2 + CH_SLOTS) * CH_SLOT + CH_SOFTMAX_WARPS *
 constexpr int CH_INFO = 8;                        // tiles whose description is kept (a softmax warp is at most three behind the loads)
 // Every CH_POLY-th pair of exponentials goes to the FMA units.  (2048 behind 6000, thousand cycles: every 4th 369, every 8th 396, none 385.)
 constexpr int CH_POLY = 4;
+constexpr int CH_WORKS = 4;                       // segments whose description is kept
 // (Six requests of up to 500 tokens behind up to 3000: 95 us with a fixed cost of one tile an item, 87 with two, 91 with three; cuts that
 // leave a tile or two are moved: an item's records are 135 KB.)
 constexpr int CH_FIXED = 2, CH_SNAP = 3, CH_WHOLE = 8;
@@ -44,9 +45,10 @@ static_assert(CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS <= 
               "the split draws on what the block was launched with");
 
 // Barriers: Q arrived / free; [2 half + buffer] scores done, weights written, product with the values done; [slot] tile arrived / free,
-// values looked after; [half] products ended early.
+// values looked after; [half] products ended early; [segment's place] its description written / no longer needed.
 enum { CH_Q_FULL = 0, CH_Q_FREE = 1, CH_S_FULL = 2, CH_P_READY = 6, CH_O_DONE = 10, CH_FULL = 14, CH_FREE = CH_FULL + CH_SLOTS,
-       CH_V_OK = CH_FREE + CH_SLOTS, CH_DRAINED = CH_V_OK + CH_SLOTS, CH_BARS = CH_DRAINED + 2 };
+       CH_V_OK = CH_FREE + CH_SLOTS, CH_DRAINED = CH_V_OK + CH_SLOTS, CH_W_FULL = CH_DRAINED + 2, CH_W_FREE = CH_W_FULL + CH_WORKS,
+       CH_BARS = CH_W_FREE + CH_WORKS };
 
 struct ChunkTile { int key0, there, edge; };      // first key, a bit per 16 keys whose page is there, some row does not see all of it
 
@@ -93,6 +95,7 @@ __device__ __forceinline__ bool chunk_edge(const PagedArgs& A, const PagedItem& 
 template <bool WINDOW>
 struct ChunkSteps {
   int n, end, skip_sinks, skip_front;             // steps taken; end of all; the two that may be left out (-1: none)
+  ChunkSteps() = default;
   __device__ __forceinline__ ChunkSteps(const PagedArgs& A, const PagedSegment& s, int h, int tm) : n(0), end(0), skip_sinks(-1), skip_front(-1) {
     const int n_tok = min(tm, s.item.n_tok - h * tm);
     if (n_tok <= 0) return;
@@ -112,17 +115,42 @@ struct ChunkSteps {
   }
 };
 
-template <bool BF16>
+// A segment as the loading warp worked it out, for the other warps.  (Each of them used to walk the line of units by itself: that cost the
+// softmax warps 2400 cycles a segment, most of them waits for code that is seldom run.)
+template <bool WINDOW>
+struct ChunkWork { PagedSegment s; ChunkSteps<WINDOW> st[2]; };   // s.k0 < 0: there are no more
+
+template <bool WINDOW>
+__device__ __forceinline__ bool chunk_work(const ChunkWork<WINDOW>* works, unsigned at, uint32_t bar, bool& ok) {
+  ok = ok && bar_wait_warp(bar + 8 * (CH_W_FULL + at % CH_WORKS), (at / CH_WORKS) & 1);
+  return ok && works[at % CH_WORKS].s.k0 >= 0;
+}
+__device__ __forceinline__ void chunk_work_done(unsigned at, uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(bar + 8 * (CH_W_FREE + at % CH_WORKS));
+}
+
+template <bool BF16, bool WINDOW>
 __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
-                           PagedWalk<CH_KEYS> walk, uint32_t q32, uint32_t ring, uint32_t bar, ChunkTile* s_info, int* s_trouble) {
+                           PagedWalk<CH_KEYS> walk, uint32_t q32, uint32_t ring, uint32_t bar, ChunkTile* s_info, ChunkWork<WINDOW>* works, int* s_trouble) {
   const int lane = threadIdx.x & 31, tm = A.group >> 1;
   const int rows_log2 = min(A.page_log2, 7), rows = 1 << rows_log2, per_log2 = 7 - rows_log2, per_tile = 1 << per_log2, batch = 32 >> per_log2;
   const int box = lane >> 1, panel = lane & 1;               // this lane's box of a tile
-  unsigned use = 0, tile = 0, segments = 0;                  // slots filled; tiles; segments
+  unsigned use = 0, tile = 0, segments = 0, published = 0;   // slots filled; tiles; segments that have some; all segments
   PagedSegment s;
   bool ok = true;
+  auto publish = [&]() {
+    const int at = published % CH_WORKS;
+    if (published >= CH_WORKS) ok = ok && bar_wait_warp(bar + 8 * (CH_W_FREE + at), (published / CH_WORKS - 1) & 1);
+    if (!ok) return;
+    if (lane < 2) works[at].st[lane] = ChunkSteps<WINDOW>(A, s, lane, tm);
+    if (lane == 0) works[at].s = s;
+    __syncwarp();
+    if (lane == 0) bar_arrive(bar + 8 * (CH_W_FULL + at));
+    ++published;
+  };
   while (ok && walk.next(A, s)) {
-    if (s.k0 == s.k1) continue;
+    if (s.k0 == s.k1) { publish(); continue; }
     const int32_t* table = A.table + s.i * A.table_stride;
     auto page_of = [&](int k) {                              // lane's entry of the batch that starts with tile k
       const int kk = k + (lane >> per_log2);
@@ -169,8 +197,10 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
           tma_load_4d(ring + slot * CH_SLOT + panel * CH_PANEL + box * rows * 128, t == 0 ? tm_k : tm_v, 64 * panel, key0 & (A.page - 1),
                       s.head, id, bar + 8 * (CH_FULL + slot));
       }
+      if (k == s.k0) publish();                              // (behind the first loads, which the start waits for)
     }
   }
+  if (ok) { s.k0 = s.k1 = -1; s.item.n_tok = 0; publish(); }
   if (!ok) {                                                 // wait (again bounded) for the copies in flight
     *s_trouble = 1;
     for (unsigned n = use < CH_SLOTS ? 0 : use - CH_SLOTS; n < use; ++n) bar_wait(bar + 8 * (CH_FULL + n % CH_SLOTS), (n / CH_SLOTS) & 1);
@@ -182,15 +212,13 @@ __device__ __forceinline__ int chunk_uniform(int x) { return __shfl_sync(0xfffff
 
 // Two warps: the products of half 0, of half 1.
 template <bool BF16, bool WINDOW>
-__device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int h, uint32_t q32, uint32_t ring, uint32_t bar, uint32_t tmem_,
-                               const ChunkTile* s_info, int* s_trouble) {
+__device__ void chunk_products(int h, uint32_t q32, uint32_t ring, uint32_t bar, uint32_t tmem_, const ChunkTile* s_info,
+                               const ChunkWork<WINDOW>* works, int* s_trouble) {
   constexpr uint32_t QK = mma_idesc<BF16>(CH_STEP, false), PV = mma_idesc<BF16>(128, true);
-  const int tm = A.group >> 1;
   const uint32_t t_s = (uint32_t)chunk_uniform((int)tmem_ + 128 * h), t_o = t_s + 256, one = elect_one();
   const uint64_t q = desc_k_major((uint32_t)chunk_uniform((int)(q32 + h * CH_SLOT)));
   int tile = 0;                                              // tile x is in slots 2 (x & 1) and the next, their phase is x >> 1
   uint32_t segments = 0, v_ok = 0, p_phase = 0;              // a bit per V slot / buffer: parity of its next use
-  PagedSegment s;
   bool ok = true;
   auto wait = [&](int b, uint32_t parity) { ok = ok && bar_wait_warp(bar + 8 * b, parity); };
   auto wait_k = [&](int x) { wait(CH_FULL + 2 * (x & 1), x >> 1 & 1); };
@@ -201,10 +229,12 @@ __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int 
       v_ok ^= 1u << (x & 1);
     }
   };
-  while (ok && chunk_uniform(walk.next(A, s))) {
-    const int n = chunk_uniform(s.k1 - s.k0);
+  for (unsigned at = 0; chunk_uniform(chunk_work(works, at, bar, ok)); ++at) {
+    const ChunkWork<WINDOW>& work = works[at % CH_WORKS];
+    const int n = chunk_uniform(work.s.k1 - work.s.k0);
+    ChunkSteps<WINDOW> st = work.st[h];
+    chunk_work_done(at, bar);
     if (n == 0) continue;
-    ChunkSteps<WINDOW> st(A, s, h, tm);
     st.skip_sinks = chunk_uniform(st.skip_sinks); st.skip_front = chunk_uniform(st.skip_front);
     const int steps = chunk_uniform(st.n), end = chunk_uniform(st.end);
     wait(CH_Q_FULL, segments++ & 1);
@@ -262,13 +292,14 @@ __device__ void chunk_products(const PagedArgs& A, PagedWalk<CH_KEYS> walk, int 
 
 // One warp: values in masked places.
 template <bool BF16, bool WINDOW>
-__device__ void chunk_values(const PagedArgs& A, PagedWalk<CH_KEYS> walk, unsigned char* ring_ptr, uint32_t bar, const ChunkTile* s_info,
+__device__ void chunk_values(const PagedArgs& A, unsigned char* ring_ptr, uint32_t bar, const ChunkTile* s_info, const ChunkWork<WINDOW>* works,
                              int* s_again, int* s_trouble) {
   const int lane = threadIdx.x & 31;
   unsigned use = 0, tile = 0, segments = 0;
-  PagedSegment s;
   bool ok = true;
-  while (ok && walk.next(A, s)) {
+  for (unsigned at = 0; chunk_work(works, at, bar, ok); ++at) {
+    const PagedSegment s = works[at % CH_WORKS].s;
+    chunk_work_done(at, bar);
     if (s.k0 == s.k1) continue;
     const int p_first = s.item.p0, p_last = s.item.p0 + s.item.n_tok - 1;
     for (int j = s.k0; ok && j < s.k1; ++j, ++tile) {
@@ -320,7 +351,7 @@ __device__ void chunk_values(const PagedArgs& A, PagedWalk<CH_KEYS> walk, unsign
 }
 
 template <bool BF16, bool WINDOW>
-__device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint32_t bar, uint32_t tmem, const ChunkTile* s_info,
+__device__ void chunk_softmax(const PagedArgs& A, uint32_t bar, uint32_t tmem, const ChunkTile* s_info, const ChunkWork<WINDOW>* works,
                               const int* s_again, int* s_trouble, int cta, unsigned char* stage) {
   constexpr float RAISE = PagedWeights<BF16>::RAISE, LIFT = PagedWeights<BF16>::LIFT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = warp >> 2, quad = warp & 3, row = quad * 32 + lane, tm = A.group >> 1;
@@ -331,14 +362,15 @@ __device__ void chunk_softmax(const PagedArgs& A, PagedWalk<CH_KEYS> walk, uint3
   // The product of buffer b's last step.  (A barrier a buffer: the one of the step before that is done when the scores that
   // came after it are, so no phase can be mistaken for another.)
   auto product_done = [&](int b) { return bar_wait_warp(bar + 8 * (CH_O_DONE + 2 * h + b), (s_phase >> b & 1) ^ 1u); };
-  PagedSegment s;
   bool ok = true;
-  while (ok && walk.next(A, s)) {
+  for (unsigned at = 0; chunk_work(works, at, bar, ok); ++at) {
+    const PagedSegment s = works[at % CH_WORKS].s;           // (a copy: with reads from shared memory in the steps they took 3 % longer)
+    const ChunkSteps<WINDOW> st = works[at % CH_WORKS].st[h];
+    chunk_work_done(at, bar);
     const int tok = row / A.g, n_tok = min(tm, s.item.n_tok - h * tm);      // new tokens of this half
     const bool live = tok < n_tok && row < tm * A.g;
     const int item_row = h * tm * A.g + row;
     const int n = s.k1 - s.k0;
-    const ChunkSteps<WINDOW> st(A, s, h, tm);
     const int steps = st.n;
     const int pos = live ? s.item.p0 + h * tm + tok : -1;
     // the tokens of this warp's live rows, for whether a step needs masks
@@ -506,6 +538,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   __shared__ ChunkTile s_info[CH_INFO];
   __shared__ PagedPlaceScratch s_place;
   __shared__ uint32_t s_tmem;
+  __shared__ ChunkWork<WINDOW> s_work[CH_WORKS];
   __shared__ int s_again[4];                                 // segment (its number + 1) whose rows are done again
   __shared__ int s_trouble;
   const int tid = threadIdx.x, warp = tid >> 5, cta = blockIdx.x;
@@ -514,6 +547,8 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
     bar_init(bar + 8 * CH_Q_FULL, 1); bar_init(bar + 8 * CH_Q_FREE, 2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { bar_init(bar + 8 * (CH_S_FULL + i), 1); bar_init(bar + 8 * (CH_P_READY + i), 4); bar_init(bar + 8 * (CH_O_DONE + i), 1); }
+#pragma unroll
+    for (int i = 0; i < CH_WORKS; ++i) { bar_init(bar + 8 * (CH_W_FULL + i), 1); bar_init(bar + 8 * (CH_W_FREE + i), CH_SOFTMAX_WARPS + 3); }
     bar_init(bar + 8 * CH_DRAINED, 1); bar_init(bar + 8 * (CH_DRAINED + 1), 1);
 #pragma unroll
     for (int i = 0; i < CH_SLOTS; ++i) {
@@ -536,17 +571,16 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = s_tmem;
-  const PagedWalk<CH_KEYS> walk(A, from, to);
   unsigned char* ring_ptr = ch_raw + 2 * CH_SLOT;
   if (warp >= CH_SOFTMAX_WARPS) {
     const int role = warp - CH_SOFTMAX_WARPS;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_HELPER_REGS));
-    if (role == 0) chunk_load<BF16>(A, &tm_q, &tm_k, &tm_v, walk, q32, ring, bar, s_info, &s_trouble);
-    else if (role < 3) chunk_products<BF16, WINDOW>(A, walk, role - 1, q32, ring, bar, tmem, s_info, &s_trouble);
-    else chunk_values<BF16, WINDOW>(A, walk, ring_ptr, bar, s_info, s_again, &s_trouble);
+    if (role == 0) chunk_load<BF16, WINDOW>(A, &tm_q, &tm_k, &tm_v, PagedWalk<CH_KEYS>(A, from, to), q32, ring, bar, s_info, s_work, &s_trouble);
+    else if (role < 3) chunk_products<BF16, WINDOW>(role - 1, q32, ring, bar, tmem, s_info, s_work, &s_trouble);
+    else chunk_values<BF16, WINDOW>(A, ring_ptr, bar, s_info, s_work, s_again, &s_trouble);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CH_SOFTMAX_REGS));
-    chunk_softmax<BF16, WINDOW>(A, walk, bar, tmem, s_info, s_again, &s_trouble, cta, ring_ptr + CH_SLOTS * CH_SLOT + warp * CH_STAGE);
+    chunk_softmax<BF16, WINDOW>(A, bar, tmem, s_info, s_work, s_again, &s_trouble, cta, ring_ptr + CH_SLOTS * CH_SLOT + warp * CH_STAGE);
   }
   tmem_fence_before();
   __syncthreads();

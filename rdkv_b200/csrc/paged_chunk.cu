@@ -8,7 +8,7 @@
 // the weights of step t are used up, so a warpgroup has its next scores waiting when it is done with a step (with one
 // buffer of 128 scores a half had nothing to do between its weights and its next scores, 1700 cycles of 3900 a tile).
 //
-// 12 warps: two warpgroups of softmax (half 0, half 1), and one of helpers: one warp brings in Q and the tiles (tiled TMA, one box
+// 12 warps: two warpgroups of softmax (half 0, half 1), and one of helpers: one warp works out the segments and brings in Q and the tiles (tiled TMA, one box
 // per page and 64-channel panel, 128-byte swizzle, four slots of 32 KB for K and V in turn), two issue the products of a
 // half each, one looks after masked values: 0 x NaN is NaN, so in tiles that some row of the item does not see whole it
 // sets values of keys that no row sees to zero before the product, and looks for values that are not finite among the

@@ -329,6 +329,22 @@ def test_windows_and_sinks_that_begin_and_end_in_either_half_of_a_tile(window, s
         run([700 + lead, 1500], [200 + lead, 130], 1, 4, 32, BF16, seed=80 + lead, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("every", [0, 1, 7, 25])
+def test_chunks_that_see_nothing_one_after_another(every):
+    """Runs of items without a tile, longer than what the warps of a CTA may be apart, between items with some."""
+    from rdkv_b200.paged import paged_attention
+    lens = [300 if every and i % every == 0 else 0 for i in range(50)]
+    k, v, table = R.build_cache([300] * 50, 2, 32, BF16, seed=91)
+    new = [(130, 64, 17, 200)[i % 4] for i in range(50)]
+    q = randn(sum(new), 8, 128, seed=92, dtype=BF16)
+    for kw in ({}, dict(window=40, sinks=3)):
+        got = paged_attention(q, k, v, table, starts(new), ints(lens), max_new=200, check_status=True, **kw)
+        check(got, R.attention(q, k, v, table, starts(new), ints(lens), **kw))
+        rec = torch.full((q.shape[0] * 8, 132), 7.0, device="cuda")
+        paged_attention(q, k, v, table, starts(new), ints(lens), max_new=200, out_partial=rec, check_status=True, **kw)
+        assert torch.isfinite(rec[:, 1]).all() and ((rec[:, 1] == 0) == (rec[:, 0] == float("-inf"))).all()
+
+
 @pytest.mark.parametrize("new", [[1, 1], [150, 70]])
 def test_broadcast_views(new):
     """Queries are taken as they are; pages and results are refused."""

@@ -530,6 +530,13 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
       workspace_bytes < rdkv_paged_attention_workspace(g.n_requests, g.n_tokens, g.H_q, g.H_kv, g.max_new))
     return RDKV_ERR_BAD_ARG;
+  // queries are read, results and records written, 16 bytes at a time
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(out_partial) & 15))
+    return RDKV_ERR_BAD_ARG;
+  auto whole = [](int64_t n, int64_t stride) { return n == 1 || (stride & 7) == 0; };   // (strides of dimensions of one element mean nothing)
+  if (!whole(g.n_tokens, g.q_tok_stride) || !whole(g.H_q, g.q_head_stride) ||
+      (out != nullptr && (!whole(g.n_tokens, out_tok_stride) || !whole(g.H_q, out_head_stride))))
+    return RDKV_ERR_BAD_SHAPE;
   PagedArgs A = {};
   A.q = (const uint16_t*)q; A.k = (const uint16_t*)k_pages; A.v = (const uint16_t*)v_pages;
   A.q_tok = g.q_tok_stride; A.q_head = g.q_head_stride;

@@ -269,8 +269,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
             raise ValueError("either out or out_partial")
         require_cuda(out_partial, "out_partial")
         if (out_partial.dtype != torch.float32 or not out_partial.is_contiguous() or out_partial.device != q.device
-                or out_partial.numel() != q.shape[0] * q.shape[1] * PARTIAL_STRIDE):
-            raise ValueError(f"out_partial must be contiguous float32 [{q.shape[0] * q.shape[1]},{PARTIAL_STRIDE}] on {q.device}")
+                or out_partial.numel() != q.shape[0] * q.shape[1] * PARTIAL_STRIDE or out_partial.data_ptr() & 15):
+            raise ValueError(f"out_partial must be contiguous float32 [{q.shape[0] * q.shape[1]},{PARTIAL_STRIDE}] on {q.device}, on 16 bytes")
         os, out_ptr, rec_ptr, zero = (0, 0), None, out_partial.data_ptr(), 0
     ws = kv_lens.new_empty(n_ws)
     status = lib().rdkv_paged_attention(args, q.data_ptr(), k_ptr, v_ptr, block_tables.data_ptr(), q_start.data_ptr(), kv_lens.data_ptr(),

@@ -654,7 +654,7 @@ int rdkv_paged_append(const rdkv_paged_append_args* args, const void* k, const v
 
 /* Attention of the new tokens of n_requests requests over their pages (fp16 / bf16; page_size a power of two, 16 to 1024;
  * up to 16 query heads a KV head; bases on 16 bytes, strides of whole 16 bytes).  Query row q_start[i]+j is request i's
- * token kv_lens[i]-n_i+j (n_i = q_start[i+1]-q_start[i]); it sees the tokens up to itself, under window > 0 only the last
+ * token kv_lens[i]-n_i+j (n_i = q_start[i+1]-q_start[i], whether n_tokens rows hold all of them or not); it sees the tokens up to itself, under window > 0 only the last
  * `window` of them and the first `sinks`, and none whose page number is outside [0, n_pages).  max_new: the longest chunk
  * (a hint: it chooses the kernel).  Either out [n_tokens][H_q][128] (rows in front of q_start[0] and from
  * q_start[n_requests] on: zeroed with zero_padding, else left) or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace:

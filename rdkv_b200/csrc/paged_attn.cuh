@@ -1,7 +1,7 @@
 // Attention of the new tokens of a batch of requests over their paged keys and values: what its two kernels share.
 //
 // Request i's cache holds kv_len_i tokens, the last n_i = q_start[i+1] - q_start[i] of them new ones: query row j of
-// the request stands at position p = kv_len_i - n_i + j and sees key s if s <= p, and, under a window of w tokens,
+// the request stands at position p = kv_len_i - n_i + j (also where the tensor has not all of the n_i rows) and sees key s if s <= p, and, under a window of w tokens,
 // s > p - w or s < sinks, and if the page of s is there (a page number outside the pages stands for none):
 //   o = sum_s softmax_s(scale * q.k_s) v_s;  a row that sees nothing is zero (record: m = -inf, l = 0).
 //
@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t paged_fma2(uint32_t x, uint32_t y, uint32_t 
 }
 
 // ── items ───────────────────────────────────────────────────────────────────
-struct PagedRequest { int q0, n, len; };          // first query row, new tokens, tokens
+struct PagedRequest { int q0, n, len; };          // first query row, query rows, tokens up to the last row's (at most 0: none is seen)
 struct PagedItem {
   int tok0, n_tok;                                // query rows of the group
   int p0;                                         // position of the first (below zero: it sees nothing)
@@ -97,8 +97,9 @@ struct PagedItem {
 __device__ __forceinline__ PagedRequest paged_request(const PagedArgs& A, int i) {
   PagedRequest r;
   r.q0 = min(max(A.q_start[i], 0), A.T);
-  r.n = min(max(A.q_start[i + 1], r.q0), A.T) - r.q0;
-  r.len = max(A.kv_lens[i], 0);
+  const int end = A.q_start[i + 1], t1 = min(max(end, r.q0), A.T);
+  r.n = t1 - r.q0;
+  r.len = max(max(A.kv_lens[i], 0) - max(end - A.T, 0), 0);   // (tokens behind the last row there is are not this call's, but they are among kv_lens)
   return r;
 }
 // Whether q_start falls behind request i (one of a batch's requests; other numbers: no).

@@ -223,7 +223,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     q [T,H_q,128] (fp16 / bf16, the pages' dtype, after rotation); k_pages, v_pages [n_pages,H_kv,page_size,128] with
     page_size a power of two from 16 to 1024 and up to 16 query heads a KV head; block_tables int32 [S,width], q_start
     int32 [S+1], kv_lens int32 [S] (as :func:`build_block_tables` leaves them: q_start must not fall).  The last ``q_start[i+1]-q_start[i]`` of
-    request i's ``kv_lens[i]`` tokens are the new ones, whose keys and values are in the pages already.  A token
+    request i's ``kv_lens[i]`` tokens are the new ones, whose keys and values are in the pages already; where q_start goes past
+    T, the rows that q has keep the places they have among these (a step with fewer token places than tokens).  A token
     sees its request's tokens up to itself; with ``window`` > 0 only the last ``window`` of them (itself included)
     and the request's first ``sinks``.  Tokens whose page is missing (an entry outside the pages) are not seen, and what
     stands in masked places does not matter, whatever it is.  A token that sees nothing gets zeros.

@@ -27,7 +27,7 @@ from torch import Tensor
 
 from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, check, lib, q_dtype_tag, raw_stream,
                    require_cuda, separate_rows)
-from .rope import axes_check, empty_rows
+from .rope import axes_check, empty_rows, plain_sections
 
 MAX_REQUESTS = 16384
 _TABLES_CALLS, _APPEND_CALLS, _ATTENTION_CALLS = CallCache(), CallCache(), CallCache()
@@ -152,9 +152,11 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     [T]: slot of every token; a slot below zero or behind the last page is not written.  The slots of a call must
     differ from one another.  q [T,H_q,128] of the same dtype goes to ``q_out`` (default: a new tensor; may be q
     itself), which is returned; k is not changed.  positions [T] or [axes,T], inv_freq and sections: see ``rope_axes``."""
+    if sections is not None:
+        sections = plain_sections(sections)
     key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), k_pages.shape, k_pages.stride(),
            k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype, v_pages.get_device(), slot_map.shape,
-           slot_map.stride(), slot_map.dtype, slot_map.get_device(), None if sections is None else tuple(sections),
+           slot_map.stride(), slot_map.dtype, slot_map.get_device(), sections,
            None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.get_device()),
            None if inv_freq is None else (inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.get_device()),
            None if q is None else (q.shape, q.stride(), q.dtype, q.get_device()),
@@ -236,6 +238,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     last one's are padding: zero in an ``out`` that the
     call allocates, left as they were in one that it is given (which must not be q itself).  ``out_partial`` float32 [T*H_q,132] receives
     un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
+    window, sinks = int(window), int(sinks)                # (numbers: a key must not go by the identity of a tensor that holds one)
+    max_new, scale = None if max_new is None else int(max_new), None if scale is None else float(scale)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape,
            v_pages.stride(), v_pages.dtype, v_pages.get_device(), block_tables.shape, block_tables.stride(), block_tables.dtype,
            block_tables.get_device(), q_start.shape, q_start.stride(), q_start.dtype, q_start.get_device(), kv_lens.shape, kv_lens.stride(),
@@ -308,10 +312,10 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
         raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError("window and sinks must not be negative, and sinks need a window")
-    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    scale = HEAD_DIM ** -0.5 if scale is None else scale
     if not 1e-30 < scale < 1e30:                           # (an ordinary number in 32 bits)
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    max_new = T if max_new is None else min(int(max_new), T)
+    max_new = T if max_new is None else min(max_new, T)
     if max_new < 0:
         raise ValueError("max_new must not be negative")
     ks, vs = k_pages.stride()[:3], v_pages.stride()[:3]
@@ -324,5 +328,5 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
         q_tok_stride=q.stride(0), q_head_stride=q.stride(1), k_page_stride=ks[0], k_head_stride=ks[1], k_row_stride=ks[2], v_page_stride=vs[0],
         v_head_stride=vs[1], v_row_stride=vs[2], table_stride=block_tables.stride(0), dtype=q_dtype_tag(q), n_tokens=T, H_q=H_q, H_kv=H_kv,
         n_pages=n_pages, page_size=page_size, width=block_tables.shape[1], n_requests=S, max_new=max_new,
-        window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30), scale=scale)
+        window=min(window, 1 << 30), sinks=min(sinks, 1 << 30), scale=scale)
     return C.addressof(args), direct, n_ws, q.device.index, args, q.is_contiguous()

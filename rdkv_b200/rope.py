@@ -67,6 +67,11 @@ def empty_rows(t: Tensor, dense: bool) -> Tensor:
     return torch.empty_like(t) if dense else t.new_empty(t.shape)
 
 
+def plain_sections(sections: Sequence[int]) -> tuple:
+    """Sections as numbers (a key must not go by the identity of tensors that hold them)."""
+    return tuple(map(float, sections))
+
+
 _ROPE_CALLS = CallCache()
 
 
@@ -80,9 +85,11 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     lose nothing (below 2^24).  sections: how many of the 64 frequencies each axis owns, in order (text
     with one axis: all of them).  Returns (q_out, k_out): new tensors, or the given ones, which may be q and k
     themselves."""
+    if sections is not None:
+        sections = plain_sections(sections)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), positions.shape, positions.stride(),
            positions.dtype, positions.get_device(), inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.get_device(),
-           None if sections is None else tuple(sections), None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device()),
+           sections, None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.get_device()),
            None if k_out is None else (k_out.shape, k_out.stride(), k_out.dtype, k_out.get_device()))
     call = _ROPE_CALLS.get(key)
     if call is None:

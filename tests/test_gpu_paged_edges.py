@@ -56,3 +56,37 @@ def test_a_step_with_fewer_token_places_than_tokens():
     got = paged_attention(rot, kp, vp, table, plan.q_start, plan.kv_lens, check_status=True)
     kp, vp = kp.nan_to_num(), vp.nan_to_num()
     check(got, R.attention(rot, kp, vp, table, ints([0, 20, 25]), ints([20, 5])))
+
+
+# ── what a call remembers ────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 30]])
+def test_numbers_in_tensors_are_read_at_every_call(new):
+    """window, sinks, scale and max_new may be tensors of one element: their values count, not their identity."""
+    from rdkv_b200.paged import paged_attention
+    lens = [300, 111]
+    k, v, table = R.build_cache(lens, 2, 32, BF16, seed=31)
+    q = randn(sum(new), 8, 128, seed=32, dtype=BF16)
+    args = (q, k, v, table, starts(new), ints(lens))
+    window, sinks, scale, most = (torch.tensor(x) for x in (200, 3, 0.08, 1))
+    for w, s, c in ((200, 3, 0.08), (17, 0, 0.3), (64, 40, 0.01)):
+        window.fill_(w); sinks.fill_(s); scale.fill_(c); most.fill_(max(new))
+        got = paged_attention(*args, max_new=most, window=window, sinks=sinks, scale=scale)
+        assert torch.equal(got, paged_attention(*args, max_new=max(new), window=w, sinks=s, scale=float(scale)))
+
+
+def test_sections_in_tensors_are_read_at_every_call():
+    from rdkv_b200.paged import append_kv
+    from rdkv_b200.rope import rope_axes
+    T = 9
+    q, k = randn(T, 4, 128, seed=1, dtype=BF16), randn(T, 2, 128, seed=2, dtype=BF16)
+    pos = torch.randint(0, 5000, (2, T), generator=gen(3), device="cuda", dtype=torch.int32)
+    kp, vp = (torch.zeros(1, 2, 16, 128, dtype=BF16, device="cuda") for _ in range(2))
+    sections = [torch.tensor(64), torch.tensor(0)]
+    for n in (64, 20, 0):
+        sections[0].fill_(n); sections[1].fill_(64 - n)
+        want = rope_axes(q, k, pos, INV(), sections=(n, 64 - n))
+        for x, y in zip(rope_axes(q, k, pos, INV(), sections=sections), want):
+            assert torch.equal(x, y)
+        got = append_kv(k, k, kp, vp, torch.arange(T, device="cuda"), q=q, positions=pos, inv_freq=INV(), sections=sections)
+        assert torch.equal(got, want[0]) and torch.equal(kp[0, :, :T].transpose(0, 1), want[1])

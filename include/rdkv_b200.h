@@ -660,7 +660,7 @@ int rdkv_paged_append(const rdkv_paged_append_args* args, const void* k, const v
  * q_start[n_requests] on: zeroed with zero_padding, else left) or out_partial [n_tokens*H_q][132] records (m, l, -, -, o[128]).  workspace:
  * rdkv_paged_attention_workspace() bytes (16-byte aligned; of one call at a time), contents arbitrary.  Its first
  * rdkv_paged_attention_status_words() int32 are 0 after the call, or hold bit 1 (a device-side wait ran out: the
- * results are invalid) or 2 (q_start falls somewhere: no request was computed). */
+ * results are invalid) or 2 (q_start falls somewhere: no request was computed; with zero_padding all of out is zero). */
 typedef struct {
   int64_t q_tok_stride, q_head_stride;
   int64_t k_page_stride, k_head_stride, k_row_stride, v_page_stride, v_head_stride, v_row_stride;

@@ -433,7 +433,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     }
   }
   __syncthreads();
-  paged_zero_padding(A, DEC_THREADS);
+  paged_zero_padding(A, DEC_THREADS, s_trouble == 2);
   paged_report(A, s_trouble);
 }
 

@@ -378,11 +378,12 @@ __device__ __noinline__ void paged_slow_row(const PagedArgs& A, const PagedSegme
   }
 }
 
-// Rows that belong to no request, in a result that the call allocated: zeros.  All threads of the grid.
-__device__ __forceinline__ void paged_zero_padding(const PagedArgs& A, int n_threads) {
+// Rows that belong to no request (all rows, where q_start falls and nothing was computed), in a result that the call allocated: zeros.
+// All threads of the grid.
+__device__ __forceinline__ void paged_zero_padding(const PagedArgs& A, int n_threads, bool falls) {
   if (!A.zero_pad || A.rec != nullptr) return;
-  const int first = A.S > 0 ? min(max(A.q_start[0], 0), A.T) : A.T;
-  const int end = A.S > 0 ? min(max(A.q_start[A.S], first), A.T) : A.T;
+  const int first = A.S > 0 && !falls ? min(max(A.q_start[0], 0), A.T) : A.T;
+  const int end = A.S > 0 && !falls ? min(max(A.q_start[A.S], first), A.T) : A.T;
   const int64_t rows = (int64_t)(first + A.T - end) * A.H_q * 16;           // 16 bytes a step
   for (int64_t x = (int64_t)blockIdx.x * n_threads + threadIdx.x; x < rows; x += (int64_t)gridDim.x * n_threads) {
     const int64_t row = x >> 4, tk = row / A.H_q, hq = row - tk * A.H_q;

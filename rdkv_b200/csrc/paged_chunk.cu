@@ -586,7 +586,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   __syncthreads();
   tmem_fence_after();
   if (warp == CH_SOFTMAX_WARPS + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-  paged_zero_padding(A, CH_THREADS);
+  paged_zero_padding(A, CH_THREADS, s_trouble == 2);
   paged_report(A, s_trouble);
 }
 

@@ -233,7 +233,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
 
     max_new: the longest chunk of the batch (default T), which chooses the kernel: a hint, results do not depend on it.
     scale: of the scores, positive, default 1/sqrt(128).  check_status: wait for the kernels and raise if one of their
-    bounded waits ran out or q_start falls, in which case the results are invalid; without it the call returns at once.
+    bounded waits ran out or q_start falls, in which case the results are invalid (where q_start falls nothing is computed: an
+    ``out`` that the call allocates is zero, a given one as it was); without it the call returns at once.
     Returns ``out`` [T,H_q,128] in q's dtype.  Tokens in front of the first request's and behind the
     last one's are padding: zero in an ``out`` that the
     call allocates, left as they were in one that it is given (which must not be q itself).  ``out_partial`` float32 [T*H_q,132] receives

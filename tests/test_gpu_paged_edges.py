@@ -90,3 +90,19 @@ def test_sections_in_tensors_are_read_at_every_call():
             assert torch.equal(x, y)
         got = append_kv(k, k, kp, vp, torch.arange(T, device="cuda"), q=q, positions=pos, inv_freq=INV(), sections=sections)
         assert torch.equal(got, want[0]) and torch.equal(kp[0, :, :T].transpose(0, 1), want[1])
+
+
+# ── starts that fall ─────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("S,H_kv,max_new", [(2, 2, 1), (2, 2, 200), (60, 2, 1), (600, 1, 200)])
+def test_starts_that_fall_leave_zeros_in_a_result_of_the_call(S, H_kv, max_new):
+    """Without check_status nobody is told; what comes back is not what memory happened to hold."""
+    from rdkv_b200.paged import paged_attention
+    k, v, table = R.build_cache([40] * S, H_kv, 32, BF16, seed=63)
+    q = randn(S + 9, 4 * H_kv, 128, seed=64, dtype=BF16)
+    for at in sorted({1, S // 2 + 1, S}):
+        start = [i + 3 if i < at else i for i in range(S + 1)]
+        held = torch.full_like(q, 7.0)
+        del held                                                        # (the allocator hands out this memory next)
+        out = paged_attention(q, k, v, table, ints(start), ints([40] * S), max_new=max_new)
+        assert (out == 0).all()

@@ -15,8 +15,8 @@
 // shared memory; there is no line of units to find a place in and no second launch.
 //
 // Masks are applied only to 16-key blocks that reach past some row's limits.  There, values of keys that no row of
-// the item sees are set to zero (0 x NaN), and a value that is not finite at a key that only some rows see makes the
-// segment's rows be done again, one by one (paged_slow_row).
+// the item sees are set to zero (0 x NaN), and so is a value that is not finite at a key that only some rows see; the rows
+// that see it get it added in the end (paged_repair).
 #include "paged_attn.cuh"
 
 namespace rdkv {
@@ -94,10 +94,10 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
   __shared__ __align__(8) uint64_t s_bar[2 * DEC_STAGES];   // [slot] tile arrived, [DEC_STAGES + slot] slot free
   __shared__ int2 s_info[DEC_STAGES];                       // first key of the tile, a bit per 16 keys whose page is there
   __shared__ float2 s_ml[DEC_WARPS][DEC_ROWS];
-  __shared__ int s_again[2];                                // segment (its number + 1) whose rows are done again
+  __shared__ int s_again[2];                                // segment (its number + 1) whose rows are repaired
   __shared__ int s_trouble;
   __shared__ PagedPlaceScratch s_place;
-  __shared__ __align__(16) float s_rec[CLUSTER ? DEC_ROWS : 1][RDKV_PARTIAL_STRIDE];   // this CTA's records (m in base 2; word 2 of the first: done again)
+  __shared__ __align__(16) float s_rec[CLUSTER ? DEC_ROWS : 1][RDKV_PARTIAL_STRIDE];   // this CTA's records (m in base 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
   const uint32_t ring = (smem_addr(dec_raw) + 1023u) & ~1023u, bar = smem_addr(s_bar);
   unsigned char* ring_ptr = dec_raw + (ring - smem_addr(dec_raw));
@@ -302,9 +302,15 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
             const int c16 = 2 * cc + half;
             dec_ldmatrix_t(b, vb + (c16 >> 3) * DEC_PANEL + row * 128 + (((c16 & 7) ^ (row & 7)) << 4));
             if (edge) {
-              if ((some0 | some1) != 0u)
-                again |= paged_not_finite<BF16>(b[0] & some0) || paged_not_finite<BF16>(b[1] & some1) || paged_not_finite<BF16>(b[2] & some0) ||
-                         paged_not_finite<BF16>(b[3] & some1);
+              if ((some0 | some1) != 0u) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t some = e & 1 ? some1 : some0;
+                  const uint32_t x = b[e] & some, y = paged_finite<BF16>(x);
+                  again |= x != y;
+                  b[e] ^= x ^ y;
+                }
+              }
               b[0] &= live0; b[1] &= live1; b[2] &= live0; b[3] &= live1;
             }
             dec_mma<BF16>(o[2 * cc], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
@@ -342,40 +348,39 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       }
       dec_barrier();
       if (ok) {
-        if (!CLUSTER && s_again[segment & 1] == (int)segment + 1) {
-          const PagedSegment copy = s;
-          for (int row = warp; row < rows; row += DEC_WARPS) paged_slow_row<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, cta);
-        } else {
-          for (int row = warp; row < rows; row += DEC_WARPS) {   // four channels a lane
-            float M = -INFINITY, L = 0.f;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int row = warp; row < rows; row += DEC_WARPS) {   // four channels a lane
+          float M = -INFINITY, L = 0.f;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < DEC_WARPS; ++w) if (some) M = fmaxf(M, s_ml[w][row].x);
+          for (int w = 0; w < DEC_WARPS; ++w) if (some) M = fmaxf(M, s_ml[w][row].x);
 #pragma unroll
-            for (int w = 0; w < DEC_WARPS; ++w) {
-              if (!some) break;
-              const float2 ml = s_ml[w][row];
-              const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
-              const float4 x = *reinterpret_cast<const float4*>(buf + ((w * DEC_ROWS + row) * 128 + 4 * lane));
-              if (ml.x != -INFINITY || ml.y != 0.f) {        // (a warp that saw nothing of the row adds nothing)
-                L = fmaf(ml.y, f, L);
-                sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
-              }
-            }
-            if (CLUSTER) {
-              *reinterpret_cast<float4*>(&s_rec[row][4 + 4 * lane]) = sum;
-              if (lane == 0) *reinterpret_cast<float4*>(&s_rec[row][0]) = make_float4(M, L, 0.f, 0.f);
-              continue;
-            }
-            const PagedRow d = paged_row<DEC_ROWS>(A, s, row, cta);
-            if (d.rec != nullptr) {
-              *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = sum;
-              if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4((M - LIFT) * PAGED_LN2, L, 0.f, 0.f);
-            } else {
-              const float w = paged_over(L);
-              *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(sum.x * w, sum.y * w), paged_pack<BF16>(sum.z * w, sum.w * w));
+          for (int w = 0; w < DEC_WARPS; ++w) {
+            if (!some) break;
+            const float2 ml = s_ml[w][row];
+            const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
+            const float4 x = *reinterpret_cast<const float4*>(buf + ((w * DEC_ROWS + row) * 128 + 4 * lane));
+            if (ml.x != -INFINITY || ml.y != 0.f) {        // (a warp that saw nothing of the row adds nothing)
+              L = fmaf(ml.y, f, L);
+              sum.x = fmaf(x.x, f, sum.x); sum.y = fmaf(x.y, f, sum.y); sum.z = fmaf(x.z, f, sum.z); sum.w = fmaf(x.w, f, sum.w);
             }
           }
+          if (CLUSTER) {
+            *reinterpret_cast<float4*>(&s_rec[row][4 + 4 * lane]) = sum;
+            if (lane == 0) *reinterpret_cast<float4*>(&s_rec[row][0]) = make_float4(M, L, 0.f, 0.f);
+            continue;
+          }
+          const PagedRow d = paged_row<DEC_ROWS>(A, s, row, cta);
+          if (d.rec != nullptr) {
+            *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = sum;
+            if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4((M - LIFT) * PAGED_LN2, L, 0.f, 0.f);
+          } else {
+            const float w = paged_over(L);
+            *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(sum.x * w, sum.y * w), paged_pack<BF16>(sum.z * w, sum.w * w));
+          }
+        }
+        if (!CLUSTER && s_again[segment & 1] == (int)segment + 1) {
+          const PagedSegment copy = s;
+          for (int row = warp; row < rows; row += DEC_WARPS) paged_repair<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, row + 1, cta);
         }
         fence_async_smem();                                  // (the slot's next writer is a TMA copy)
         __syncwarp();
@@ -387,20 +392,15 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
         const uint32_t recs = smem_addr(s_rec), flag = smem_addr(&s_again[segment & 1]);
         __syncwarp();
         dec_cluster_sync();
-        bool redo = false;
+        bool repair = false;
         if (lane < size) {
           int x;
           asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(dec_map(flag, lane)) : "memory");
-          redo = x == (int)segment + 1;
+          repair = x == (int)segment + 1;
         }
-        redo = __any_sync(0xffffffffu, redo);
+        repair = __any_sync(0xffffffffu, repair);
         s.k0 = 0; s.k1 = s.item.n;
         for (int row = rank + warp * size; row < rows; row += DEC_WARPS * size) {
-          if (redo) {
-            const PagedSegment copy = s;
-            paged_slow_row<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, cta);
-            continue;
-          }
           const uint32_t at = recs + (uint32_t)row * RDKV_PARTIAL_STRIDE * 4u;
           float4 ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
           if (lane < size) ml = dec_remote4(dec_map(at, lane));
@@ -424,6 +424,10 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
           } else {
             const float w = paged_over(L);
             *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(sum.x * w, sum.y * w), paged_pack<BF16>(sum.z * w, sum.w * w));
+          }
+          if (repair) {
+            const PagedSegment copy = s;
+            paged_repair<BF16, DEC_KEYS, DEC_ROWS>(A, copy, row, row + 1, cta);
           }
         }
         __syncwarp();

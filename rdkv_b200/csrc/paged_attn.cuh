@@ -73,6 +73,9 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t paged_exponent_full(uint32_t x) {
   return BF16 ? (x & 0x7F807F80u) + 0x00800080u : (x & 0x7C007C00u) + 0x04000400u;
 }
+// The pair with zeros in the place of what is not finite.
+template <bool BF16>
+__device__ __forceinline__ uint32_t paged_finite(uint32_t x) { return x & ~((paged_exponent_full<BF16>(x) >> 15 & 0x00010001u) * 0xFFFFu); }
 template <bool BF16>
 __device__ __forceinline__ bool paged_not_finite(uint32_t x) { return (paged_exponent_full<BF16>(x) & 0x80008000u) != 0u; }
 
@@ -338,43 +341,67 @@ __device__ __forceinline__ PagedRow paged_row(const PagedArgs& A, const PagedSeg
 // 1 / l, or zero for a row that saw nothing (NaN stays NaN).
 __device__ __forceinline__ float paged_over(float l) { return l == 0.f ? 0.f : __fdividef(1.f, l); }
 
-// One row of a segment, by one warp in 32 bits, a key after the other: for rows whose tile holds values that are not
-// finite at keys that some of its rows see and others do not (a product with a zero weight would carry them over).
+// What values that are not finite add to rows [row0, row1) of a segment, whose results this warp has written.  A weight of zero times such a
+// value is NaN, so the products take zero for it at keys that some rows of the item see and others do not.  Here every row that sees
+// such a key gets the values themselves added, whose weight is positive: infinities and NaN stay what they are whatever it is.  These
+// keys lie in front of the last row and behind the first, or at the window's end: fewer than two of them a new token of the
+// item, however long the context, so that the other warps, which wait meanwhile, do so for microseconds.
 template <bool BF16, int KEYS, int ROWS>
-__device__ __noinline__ void paged_slow_row(const PagedArgs& A, const PagedSegment& s, int row, int cta) {
-  const int lane = threadIdx.x & 31, tok = row / A.g, hq = s.head * A.g + (row - tok * A.g);
-  const int pos = s.item.p0 + tok;
-  const uint2 qw = *reinterpret_cast<const uint2*>(A.q + (int64_t)(s.item.tok0 + tok) * A.q_tok + (int64_t)hq * A.q_head + 4 * lane);
-  const float q[4] = {paged_up<BF16>(qw.x & 0xFFFF), paged_up<BF16>(qw.x >> 16), paged_up<BF16>(qw.y & 0xFFFF), paged_up<BF16>(qw.y >> 16)};
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = s.k0; k < s.k1; ++k) {
-    const int key0 = paged_tile(s.item, k) * KEYS;
-    for (int key = key0; key < min(key0 + KEYS, s.item.hi); ++key) {
-      if (key > pos || (A.window > 0 && key <= pos - A.window && key >= A.sinks)) continue;
-      const int id = A.table[s.i * A.table_stride + (key >> A.page_log2)];
-      if (id < 0 || id >= A.n_pages) continue;
-      const int64_t r = key & (A.page - 1);
-      const uint2 kw = *reinterpret_cast<const uint2*>(A.k + id * A.k_page + s.head * A.k_head + r * A.k_row + 4 * lane);
-      const uint2 vw = *reinterpret_cast<const uint2*>(A.v + id * A.v_page + s.head * A.v_head + r * A.v_row + 4 * lane);
-      float x = q[0] * paged_up<BF16>(kw.x & 0xFFFF);
-      x = fmaf(q[1], paged_up<BF16>(kw.x >> 16), x); x = fmaf(q[2], paged_up<BF16>(kw.y & 0xFFFF), x);
-      x = fmaf(q[3], paged_up<BF16>(kw.y >> 16), x);
-      x = warp_sum(x) * A.scale_log2;
-      const float n = fmaxf(m, x), base = n == -INFINITY ? 0.f : n;
-      const float a = exp2_approx(m - base), p = exp2_approx(x - base);   // (m = -inf: 0)
-      l = fmaf(l, a, p);
-      o[0] = fmaf(o[0], a, p * paged_up<BF16>(vw.x & 0xFFFF)); o[1] = fmaf(o[1], a, p * paged_up<BF16>(vw.x >> 16));
-      o[2] = fmaf(o[2], a, p * paged_up<BF16>(vw.y & 0xFFFF)); o[3] = fmaf(o[3], a, p * paged_up<BF16>(vw.y >> 16));
-      m = n;
+__device__ __noinline__ void paged_repair(const PagedArgs& A, const PagedSegment& s, int row0, int row1, int cta) {
+  const int lane = threadIdx.x & 31, p_first = s.item.p0, p_last = s.item.p0 + s.item.n_tok - 1;
+  const int d0 = max(p_first + 1, 0), n1 = max(s.item.hi - d0, 0);
+  const int w0 = max(max(p_first - A.window + 1, A.sinks), 0);
+  const int n = n1 + (A.window > 0 ? max(min(min(p_last - A.window, p_first), s.item.hi - 1) + 1 - w0, 0) : 0);   // (up to 510: a group has 256 tokens at most)
+  auto key_of = [&](int x) { return x < n1 ? d0 + x : w0 + x - n1; };
+  auto value = [&](int key) {                                // four channels a lane; zeros where the segment has not the key
+    const int t = key / KEYS, k = t < s.item.t_sink ? t : t >= s.item.t_lo ? t - s.item.t_lo + s.item.t_sink : -1;
+    if (k < s.k0 || k >= s.k1) return make_uint2(0u, 0u);
+    const int id = A.table[s.i * A.table_stride + (key >> A.page_log2)];
+    if (id < 0 || id >= A.n_pages) return make_uint2(0u, 0u);
+    return *reinterpret_cast<const uint2*>(A.v + id * A.v_page + s.head * A.v_head + (int64_t)(key & (A.page - 1)) * A.v_row + 4 * lane);
+  };
+  uint32_t found = 0u;                                       // lane w: a bit for each of keys 32 w ... that has such a value
+  for (int x0 = 0; x0 < n; x0 += 8) {
+    uint2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x0 + i < n ? value(key_of(x0 + i)) : make_uint2(0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool bad = __any_sync(0xffffffffu, paged_not_finite<BF16>(v[i].x) || paged_not_finite<BF16>(v[i].y));
+      if (bad && lane == x0 >> 5) found |= 1u << ((x0 + i) & 31);
     }
   }
-  const PagedRow d = paged_row<ROWS>(A, s, row, cta);
-  if (d.rec != nullptr) {
-    *reinterpret_cast<float4*>(d.rec + 4 + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
-    if (lane == 0) *reinterpret_cast<float4*>(d.rec) = make_float4(m * PAGED_LN2, l, 0.f, 0.f);
-  } else {
-    const float w = paged_over(l);
-    *reinterpret_cast<uint2*>(d.out + 4 * lane) = make_uint2(paged_pack<BF16>(o[0] * w, o[1] * w), paged_pack<BF16>(o[2] * w, o[3] * w));
+  __syncwarp();
+  for (int row = row0; row < row1;) {
+    const int tok = row / A.g, end = min(row1, (tok + 1) * A.g), pos = p_first + tok;
+    float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto plus = [](float& a, float x) { a += fabsf(x) < INFINITY ? 0.f : x; };
+    for (int w = 0; 32 * w < n; ++w) {
+      uint32_t bits = __shfl_sync(0xffffffffu, found, w);
+      while (bits != 0u) {
+        const int key = key_of(32 * w + __ffs(bits) - 1);
+        bits &= bits - 1;
+        if (key > pos || (A.window > 0 && key <= pos - A.window && key >= A.sinks)) continue;
+        const uint2 v = value(key);
+        plus(add.x, paged_up<BF16>(v.x & 0xFFFF)); plus(add.y, paged_up<BF16>(v.x >> 16));
+        plus(add.z, paged_up<BF16>(v.y & 0xFFFF)); plus(add.w, paged_up<BF16>(v.y >> 16));
+      }
+    }
+    const bool mine = add.x != 0.f || add.y != 0.f || add.z != 0.f || add.w != 0.f;
+    for (; row < end; ++row) {
+      if (!mine) continue;
+      const PagedRow d = paged_row<ROWS>(A, s, row, cta);
+      if (d.rec != nullptr) {
+        float4* at = reinterpret_cast<float4*>(d.rec + 4 + 4 * lane);
+        const float4 o = *at;
+        *at = make_float4(o.x + add.x, o.y + add.y, o.z + add.z, o.w + add.w);
+      } else {
+        uint2* at = reinterpret_cast<uint2*>(d.out + 4 * lane);
+        const uint2 o = *at;
+        *at = make_uint2(paged_pack<BF16>(paged_up<BF16>(o.x & 0xFFFF) + add.x, paged_up<BF16>(o.x >> 16) + add.y),
+                         paged_pack<BF16>(paged_up<BF16>(o.y & 0xFFFF) + add.z, paged_up<BF16>(o.y >> 16) + add.w));
+      }
+    }
   }
 }
 

@@ -11,8 +11,8 @@
 // 12 warps: two warpgroups of softmax (half 0, half 1), and one of helpers: one warp works out the segments and brings in Q and the tiles (tiled TMA, one box
 // per page and 64-channel panel, 128-byte swizzle, four slots of 32 KB for K and V in turn), two issue the products of a
 // half each, one looks after masked values: 0 x NaN is NaN, so in tiles that some row of the item does not see whole it
-// sets values of keys that no row sees to zero before the product, and looks for values that are not finite among the
-// others; such a segment's rows are done again one by one (paged_slow_row).
+// sets values of keys that no row sees to zero before the product, and values that are not finite where only some rows
+// see their key; the rows that do get them added in the end (paged_repair).
 //
 // An accumulator is rescaled by the threads that own its rows, and only when a score passes the row's reference by more
 // than PagedWeights::RAISE.  Every wait is bounded; a wait that runs out ends the CTA's work and sets its status word.
@@ -336,7 +336,24 @@ __device__ void chunk_values(const PagedArgs& A, unsigned char* ring_ptr, uint32
           }
           const bool again = paged_not_finite<BF16>(sum[0]) || paged_not_finite<BF16>(sum[1]) || paged_not_finite<BF16>(sum[2]) ||
                              paged_not_finite<BF16>(sum[3]);
-          if (again) s_again[segments & 3] = (int)segments + 1;
+          if (__any_sync(0xffffffffu, again)) {
+            if (lane == 0) s_again[segments & 3] = (int)segments + 1;
+            for (int g = 0; g < 8; ++g) {
+              uint4* at = reinterpret_cast<uint4*>(ring_ptr + slot * CH_SLOT + (16 * g + (lane >> 3)) * 128 + (lane & 7) * 16);
+              const int mine = info.key0 + 16 * g + (lane >> 3);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int key = mine + 4 * i;
+                if (key <= p_first && !(WINDOW && key >= A.sinks && key <= p_last - A.window)) continue;   // (all rows see it)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                  uint4 x = at[i * 32 + p * (CH_PANEL / 16)];
+                  x.x = paged_finite<BF16>(x.x); x.y = paged_finite<BF16>(x.y); x.z = paged_finite<BF16>(x.z); x.w = paged_finite<BF16>(x.w);
+                  at[i * 32 + p * (CH_PANEL / 16)] = x;
+                }
+              }
+            }
+          }
           fence_async_smem();                                // (the product reads the zeros)
           __syncwarp();
           if (lane == 0) bar_arrive(bar + 8 * (CH_V_OK + slot));
@@ -462,65 +479,66 @@ __device__ void chunk_softmax(const PagedArgs& A, uint32_t bar, uint32_t tmem, c
       if (!ok) break;
       tmem_fence_after();
     }
-    if (steps > 0 && s_again[segments & 3] == (int)segments + 1) {
-      const PagedSegment copy = s;
-      for (int r = 0; r < 32; ++r)
-        if (__shfl_sync(0xffffffffu, live ? 1 : 0, r) != 0) paged_slow_row<BF16, CH_KEYS, CH_ROWS>(A, copy, item_row - lane + r, cta);
-    } else {
-      // a row a thread in tensor memory, a row eight lanes on the way out: 128 bytes of every row pass through shared memory, their
-      // 16-byte chunks swapped about by row (32 rows of 16 bytes each would be 32 lines an instruction)
-      const bool whole = s.k0 == 0 && s.k1 == s.item.n, records = A.rec != nullptr || !whole;
-      const float w = steps == 0 ? 0.f : records ? 1.f : paged_over(l);
-      const int64_t at_tok = s.item.tok0 + h * tm + tok, at_head = s.head * A.g + row - tok * A.g;
-      uint64_t to = 0ull;
-      if (live) {
-        if (records) {
-          float* rec = whole ? A.rec + (at_tok * A.H_q + at_head) * RDKV_PARTIAL_STRIDE
-                             : A.part + ((int64_t)(2 * cta + (s.k0 > 0 ? 0 : 1)) * CH_ROWS + item_row) * RDKV_PARTIAL_STRIDE;
-          *reinterpret_cast<float4*>(rec) = make_float4((m - LIFT) * PAGED_LN2, l, 0.f, 0.f);
-          to = reinterpret_cast<uint64_t>(rec + 4);
-        } else {
-          to = reinterpret_cast<uint64_t>(A.out + at_tok * A.o_tok + at_head * A.o_head);
-        }
+    // (a flag for a tile behind this half's last may be up already or not: none of its rows sees a key there, so nothing is added)
+    const bool repair = steps > 0 && s_again[segments & 3] == (int)segments + 1;
+    // a row a thread in tensor memory, a row eight lanes on the way out: 128 bytes of every row pass through shared memory, their
+    // 16-byte chunks swapped about by row (32 rows of 16 bytes each would be 32 lines an instruction)
+    const bool whole = s.k0 == 0 && s.k1 == s.item.n, records = A.rec != nullptr || !whole;
+    const float w = steps == 0 ? 0.f : records ? 1.f : paged_over(l);
+    const int64_t at_tok = s.item.tok0 + h * tm + tok, at_head = s.head * A.g + row - tok * A.g;
+    uint64_t to = 0ull;
+    if (live) {
+      if (records) {
+        float* rec = whole ? A.rec + (at_tok * A.H_q + at_head) * RDKV_PARTIAL_STRIDE
+                           : A.part + ((int64_t)(2 * cta + (s.k0 > 0 ? 0 : 1)) * CH_ROWS + item_row) * RDKV_PARTIAL_STRIDE;
+        *reinterpret_cast<float4*>(rec) = make_float4((m - LIFT) * PAGED_LN2, l, 0.f, 0.f);
+        to = reinterpret_cast<uint64_t>(rec + 4);
+      } else {
+        to = reinterpret_cast<uint64_t>(A.out + at_tok * A.o_tok + at_head * A.o_head);
       }
-      uint4* mine = reinterpret_cast<uint4*>(stage) + lane * 8;
+    }
+    uint4* mine = reinterpret_cast<uint4*>(stage) + lane * 8;
 #pragma unroll 1
-      for (int c = 0; c < (records ? 4 : 2); ++c) {
-        uint4 y[8];
+    for (int c = 0; c < (records ? 4 : 2); ++c) {
+      uint4 y[8];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (records && e == 1) break;
-          uint32_t x[32];
-          if (steps > 0) tmem_ld32(t_o + (records ? 32 * c : 64 * c + 32 * e), x);
-          else
+      for (int e = 0; e < 2; ++e) {
+        if (records && e == 1) break;
+        uint32_t x[32];
+        if (steps > 0) tmem_ld32(t_o + (records ? 32 * c : 64 * c + 32 * e), x);
+        else
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = 0u;          // (no step wrote the accumulator)
-          if (records) {
+          for (int i = 0; i < 32; ++i) x[i] = 0u;          // (no step wrote the accumulator)
+        if (records) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          } else {
+          for (int i = 0; i < 8; ++i) y[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              auto two16 = [&](int k) { return paged_pack<BF16>(__uint_as_float(x[8 * i + k]) * w, __uint_as_float(x[8 * i + k + 1]) * w); };
-              y[4 * e + i] = make_uint4(two16(0), two16(2), two16(4), two16(6));
-            }
+          for (int i = 0; i < 4; ++i) {
+            auto two16 = [&](int k) { return paged_pack<BF16>(__uint_as_float(x[8 * i + k]) * w, __uint_as_float(x[8 * i + k + 1]) * w); };
+            y[4 * e + i] = make_uint4(two16(0), two16(2), two16(4), two16(6));
           }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine[i ^ (lane & 7)] = y[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {                        // four rows at a time
-          const int r = 4 * i + (lane >> 3);
-          y[i] = reinterpret_cast<const uint4*>(stage)[r * 8 + ((lane & 7) ^ (r & 7))];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint64_t at = __shfl_sync(0xffffffffu, to, 4 * i + (lane >> 3));
-          if (at != 0ull) store_global(at + 128 * c + 16 * (lane & 7), y[i]);
-        }
-        __syncwarp();
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[i ^ (lane & 7)] = y[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {                        // four rows at a time
+        const int r = 4 * i + (lane >> 3);
+        y[i] = reinterpret_cast<const uint4*>(stage)[r * 8 + ((lane & 7) ^ (r & 7))];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t at = __shfl_sync(0xffffffffu, to, 4 * i + (lane >> 3));
+        if (at != 0ull) store_global(at + 128 * c + 16 * (lane & 7), y[i]);
+      }
+      __syncwarp();
+    }
+    if (repair) {
+      const PagedSegment copy = s;
+      const int row0 = h * tm * A.g + quad * 32, row1 = min(row0 + 32, (h * tm + n_tok) * A.g);
+      paged_repair<BF16, CH_KEYS, CH_ROWS>(A, copy, row0, row1, cta);
     }
     tmem_fence_before();
     tile += n;
@@ -539,7 +557,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
   __shared__ PagedPlaceScratch s_place;
   __shared__ uint32_t s_tmem;
   __shared__ ChunkWork<WINDOW> s_work[CH_WORKS];
-  __shared__ int s_again[4];                                 // segment (its number + 1) whose rows are done again
+  __shared__ int s_again[4];                                 // segment (its number + 1) whose rows are repaired
   __shared__ int s_trouble;
   const int tid = threadIdx.x, warp = tid >> 5, cta = blockIdx.x;
   const uint32_t q32 = smem_addr(ch_raw), ring = q32 + 2 * CH_SLOT, bar = smem_addr(s_bar);

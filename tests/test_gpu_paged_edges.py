@@ -106,3 +106,92 @@ def test_starts_that_fall_leave_zeros_in_a_result_of_the_call(S, H_kv, max_new):
         del held                                                        # (the allocator hands out this memory next)
         out = paged_attention(q, k, v, table, ints(start), ints([40] * S), max_new=max_new)
         assert (out == 0).all()
+
+
+# ── values that are not finite ───────────────────────────────────────────────
+
+def bits(x):
+    return x.contiguous().view(torch.int16)
+
+
+def spoil(k, v, table, lens, at, seed, dtype):
+    """A copy of v with NaN and infinities in some channels of the tokens ``at`` = [(request, token)], and where they are."""
+    rng = random.Random(seed)
+    v, where = v.clone(), []
+    page = k.shape[2]
+    for i, s in at:
+        for h in range(k.shape[1]):
+            channels = rng.sample(range(128), rng.choice([1, 1, 3, 128]))
+            kind = torch.tensor([rng.choice([float("nan"), float("inf"), -float("inf")]) for _ in channels], dtype=dtype, device="cuda")
+            v[table[i, s // page], h, s % page, channels] = kind
+            where.append((i, s, h, channels))
+    return v, where
+
+
+def touched(T, H_q, H_kv, start, lens, where, window, sinks):
+    """Which results see one of these values."""
+    out = torch.zeros(T, H_q, 128, dtype=torch.bool)
+    g = H_q // H_kv
+    for i, s, h, channels in where:
+        p = torch.arange(start[i], start[i + 1]) + lens[i] - start[i + 1]
+        sees = (s <= p) & ((s > p - window) if window > 0 and s >= sinks else torch.ones_like(p, dtype=torch.bool))
+        for c in channels:
+            out[start[i]:start[i + 1], h * g:(h + 1) * g, c] |= sees[:, None]
+    return out.cuda()
+
+
+def spoiled(lens, new, H_kv, g, page, dtype, at, seed=0, window=0, sinks=0, max_new=None):
+    """Results that see such a value are not finite, all others are those of the same call with clean values, bit for bit;
+    and so in records."""
+    from rdkv_b200.paged import paged_attention
+    k, v, table = R.build_cache(lens, H_kv, page, dtype, seed=seed)
+    T, H_q = sum(new), H_kv * g
+    q = randn(T, H_q, 128, seed=seed + 1, dtype=dtype)
+    args = (table, starts(new), ints(lens))
+    kw = dict(max_new=max(new) if max_new is None else max_new, window=window, sinks=sinks, check_status=True)
+    bad, where = spoil(k, v, table, lens, at, seed, dtype)
+    seen = touched(T, H_q, H_kv, starts(new).tolist(), lens, where, window, sinks)
+    clean = paged_attention(q, k, v, *args, **kw)
+    check(clean, R.attention(q, k, v, *args, window, sinks))
+    got = paged_attention(q, k, bad, *args, **kw)
+    assert not torch.isfinite(got[seen]).any()
+    assert torch.equal(bits(got[~seen]), bits(clean[~seen]))
+    recs = [torch.zeros(T * H_q, 132, device="cuda") for _ in range(2)]
+    for x, r in zip((v, bad), recs):
+        paged_attention(q, k, x, *args, out_partial=r, **kw)
+    assert torch.equal(recs[0][:, :2], recs[1][:, :2])
+    o, o_bad = (r[:, 4:].reshape(T, H_q, 128) for r in recs)
+    assert not torch.isfinite(o_bad[seen]).any() and torch.equal(o_bad[~seen], o[~seen])
+    return q, k, bad, args, kw, got
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("g", [1, 4, 5])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (3, 2), (40, 20), (150, 70), (300, 0)])
+@pytest.mark.parametrize("new", [[3, 2, 1], [260, 130, 1]])
+def test_bad_values_reach_the_results_that_see_them(dtype, g, window, sinks, new):
+    """In the chunk, at either end of the window, at the last sink, in front of everything, at a page's first and last row."""
+    lens = [700, 333, 64]
+    at = [(0, s) for s in (0, 1, 19, 20, 69, 70, 300, 399, 400, 438, 439, 440, 441, 511, 512, 550, 600, 697, 698, 699)]
+    at += [(1, s) for s in (2, 31, 200, 203, 300, 331, 332)] + [(2, 62), (2, 63)]
+    spoiled(lens, new, 2, g, 32, dtype, at, seed=g + window, window=window, sinks=sinks)
+    spoiled(lens, new, 2, g, 32, dtype, [(0, sum(lens) % 97 + 600)], seed=g, window=window, sinks=sinks)
+    spoiled([5 * n for n in new], new, 1, g, 16, dtype, [(0, 4 * new[0] + 1), (1, 5 * new[1] - 1)], seed=g, window=window, sinks=sinks)   # (clusters)
+
+
+@pytest.mark.parametrize("new,max_new", [([700, 700, 690], 700), ([16] * 9, 16), ([4] * 60, 4)])
+def test_bad_values_behind_a_long_context_among_other_requests(new, max_new):
+    """One bad value in the first request's chunk behind 20000 tokens, CTAs with several segments: the others' results are
+    there, and no wait runs out (check_status)."""
+    lens = [20000 + n for n in new[:1]] + [3000 + 400 * (i % 5) + n for i, n in enumerate(new[1:])]
+    spoiled(lens, new, 2, 4, 64, BF16, [(0, 20000 + new[0] // 2)], seed=5, max_new=max_new)
+
+
+def test_results_repeat_with_bad_values():
+    """A value in a tile that only the second half of an item sees: the first half's results are the same every time."""
+    from rdkv_b200.paged import paged_attention
+    lens, new = [992 + 64, 608 + 64], [64, 64]               # (4 query heads: an item is two halves of 32 tokens; tiles of 128 keys)
+    for at in ([(0, 1024 + 20)], [(0, 1024 + 31), (1, 640 + 5)]):
+        q, k, bad, args, kw, got = spoiled(lens, new, 2, 4, 32, F16, at, seed=17)
+        for _ in range(30):
+            assert torch.equal(bits(paged_attention(q, k, bad, *args, **kw)), bits(got))

@@ -215,7 +215,6 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       float o[16][4];
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      bool again = false;
       for (int k = s.k0; k < s.k1; ++k, ++count) {
         const int slot = count % DEC_STAGES;
         ok = bar_wait_warp(bar + 8 * slot, (count / DEC_STAGES) & 1);
@@ -223,6 +222,24 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
         const int2 info = s_info[slot];
         const int key0 = info.x + warp * 16;
         if ((info.y >> warp & 1) != 0 && key0 < s.item.hi) {
+          const bool edge = key0 + 15 > p_first || key0 + 16 > s.item.hi ||
+                            (A.window > 0 && key0 <= p_last - A.window && key0 + 15 >= A.sinks);
+          if (edge && s.item.n_tok > 1) {
+            // values of keys that some rows see and others do not: two lanes a key, a panel each
+            const int at_key = lane >> 1, key = key0 + at_key;
+            const bool low = A.window > 0 && key >= A.sinks;
+            if (key < s.item.hi && !(low && key <= p_first - A.window) && (key > p_first || (low && key <= p_last - A.window))) {
+              uint4* at = reinterpret_cast<uint4*>(ring_ptr + slot * DEC_STAGE + (2 + (lane & 1)) * DEC_PANEL + (warp * 16 + at_key) * 128);
+#pragma unroll 1
+              for (int i = 0; i < 8; ++i) {                  // (in an order that keeps the keys' banks apart)
+                const uint4 x = at[i ^ (at_key & 7)];
+                const uint4 y = {paged_finite<BF16>(x.x), paged_finite<BF16>(x.y), paged_finite<BF16>(x.z), paged_finite<BF16>(x.w)};
+                if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) { at[i ^ (at_key & 7)] = y; s_again[segment & 1] = (int)segment + 1; }
+              }
+            }
+            fence_async_smem();                              // (the slot's next writer is a TMA copy)
+            __syncwarp();
+          }
           const uint32_t kb = ring + slot * DEC_STAGE, vb = kb + 2 * DEC_PANEL;
           // scores of 16 keys: two tiles of 8
           float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -238,9 +255,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
               dec_mma<BF16>(sc[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2], b[3]);
             }
           }
-          const bool edge = key0 + 15 > p_first || key0 + 16 > s.item.hi ||
-                            (A.window > 0 && key0 <= p_last - A.window && key0 + 15 >= A.sinks);
-          uint32_t live0 = 0xFFFFFFFFu, live1 = 0xFFFFFFFFu, some0 = 0u, some1 = 0u;   // this thread's keys of the V operand
+          uint32_t live0 = 0xFFFFFFFFu, live1 = 0xFFFFFFFFu;   // this thread's keys of the V operand
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -248,7 +263,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
           if (edge) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              uint32_t live = 0xFFFFFFFFu, some = 0u;
+              uint32_t live = 0xFFFFFFFFu;
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int key = key0 + 8 * n + c2 + e;
@@ -259,11 +274,9 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
                 }
                 const bool low = A.window > 0 && key >= A.sinks;
                 const bool none = key >= s.item.hi || (low && key <= p_first - A.window);       // no row sees the key
-                const bool not_all = key > p_first || (low && key <= p_last - A.window);
                 if (none) live &= e == 0 ? 0xFFFF0000u : 0x0000FFFFu;
-                else if (not_all) some |= e == 0 ? 0x0000FFFFu : 0xFFFF0000u;
               }
-              if (n == 0) { live0 = live; some0 = some; } else { live1 = live; some1 = some; }
+              if (n == 0) live0 = live; else live1 = live;
             }
           }
           float top[2];
@@ -301,18 +314,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
             uint32_t b[4];
             const int c16 = 2 * cc + half;
             dec_ldmatrix_t(b, vb + (c16 >> 3) * DEC_PANEL + row * 128 + (((c16 & 7) ^ (row & 7)) << 4));
-            if (edge) {
-              if ((some0 | some1) != 0u) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint32_t some = e & 1 ? some1 : some0;
-                  const uint32_t x = b[e] & some, y = paged_finite<BF16>(x);
-                  again |= x != y;
-                  b[e] ^= x ^ y;
-                }
-              }
-              b[0] &= live0; b[1] &= live1; b[2] &= live0; b[3] &= live1;
-            }
+            if (edge) { b[0] &= live0; b[1] &= live1; b[2] &= live0; b[3] &= live1; }
             dec_mma<BF16>(o[2 * cc], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
             dec_mma<BF16>(o[2 * cc + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
           }
@@ -328,7 +330,6 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       }
-      if (again) s_again[segment & 1] = (int)segment + 1;
       ok = !dec_barrier_any(!ok);                            // (all four warps go on, or none does)
       if (!ok) s_trouble = 1;
       const int slot = (count + DEC_STAGES - 1) % DEC_STAGES;   // (without tiles of its own, a CTA of a cluster has only empty records)

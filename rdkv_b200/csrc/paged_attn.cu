@@ -171,10 +171,9 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       }
       if (CLUSTER) { __syncwarp(); dec_cluster_sync(); dec_cluster_sync(); }
     }
-    if (!ok) {                                               // wait (again bounded) for the copies in flight
-      s_trouble = 1;
-      for (unsigned n = count < DEC_STAGES ? 0 : count - DEC_STAGES; n < count; ++n) bar_wait(bar + 8 * (n % DEC_STAGES), (n / DEC_STAGES) & 1);
-    }
+    if (!ok) s_trouble = 1;
+    // copies that are still on their way when nobody waits for them any more must not land in the shared memory of the next CTA
+    for (unsigned n = count < DEC_STAGES ? 0 : count - DEC_STAGES; n < count; ++n) bar_wait(bar + 8 * (n % DEC_STAGES), (n / DEC_STAGES) & 1);
   } else {
     // ── the computing warps ──
     constexpr float RAISE = PagedWeights<BF16>::RAISE, LIFT = PagedWeights<BF16>::LIFT;

@@ -45,7 +45,7 @@ static_assert(CH_SOFTMAX_WARPS * 32 * CH_SOFTMAX_REGS + 128 * CH_HELPER_REGS <= 
               "the split draws on what the block was launched with");
 
 // Barriers: Q arrived / free; [2 half + buffer] scores done, weights written, product with the values done; [slot] tile arrived / free,
-// values looked after; [half] products ended early; [segment's place] its description written / no longer needed.
+// values looked after; [half] products at an end; [segment's place] its description written / no longer needed.
 enum { CH_Q_FULL = 0, CH_Q_FREE = 1, CH_S_FULL = 2, CH_P_READY = 6, CH_O_DONE = 10, CH_FULL = 14, CH_FREE = CH_FULL + CH_SLOTS,
        CH_V_OK = CH_FREE + CH_SLOTS, CH_DRAINED = CH_V_OK + CH_SLOTS, CH_W_FULL = CH_DRAINED + 2, CH_W_FREE = CH_W_FULL + CH_WORKS,
        CH_BARS = CH_W_FREE + CH_WORKS };
@@ -201,11 +201,10 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
     }
   }
   if (ok) { s.k0 = s.k1 = -1; s.item.n_tok = 0; publish(); }
-  if (!ok) {                                                 // wait (again bounded) for the copies in flight
-    *s_trouble = 1;
-    for (unsigned n = use < CH_SLOTS ? 0 : use - CH_SLOTS; n < use; ++n) bar_wait(bar + 8 * (CH_FULL + n % CH_SLOTS), (n / CH_SLOTS) & 1);
-    if (segments > 0) bar_wait(bar + 8 * CH_Q_FULL, (segments - 1) & 1);
-  }
+  if (!ok) *s_trouble = 1;
+  // copies that are still on their way when nobody waits for them any more must not land in the shared memory of the next CTA
+  for (unsigned n = use < CH_SLOTS ? 0 : use - CH_SLOTS; n < use; ++n) bar_wait(bar + 8 * (CH_FULL + n % CH_SLOTS), (n / CH_SLOTS) & 1);
+  if (segments > 0) bar_wait(bar + 8 * CH_Q_FULL, (segments - 1) & 1);
 }
 
 __device__ __forceinline__ int chunk_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
@@ -283,11 +282,10 @@ __device__ void chunk_products(int h, uint32_t q32, uint32_t ring, uint32_t bar,
     }
     tile += n;
   }
-  if (!ok) {                                                 // wait (again bounded) for the products in flight
-    *s_trouble = 1;
-    mma_commit(one, bar + 8 * (CH_DRAINED + h));
-    bar_wait_warp(bar + 8 * (CH_DRAINED + h), 0);
-  }
+  if (!ok) *s_trouble = 1;
+  // products that are still under way (the softmax warps may have given up) must not outlive the tensor memory
+  mma_commit(one, bar + 8 * (CH_DRAINED + h));
+  bar_wait_warp(bar + 8 * (CH_DRAINED + h), 0);
 }
 
 // One warp: values in masked places.

@@ -667,6 +667,7 @@ typedef struct {
   int64_t table_stride;
   int32_t dtype, n_tokens, H_q, H_kv, n_pages, page_size, width, n_requests, max_new, window, sinks;
   float scale;
+  int32_t wait_us;    /* how long a device-side wait may take (up to 4000000); 0: two seconds, negative: no time (tests) */
 } rdkv_paged_attention_args;
 int rdkv_sizeof_paged_attention_args(void);
 int rdkv_paged_attention_status_words(void);

@@ -126,7 +126,8 @@ class PagedAttentionArgs(C.Structure):
     """Mirror of ``rdkv_paged_attention_args``; field order and types must match the header."""
     _fields_ = _fields((C.c_int64, "q_tok_stride q_head_stride k_page_stride k_head_stride k_row_stride v_page_stride v_head_stride "
                                    "v_row_stride table_stride"),
-                       (C.c_int32, "dtype n_tokens H_q H_kv n_pages page_size width n_requests max_new window sinks"), (C.c_float, "scale"))
+                       (C.c_int32, "dtype n_tokens H_q H_kv n_pages page_size width n_requests max_new window sinks"), (C.c_float, "scale"),
+                       (C.c_int32, "wait_us"))
 
 
 _i, _i64, _p, _f = C.c_int, C.c_int64, C.c_void_p, C.c_float

@@ -151,7 +151,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
           ids_next = page_of(k + batch);
         }
         const int slot = count % DEC_STAGES;
-        if (count >= DEC_STAGES && !bar_wait_warp(bar + 8 * (DEC_STAGES + slot), (count / DEC_STAGES - 1) & 1)) { ok = false; break; }
+        if (count >= DEC_STAGES && !bar_wait_warp(bar + 8 * (DEC_STAGES + slot), (count / DEC_STAGES - 1) & 1, A.wait_ns)) { ok = false; break; }
         const int key0 = paged_tile(s.item, k) * DEC_KEYS;
         const int id = __shfl_sync(0xffffffffu, ids, in_batch * per_tile + (box < per_tile ? box : 0));
         const bool there = box < per_tile && id >= 0 && id < A.n_pages;
@@ -173,7 +173,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
     }
     if (!ok) s_trouble = 1;
     // copies that are still on their way when nobody waits for them any more must not land in the shared memory of the next CTA
-    for (unsigned n = count < DEC_STAGES ? 0 : count - DEC_STAGES; n < count; ++n) bar_wait(bar + 8 * (n % DEC_STAGES), (n / DEC_STAGES) & 1);
+    for (unsigned n = count < DEC_STAGES ? 0 : count - DEC_STAGES; n < count; ++n) bar_wait(bar + 8 * (n % DEC_STAGES), (n / DEC_STAGES) & 1, WAIT_NS);
   } else {
     // ── the computing warps ──
     constexpr float RAISE = PagedWeights<BF16>::RAISE, LIFT = PagedWeights<BF16>::LIFT;
@@ -216,7 +216,7 @@ paged_decode_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_k,
       for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       for (int k = s.k0; k < s.k1; ++k, ++count) {
         const int slot = count % DEC_STAGES;
-        ok = bar_wait_warp(bar + 8 * slot, (count / DEC_STAGES) & 1);
+        ok = bar_wait_warp(bar + 8 * slot, (count / DEC_STAGES) & 1, A.wait_ns);
         if (!ok) break;
         const int2 info = s_info[slot];
         const int key0 = info.x + warp * 16;
@@ -552,6 +552,7 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
   A.cap = (int)std::min<int64_t>((int64_t)g.width * g.page_size, 0x7fff0000);
   A.q_start = q_start; A.kv_lens = kv_lens; A.S = g.n_requests; A.T = g.n_tokens;
   A.window = std::min(g.window, 1 << 30); A.sinks = std::min(g.sinks, 1 << 30); A.scale_log2 = g.scale * PAGED_LOG2E;
+  A.wait_ns = g.wait_us == 0 ? WAIT_NS : (uint32_t)std::min(std::max(g.wait_us, 0), 4000000) * 1000u;
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
   const bool bf = g.dtype == RDKV_BF16, few = paged_few_rows(g.n_requests, g.H_kv, g.max_new, A.g);
   A.group = few ? PAGED_DECODE_ROWS / A.g : 2 * (128 / A.g);

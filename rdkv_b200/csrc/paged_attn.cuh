@@ -39,6 +39,7 @@ struct PagedArgs {
   float scale_log2;                               // scale * log2 e: scores are kept in base 2
   uint16_t* out; int64_t o_tok, o_head; int zero_pad;
   float* rec;                                     // [T][H_q][132] instead of out
+  uint32_t wait_ns;                               // how long a wait may take
   // workspace
   int4* place;                                    // [G+1][2] where CTA c starts: request, head, group, tile; the item's tiles, rows, first query row
   int* status;                                    // [G] bits: 1 a wait of the CTA ran out, 2 q_start falls

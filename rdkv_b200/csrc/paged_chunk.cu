@@ -120,9 +120,14 @@ struct ChunkSteps {
 template <bool WINDOW>
 struct ChunkWork { PagedSegment s; ChunkSteps<WINDOW> st[2]; };   // s.k0 < 0: there are no more
 
+// Waits for the description of segment `at`; false if there is none, or (not ok) the wait ran out.  A half without rows waits here while the
+// other takes the tiles of the segment before: the limit once more for every 1024 of them (2 ms for 2 us).
 template <bool WINDOW>
-__device__ __forceinline__ bool chunk_work(const ChunkWork<WINDOW>* works, unsigned at, uint32_t bar, bool& ok) {
-  ok = ok && bar_wait_warp(bar + 8 * (CH_W_FULL + at % CH_WORKS), (at / CH_WORKS) & 1);
+__device__ __forceinline__ bool chunk_work(const ChunkWork<WINDOW>* works, unsigned at, uint32_t bar, uint32_t limit, bool& ok) {
+  for (int r = 0; ok && !bar_wait_warp(bar + 8 * (CH_W_FULL + at % CH_WORKS), (at / CH_WORKS) & 1, limit); ++r) {
+    const PagedSegment& before = works[(at + CH_WORKS - 1) % CH_WORKS].s;
+    ok = at > 0 && r < __shfl_sync(0xffffffffu, before.k1 - before.k0, 0) >> 10;
+  }
   return ok && works[at % CH_WORKS].s.k0 >= 0;
 }
 __device__ __forceinline__ void chunk_work_done(unsigned at, uint32_t bar) {
@@ -141,7 +146,7 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
   bool ok = true;
   auto publish = [&]() {
     const int at = published % CH_WORKS;
-    if (published >= CH_WORKS) ok = ok && bar_wait_warp(bar + 8 * (CH_W_FREE + at), (published / CH_WORKS - 1) & 1);
+    if (published >= CH_WORKS) ok = ok && bar_wait_warp(bar + 8 * (CH_W_FREE + at), (published / CH_WORKS - 1) & 1, A.wait_ns);
     if (!ok) return;
     if (lane < 2) works[at].st[lane] = ChunkSteps<WINDOW>(A, s, lane, tm);
     if (lane == 0) works[at].s = s;
@@ -160,7 +165,7 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
     };
     int ids = page_of(s.k0), ids_next = -1;
     const int halves = s.item.n_tok > tm ? 2 : 1;
-    if (segments > 0 && !bar_wait_warp(bar + 8 * CH_Q_FREE, (segments - 1) & 1)) { ok = false; break; }
+    if (segments > 0 && !bar_wait_warp(bar + 8 * CH_Q_FREE, (segments - 1) & 1, A.wait_ns)) { ok = false; break; }
     if (lane == 0) {
       bar_arrive_tx(bar + 8 * CH_Q_FULL, (uint32_t)halves * 2u * (uint32_t)(tm * A.g) * 128u);
       for (int h = 0; h < halves; ++h)
@@ -187,7 +192,7 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
       const uint32_t bytes = (uint32_t)__popc(lanes) * (uint32_t)rows * 128u;
       for (int t = 0; t < 2; ++t, ++use) {                   // K, then V
         const int slot = use % CH_SLOTS;
-        if (use >= CH_SLOTS && !bar_wait_warp(bar + 8 * (CH_FREE + slot), (use / CH_SLOTS - 1) & 1)) { ok = false; break; }
+        if (use >= CH_SLOTS && !bar_wait_warp(bar + 8 * (CH_FREE + slot), (use / CH_SLOTS - 1) & 1, A.wait_ns)) { ok = false; break; }
         if (lane == 0) {
           if (bytes > 0) bar_arrive_tx(bar + 8 * (CH_FULL + slot), bytes);
           else bar_arrive(bar + 8 * (CH_FULL + slot));
@@ -203,15 +208,15 @@ __device__ void chunk_load(const PagedArgs& A, const CUtensorMap* tm_q, const CU
   if (ok) { s.k0 = s.k1 = -1; s.item.n_tok = 0; publish(); }
   if (!ok) *s_trouble = 1;
   // copies that are still on their way when nobody waits for them any more must not land in the shared memory of the next CTA
-  for (unsigned n = use < CH_SLOTS ? 0 : use - CH_SLOTS; n < use; ++n) bar_wait(bar + 8 * (CH_FULL + n % CH_SLOTS), (n / CH_SLOTS) & 1);
-  if (segments > 0) bar_wait(bar + 8 * CH_Q_FULL, (segments - 1) & 1);
+  for (unsigned n = use < CH_SLOTS ? 0 : use - CH_SLOTS; n < use; ++n) bar_wait(bar + 8 * (CH_FULL + n % CH_SLOTS), (n / CH_SLOTS) & 1, WAIT_NS);
+  if (segments > 0) bar_wait(bar + 8 * CH_Q_FULL, (segments - 1) & 1, WAIT_NS);
 }
 
 __device__ __forceinline__ int chunk_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // Two warps: the products of half 0, of half 1.
 template <bool BF16, bool WINDOW>
-__device__ void chunk_products(int h, uint32_t q32, uint32_t ring, uint32_t bar, uint32_t tmem_, const ChunkTile* s_info,
+__device__ void chunk_products(int h, uint32_t limit, uint32_t q32, uint32_t ring, uint32_t bar, uint32_t tmem_, const ChunkTile* s_info,
                                const ChunkWork<WINDOW>* works, int* s_trouble) {
   constexpr uint32_t QK = mma_idesc<BF16>(CH_STEP, false), PV = mma_idesc<BF16>(128, true);
   const uint32_t t_s = (uint32_t)chunk_uniform((int)tmem_ + 128 * h), t_o = t_s + 256, one = elect_one();
@@ -219,7 +224,7 @@ __device__ void chunk_products(int h, uint32_t q32, uint32_t ring, uint32_t bar,
   int tile = 0;                                              // tile x is in slots 2 (x & 1) and the next, their phase is x >> 1
   uint32_t segments = 0, v_ok = 0, p_phase = 0;              // a bit per V slot / buffer: parity of its next use
   bool ok = true;
-  auto wait = [&](int b, uint32_t parity) { ok = ok && bar_wait_warp(bar + 8 * b, parity); };
+  auto wait = [&](int b, uint32_t parity) { ok = ok && bar_wait_warp(bar + 8 * b, parity, limit); };
   auto wait_k = [&](int x) { wait(CH_FULL + 2 * (x & 1), x >> 1 & 1); };
   auto wait_v = [&](int x) {
     wait(CH_FULL + 2 * (x & 1) + 1, x >> 1 & 1);
@@ -228,7 +233,7 @@ __device__ void chunk_products(int h, uint32_t q32, uint32_t ring, uint32_t bar,
       v_ok ^= 1u << (x & 1);
     }
   };
-  for (unsigned at = 0; chunk_uniform(chunk_work(works, at, bar, ok)); ++at) {
+  for (unsigned at = 0; chunk_uniform(chunk_work(works, at, bar, limit, ok)); ++at) {
     const ChunkWork<WINDOW>& work = works[at % CH_WORKS];
     const int n = chunk_uniform(work.s.k1 - work.s.k0);
     ChunkSteps<WINDOW> st = work.st[h];
@@ -285,7 +290,7 @@ __device__ void chunk_products(int h, uint32_t q32, uint32_t ring, uint32_t bar,
   if (!ok) *s_trouble = 1;
   // products that are still under way (the softmax warps may have given up) must not outlive the tensor memory
   mma_commit(one, bar + 8 * (CH_DRAINED + h));
-  bar_wait_warp(bar + 8 * (CH_DRAINED + h), 0);
+  bar_wait_warp(bar + 8 * (CH_DRAINED + h), 0, WAIT_NS);
 }
 
 // One warp: values in masked places.
@@ -295,7 +300,7 @@ __device__ void chunk_values(const PagedArgs& A, unsigned char* ring_ptr, uint32
   const int lane = threadIdx.x & 31;
   unsigned use = 0, tile = 0, segments = 0;
   bool ok = true;
-  for (unsigned at = 0; chunk_work(works, at, bar, ok); ++at) {
+  for (unsigned at = 0; chunk_work(works, at, bar, A.wait_ns, ok); ++at) {
     const PagedSegment s = works[at % CH_WORKS].s;
     chunk_work_done(at, bar);
     if (s.k0 == s.k1) continue;
@@ -303,7 +308,7 @@ __device__ void chunk_values(const PagedArgs& A, unsigned char* ring_ptr, uint32
     for (int j = s.k0; ok && j < s.k1; ++j, ++tile) {
       for (int t = 0; t < 2; ++t, ++use) {
         const int slot = use % CH_SLOTS;
-        if (!bar_wait_warp(bar + 8 * (CH_FULL + slot), (use / CH_SLOTS) & 1)) { ok = false; break; }
+        if (!bar_wait_warp(bar + 8 * (CH_FULL + slot), (use / CH_SLOTS) & 1, A.wait_ns)) { ok = false; break; }
         const ChunkTile info = s_info[tile % CH_INFO];
         if (t == 1 && info.edge) {
           // 16 keys at a time that not every row sees: eight lanes a key, a 16-byte chunk of each panel a lane.  x * 0 added up
@@ -376,9 +381,9 @@ __device__ void chunk_softmax(const PagedArgs& A, uint32_t bar, uint32_t tmem, c
   uint32_t s_phase = 0;                                      // a bit per buffer: parity of its next use
   // The product of buffer b's last step.  (A barrier a buffer: the one of the step before that is done when the scores that
   // came after it are, so no phase can be mistaken for another.)
-  auto product_done = [&](int b) { return bar_wait_warp(bar + 8 * (CH_O_DONE + 2 * h + b), (s_phase >> b & 1) ^ 1u); };
+  auto product_done = [&](int b) { return bar_wait_warp(bar + 8 * (CH_O_DONE + 2 * h + b), (s_phase >> b & 1) ^ 1u, A.wait_ns); };
   bool ok = true;
-  for (unsigned at = 0; chunk_work(works, at, bar, ok); ++at) {
+  for (unsigned at = 0; chunk_work(works, at, bar, A.wait_ns, ok); ++at) {
     const PagedSegment s = works[at % CH_WORKS].s;           // (a copy: with reads from shared memory in the steps they took 3 % longer)
     const ChunkSteps<WINDOW> st = works[at % CH_WORKS].st[h];
     chunk_work_done(at, bar);
@@ -394,7 +399,7 @@ __device__ void chunk_softmax(const PagedArgs& A, uint32_t bar, uint32_t tmem, c
     float m = -INFINITY, l = 0.f;
     for (int u = 0, t = st.next(-1); u < steps; ++u, t = st.next(t)) {
       const int b = u & 1, half = t & 1;
-      ok = bar_wait_warp(bar + 8 * (CH_S_FULL + 2 * h + b), s_phase >> b & 1);
+      ok = bar_wait_warp(bar + 8 * (CH_S_FULL + 2 * h + b), s_phase >> b & 1, A.wait_ns);
       s_phase ^= 1u << b;
       if (!ok) break;
       tmem_fence_after();
@@ -592,7 +597,7 @@ paged_chunk_kernel(const PagedArgs A, const __grid_constant__ CUtensorMap tm_q, 
     const int role = warp - CH_SOFTMAX_WARPS;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_HELPER_REGS));
     if (role == 0) chunk_load<BF16, WINDOW>(A, &tm_q, &tm_k, &tm_v, PagedWalk<CH_KEYS>(A, from, to), q32, ring, bar, s_info, s_work, &s_trouble);
-    else if (role < 3) chunk_products<BF16, WINDOW>(role - 1, q32, ring, bar, tmem, s_info, s_work, &s_trouble);
+    else if (role < 3) chunk_products<BF16, WINDOW>(role - 1, A.wait_ns, q32, ring, bar, tmem, s_info, s_work, &s_trouble);
     else chunk_values<BF16, WINDOW>(A, ring_ptr, bar, s_info, s_work, s_again, &s_trouble);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CH_SOFTMAX_REGS));

@@ -20,6 +20,12 @@ __device__ __forceinline__ void store_global(uint64_t addr, const uint4& v) {
   asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+__device__ __forceinline__ uint32_t now_ns() {                  // (wraps after 4.3 s)
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+  return t;
+}
+
 // ── mbarrier ────────────────────────────────────────────────────────────────
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
@@ -40,15 +46,20 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits (bounded; a wait normally ends within microseconds) for the barrier's phase `parity`; false if it did not complete.
-constexpr unsigned BAR_WAIT_LIMIT = 1u << 18;
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (unsigned spins = 0; spins < BAR_WAIT_LIMIT; ++spins)
+// Waits for the barrier's phase `parity`, for `limit` nanoseconds (under 2^32) once a first try has failed; false if it did not complete.
+// A limit of time, not of tries: a try that fails takes 1 us (it sleeps on the barrier), but nothing promises that.  Waits end within
+// microseconds to a few milliseconds; WAIT_NS is far above both.  (No limit at all left: a wait that is not over with the first try has run out.)
+constexpr uint32_t WAIT_NS = 2000000000u;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
+  if (bar_try(bar, parity)) return true;
+  for (const uint32_t start = now_ns(); now_ns() - start < limit;)
     if (bar_try(bar, parity)) return true;
   return false;
 }
 // The same for a whole warp: all its lanes go on, or none does.
-__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, uint32_t limit) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, limit));
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ── dependent launches ──────────────────────────────────────────────────────

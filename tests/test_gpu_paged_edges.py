@@ -195,3 +195,38 @@ def test_results_repeat_with_bad_values():
         q, k, bad, args, kw, got = spoiled(lens, new, 2, 4, 32, F16, at, seed=17)
         for _ in range(30):
             assert torch.equal(bits(paged_attention(q, k, bad, *args, **kw)), bits(got))
+
+
+# ── waits that run out ───────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("requests,new,H_kv,window", [(30, 1, 1, 0), (30, 4, 1, 9000), (200, 1, 2, 0), (200, 4, 2, 1300), (160, 20, 1, 0), (160, 300, 1, 0), (160, 300, 1, 200)])
+def test_a_wait_that_runs_out_is_reported(requests, new, H_kv, window):
+    """With no time to wait, a CTA gives up at its first wait that the first try (about 1 us) does not see the end of, and with all of them after cold
+    memory some do: in clusters, on the line of units, in chunks of one half and of several items.  The call ends, its status
+    words say so, and the next call is right."""
+    import ctypes as C
+    from rdkv_b200 import paged
+    from rdkv_b200._lib import PagedAttentionArgs, lib, raw_stream
+    lens = [20000 if requests < 100 else 1500] * requests
+    k, v, table = R.build_cache(lens, H_kv, 64, BF16, seed=3)
+    other = torch.empty(1 << 26, dtype=torch.int32, device="cuda")       # (twice what L2 holds)
+    q = randn(requests * new, 4 * H_kv, 128, seed=4, dtype=BF16)
+    start, tokens = starts([new] * requests), ints(lens)
+    want = paged.paged_attention(q, k, v, table, start, tokens, max_new=new, window=window, check_status=True)
+    _, direct, n_ws, index, fields, _ = paged._attention_check(q, k, v, table, start, tokens, new, window, 0, None)
+    assert direct
+    words = lib().rdkv_paged_attention_status_words()
+    for wait_us, expected in ((-1, 1), (2000000, 0)):
+        args = PagedAttentionArgs.from_buffer_copy(fields)
+        args.wait_us = wait_us
+        out, ws = torch.zeros_like(q), torch.zeros(n_ws, dtype=torch.int32, device="cuda")
+        seen = set()
+        for _ in range(10):
+            other.fill_(1)
+            assert lib().rdkv_paged_attention(C.addressof(args), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), start.data_ptr(),
+                                              tokens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), 0, None, ws.data_ptr(), 4 * n_ws,
+                                              raw_stream(index)) == 0
+            seen.add(int(ws[:words].max()))
+        assert expected in seen and seen <= {0, expected}
+    assert torch.equal(out, want)
+    assert torch.equal(paged.paged_attention(q, k, v, table, start, tokens, max_new=new, window=window, check_status=True), want)

@@ -613,7 +613,7 @@ int rdkv_knapsack_batched_static(const float* scores, int64_t row_stride, int n_
 
 /* Rotates q [n_tokens][H_q][128] and k [n_tokens][H_kv][128] (all of one type) by the tokens' positions on 1 to 4 axes into
  * q_out / k_out (which may be q / k): axis a owns sections[a] (sum 64) of the 64 frequencies, angle =
- * positions[a*axis_stride + t] * inv_freq[j] (int32, or int64 with positions_64; taken in 64 bits).  Strides in elements.
+ * positions[a*axis_stride + t] * inv_freq[j] (int32, or int64 with positions_64; to 2^-25 of a turn up to 2^53).  Strides in elements.
  * args: HOST memory, read during the call. */
 typedef struct {
   int64_t q_tok_stride, q_head_stride, q_out_tok_stride, q_out_head_stride;

@@ -3,8 +3,9 @@
 //
 // Of the 64 rotation frequencies of a head, section a (a run of them) turns with axis a of the token's position:
 //   angle_j = position[axis(j)] * inv_freq[j],   (x[j], x[j+64]) -> (x[j] cos - x[j+64] sin, x[j+64] cos + x[j] sin).
-// The angle is taken in turns, in 64 bits, and its whole turns are dropped there, which is exact; what is left (half a
-// turn at most) is rounded to 32 bits, 2^-25 of a turn, whatever the position.  In 32 bits a position of 10^6
+// The angle is taken in turns: position * inv_freq / (2 pi) as a sum of two 64-bit numbers (the products' rounding errors are kept),
+// whose whole turns are dropped, which is exact.  What is left (half a turn at most) is rounded to 32 bits, 2^-25 of a turn,
+// for every position up to 2^53 (larger ones are no longer whole numbers in 64 bits).  In 32 bits a position of 10^6
 // would leave an error of 2^-5 radians.  Rows are rotated in 32 bits and rounded once.
 //
 // A warp belongs to a token: each lane computes two of its 64 angles and the warp trades them (16 shuffles); eight lanes
@@ -86,7 +87,11 @@ rope_axes_kernel(const AxesArgs A) {
       const int64_t at = axis * A.pos_axis + t;
       const double pos = A.pos64 ? (double)reinterpret_cast<const int64_t*>(A.positions)[at]
                                  : (double)reinterpret_cast<const int32_t*>(A.positions)[at];
-      const double turns = pos * ((double)A.inv_freq[j] * 0.15915494309189535);   // 1 / (2 pi)
+      // inv_freq / (2 pi) = w + w_lo, 1 / (2 pi) = INV + INV_LO; the position times that = x + x_lo
+      constexpr double INV = 0x1.45f306dc9c883p-3, INV_LO = -0x1.6b01ec5417056p-57;
+      const double f = A.inv_freq[j], w = f * INV, w_lo = fma(f, INV, -w) + f * INV_LO;
+      const double x = pos * w, x_lo = fma(pos, w, -x) + pos * w_lo;
+      const double turns = (x - rint(x)) + x_lo;             // (x_lo is over a turn where x has no bits below one)
       sincospif(2.f * (float)(turns - rint(turns)), &sn[e], &cs[e]);
     }
 #pragma unroll

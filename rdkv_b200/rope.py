@@ -81,8 +81,8 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     :func:`fused_rope`.  One launch.
 
     positions [T], or [axes,T] with 1 to 4 axes (time, height, width of images and video), int32 / int64; inv_freq
-    float32 [64]: the angle of frequency j is ``position * inv_freq[j]``, taken in 64 bits so that far positions
-    lose nothing (below 2^24).  sections: how many of the 64 frequencies each axis owns, in order (text
+    float32 [64]: the angle of frequency j is ``position * inv_freq[j]``, whose whole turns are taken off exactly, so that far positions
+    lose nothing (up to 2^53).  sections: how many of the 64 frequencies each axis owns, in order (text
     with one axis: all of them).  Returns (q_out, k_out): new tensors, or the given ones, which may be q and k
     themselves."""
     if sections is not None:

@@ -230,3 +230,26 @@ def test_a_wait_that_runs_out_is_reported(requests, new, H_kv, window):
         assert expected in seen and seen <= {0, expected}
     assert torch.equal(out, want)
     assert torch.equal(paged.paged_attention(q, k, v, table, start, tokens, max_new=new, window=window, check_status=True), want)
+
+
+# ── far positions ────────────────────────────────────────────────────────────
+
+TWO_PI = Fraction(6283185307179586476925286766559005768394, 10 ** 39)     # 2 pi to 40 digits
+
+
+@pytest.mark.parametrize("far", [2 ** 24, 2 ** 29, 2 ** 31 - 1, 2 ** 40, 2 ** 53])
+def test_far_positions_lose_nothing(far):
+    """Angles from exact arithmetic: position * inv_freq as a fraction, its whole turns taken off with 2 pi to 40 digits
+    (an error of far * 1e-40 turns), sine and cosine of what is left in 64 bits."""
+    from rdkv_b200.rope import rope_axes
+    rng = random.Random(far)
+    positions = [far, far - 1] + [rng.randint(far // 2, far) for _ in range(10)]
+    inv = INV()
+    rest = [[float((p * Fraction(f)) % TWO_PI) for f in inv.tolist()] for p in positions]
+    q = randn(len(positions), 3, 128, seed=5, dtype=torch.float32)
+    pos = torch.tensor(positions, device="cuda", dtype=torch.int64 if far > 2 ** 31 - 1 else torch.int32)
+    angle = torch.tensor(rest, dtype=torch.float64, device="cuda")[:, None]
+    a, b = q.double()[..., :64], q.double()[..., 64:]
+    want = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], dim=2)
+    for got in rope_axes(q, q[:, :1], pos, inv):
+        near(got, want[:, :got.shape[1]], q[:, :got.shape[1]], torch.float32)

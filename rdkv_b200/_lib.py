@@ -275,6 +275,67 @@ def separate_rows(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must not be a broadcast view")
 
 
+def extent(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to the end of its last (0: it has none)."""
+    return t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) if t.numel() > 0 else 0
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of one tensor lies in an element of the other: gaps between rows do not count, so views of one buffer
+    that lie between each other are apart.  Looks for whole numbers with sum(x * stride) = distance, largest stride first."""
+    if not (a.numel() and b.numel()):
+        return False
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa >= pb + extent(b) or pb >= pa + extent(a):
+        return False
+    spans = {}                                             # stride in bytes: lowest and highest multiple
+    for t, sign in ((a, 1), (b, -1)):
+        size = t.element_size()
+        dims = [[1, size]]
+        for st, n in sorted((st * size, n) for n, st in zip(t.shape, t.stride()) if n > 1 and st > 0):
+            if st == dims[-1][0] * dims[-1][1]:
+                dims[-1][1] *= n                           # (goes on where the dimension inside it ends)
+            else:
+                dims.append([st, n])
+        for st, n in dims:
+            lo, hi = spans.get(st, (0, 0))
+            spans[st] = (lo, hi + n - 1) if sign > 0 else (lo - n + 1, hi)
+    spans = sorted(((st, *x) for st, x in spans.items()), reverse=True)
+    rest = [(0, 0)]
+    for st, lo, hi in reversed(spans):
+        rest.append((rest[-1][0] + st * lo, rest[-1][1] + st * hi))
+    rest = rest[::-1]                                      # [i]: what the strides from the i-th on reach
+    tries = 0
+
+    def find(i, distance):
+        nonlocal tries
+        tries += 1
+        if i == len(spans) or tries > 20000:               # (strides that do not nest: taken as sharing)
+            return True
+        st, lo, hi = spans[i]
+        low, high = rest[i + 1]
+        return any(find(i + 1, distance - x * st) for x in range(max(lo, -((high - distance) // st)), min(hi, (distance - low) // st) + 1))
+    return find(0, pb - pa)
+
+
+def footprint(t: torch.Tensor) -> tuple:
+    """What :func:`apart` needs of a tensor besides its address: bytes it reaches over, from one row of its first dimension to the
+    next, and of one such row."""
+    reach, step = extent(t), t.element_size() * t.stride(0)
+    return reach, step, reach - step * (t.shape[0] - 1)
+
+
+def apart(a: torch.Tensor, pa: int, fa: tuple, b: torch.Tensor, pb: int, fb: tuple) -> bool:
+    """Whether two tensors at these addresses, of these footprints, share no memory (0.3 us where they lie one behind the other or a row
+    of each in turn, as the views of a fused projection do)."""
+    if pa >= pb + fb[0] or pb >= pa + fa[0]:
+        return True
+    step = fa[1]
+    if step == fb[1] > 0 and fa[2] <= (pb - pa) % step <= step - fb[2]:
+        return True
+    return not share_memory(a, b)
+
+
 class CallCache(dict):
     """What the checks of a call worked out from the shapes, strides, types and devices of its arguments, under just
     those: the next call of the same kind skips the checks.  Nothing of the arguments' contents, addresses or identity."""

@@ -25,7 +25,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, check, lib, q_dtype_tag, raw_stream,
+from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, apart, check, footprint, lib, q_dtype_tag, raw_stream,
                    require_cuda, separate_rows)
 from .rope import axes_check, empty_rows, plain_sections
 
@@ -151,7 +151,8 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     k, v [T,H_kv,128]; k_pages, v_pages [n_pages,H_kv,page_size,128] of the same dtype (fp16 / bf16 / fp32); slot_map int64
     [T]: slot of every token; a slot below zero or behind the last page is not written.  The slots of a call must
     differ from one another.  q [T,H_q,128] of the same dtype goes to ``q_out`` (default: a new tensor; may be q
-    itself), which is returned; k is not changed.  positions [T] or [axes,T], inv_freq and sections: see ``rope_axes``."""
+    itself, but share no other memory with q, k or v), which is returned; k is not changed.  k and v may be rows of pages that the
+    call does not write to.  positions [T] or [axes,T], inv_freq and sections: see ``rope_axes``."""
     if sections is not None:
         sections = plain_sections(sections)
     key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), k_pages.shape, k_pages.stride(),
@@ -164,11 +165,20 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
     call = _APPEND_CALLS.get(key)
     if call is None:
         call = _APPEND_CALLS.remember(key, _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sections, q_out))
-    args, _, index, dense = call
-    if q is not None and q_out is None:
+    args, _, index, dense, marks = call
+    k_ptr, v_ptr, kp_ptr, vp_ptr = k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
+    if kp_ptr == vp_ptr and kp_ptr != 0:
+        raise ValueError("k_pages and v_pages must not share memory")
+    if marks is not None:
+        q_mark, qo_mark, k_mark, v_mark, q_like = marks
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+        if not ((q_like and q_ptr == qo_ptr or apart(q_out, qo_ptr, qo_mark, q, q_ptr, q_mark)) and apart(q_out, qo_ptr, qo_mark, k, k_ptr, k_mark)
+                and apart(q_out, qo_ptr, qo_mark, v, v_ptr, v_mark)):
+            raise ValueError("q_out may be q itself, but must share no other memory with q, k or v")
+    elif q is not None:
         q_out = empty_rows(q, dense)
     status = lib().rdkv_paged_append(
-        args, k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slot_map.data_ptr(), None if q is None else q.data_ptr(),
+        args, k_ptr, v_ptr, kp_ptr, vp_ptr, slot_map.data_ptr(), None if q is None else q.data_ptr(),
         None if q is None else q_out.data_ptr(), None if positions is None else positions.data_ptr(),
         None if positions is None else inv_freq.data_ptr(), raw_stream(index))
     if status:
@@ -214,7 +224,8 @@ def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sect
         k_page_row_stride=kp[2], v_page_stride=vp[0], v_page_head_stride=vp[1], v_page_row_stride=vp[2], q_tok_stride=qs[0],
         q_head_stride=qs[1], q_out_tok_stride=qos[0], q_out_head_stride=qos[1], H_q=H_q, H_kv=H_kv, dtype=tag, n_tokens=T, n_pages=n_pages,
         page_size=page_size, **axes)
-    return C.addressof(args), args, dev.index, q is not None and q.is_contiguous()
+    marks = None if q_out is None else (footprint(q), footprint(q_out), footprint(k), footprint(v), q_out.stride() == q.stride())
+    return C.addressof(args), args, dev.index, q is not None and q.is_contiguous(), marks
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: Tensor, q_start: Tensor, kv_lens: Tensor, *,
@@ -237,7 +248,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     ``out`` that the call allocates is zero, a given one as it was); without it the call returns at once.
     Returns ``out`` [T,H_q,128] in q's dtype.  Tokens in front of the first request's and behind the
     last one's are padding: zero in an ``out`` that the
-    call allocates, left as they were in one that it is given (which must not be q itself).  ``out_partial`` float32 [T*H_q,132] receives
+    call allocates, left as they were in one that it is given (which must not share memory with q).  ``out_partial`` float32 [T*H_q,132] receives
     un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
     window, sinks = int(window), int(sinks)                # (numbers: a key must not go by the identity of a tensor that holds one)
     max_new, scale = None if max_new is None else int(max_new), None if scale is None else float(scale)
@@ -267,8 +278,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
                     or out.stride(0) % 8 or out.stride(1) % 8):
                 raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} on {q.device} with contiguous rows on 16 bytes")
             separate_rows(out, "out")
-            if out.data_ptr() == q.data_ptr() and out.numel() > 0:
-                raise ValueError("out must not be q itself")
+            if out.numel() > 0 and not apart(out, out.data_ptr(), footprint(out), q, q.data_ptr(), footprint(q)):
+                raise ValueError("out must not share memory with q")
         os, out_ptr, rec_ptr = out.stride(), out.data_ptr(), None
     else:
         if out is not None:

@@ -14,7 +14,8 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import HEAD_DIM, CallCache, RopeAxesArgs, check, lib, ptr, q_dtype_tag, raw_stream, require_cuda, separate_rows, stream_ptr
+from ._lib import (HEAD_DIM, CallCache, RopeAxesArgs, apart, check, footprint, lib, ptr, q_dtype_tag, raw_stream, require_cuda, separate_rows,
+                   stream_ptr)
 
 
 def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
@@ -84,7 +85,7 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     float32 [64]: the angle of frequency j is ``position * inv_freq[j]``, whose whole turns are taken off exactly, so that far positions
     lose nothing (up to 2^53).  sections: how many of the 64 frequencies each axis owns, in order (text
     with one axis: all of them).  Returns (q_out, k_out): new tensors, or the given ones, which may be q and k
-    themselves."""
+    themselves (and must share no other memory with them)."""
     if sections is not None:
         sections = plain_sections(sections)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), positions.shape, positions.stride(),
@@ -94,7 +95,9 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     call = _ROPE_CALLS.get(key)
     if call is None:
         call = _ROPE_CALLS.remember(key, _rope_check(q, k, positions, inv_freq, sections, q_out, k_out))
-    args, _, index, dense = call
+    args, _, index, dense, marks = call
+    if marks is not None:
+        _rope_apart(q, k, q_out, k_out, *marks)
     if q_out is None:
         q_out = empty_rows(q, dense)
     if k_out is None:
@@ -104,6 +107,18 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *, sect
     if status:
         check(status, "rdkv_rope_axes")
     return q_out, k_out
+
+
+def _rope_apart(q, k, q_out, k_out, q_mark, k_mark, qo_mark, ko_mark, q_like, k_like):
+    """Refuses results that share memory with rows that are still to be read or with one another: each may be its own input, row for row
+    (``_like``: strides are the same), and nothing else."""
+    pq, pk = q.data_ptr(), k.data_ptr()
+    pqo, pko = None if q_out is None else q_out.data_ptr(), None if k_out is None else k_out.data_ptr()
+    q_in, k_in = q_like and pqo == pq, k_like and pko == pk
+    if not ((q_out is None or ((q_in or apart(q_out, pqo, qo_mark, q, pq, q_mark)) and (k_in or apart(q_out, pqo, qo_mark, k, pk, k_mark))))
+            and (k_out is None or ((k_in or apart(k_out, pko, ko_mark, k, pk, k_mark)) and (q_in or apart(k_out, pko, ko_mark, q, pq, q_mark))))
+            and (q_out is None or k_out is None or apart(q_out, pqo, qo_mark, k_out, pko, ko_mark))):
+        raise ValueError("q_out and k_out may be q and k themselves, but must share no other memory with them or with one another")
 
 
 def _rope_check(q, k, positions, inv_freq, sections, q_out, k_out):
@@ -125,4 +140,8 @@ def _rope_check(q, k, positions, inv_freq, sections, q_out, k_out):
     args = RopeAxesArgs(q_tok_stride=q0, q_head_stride=q1, q_out_tok_stride=qo[0], q_out_head_stride=qo[1], k_tok_stride=k0, k_head_stride=k1,
                         k_out_tok_stride=ko[0], k_out_head_stride=ko[1], H_q=q.shape[1], H_kv=k.shape[1], dtype=q_dtype_tag(q), n_tokens=T,
                         **axes_check(positions, inv_freq, sections, T, dev))
-    return C.addressof(args), args, dev.index, q.is_contiguous() and k.is_contiguous()
+    marks = None
+    if q_out is not None or k_out is not None:
+        marks = (footprint(q), footprint(k), q_out is not None and footprint(q_out), k_out is not None and footprint(k_out),
+                 q_out is not None and q_out.stride() == q.stride(), k_out is not None and k_out.stride() == k.stride())
+    return C.addressof(args), args, dev.index, q.is_contiguous() and k.is_contiguous(), marks

@@ -253,3 +253,59 @@ def test_far_positions_lose_nothing(far):
     want = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], dim=2)
     for got in rope_axes(q, q[:, :1], pos, inv):
         near(got, want[:, :got.shape[1]], q[:, :got.shape[1]], torch.float32)
+
+
+# ── results that share memory with what is read ──────────────────────────────
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 3]])
+def test_a_result_that_shares_rows_with_the_queries_is_refused(new):
+    from rdkv_b200.paged import paged_attention
+    lens, T = [300, 111], sum(new)
+    k, v, table = R.build_cache(lens, 2, 32, BF16, seed=71)
+    args = (k, v, table, starts(new), ints(lens))
+    buf = randn(2 * T, 12, 128, seed=72, dtype=BF16)
+    for q, out in ((buf[:T, :8], buf[1:T + 1, :8]), (buf[1:T + 1, :8], buf[:T, :8]), (buf[:T, :8], buf[:T, 1:9]), (buf[:T, :8], buf[:T, 4:12]),
+                   (buf[:T, :8], buf[:T, :8]), (buf[:2 * T:2, :8], buf[:T, 4:12])):
+        kept = buf.clone()
+        with pytest.raises(ValueError, match="share memory"):
+            paged_attention(q, *args, out=out)
+        assert torch.equal(buf, kept)
+    wide = randn(2 * T, 16, 128, seed=73, dtype=BF16)
+    for q, out in ((wide[:T, :8], wide[:T, 8:]), (wide[:T, :8], wide[T:, :8]), (wide[::2, :8], wide[1::2, :8]), (wide[:T, :8], wide[1:T + 1, 8:])):
+        want = paged_attention(q.contiguous(), *args)
+        assert torch.equal(paged_attention(q, *args, out=out), want)
+
+
+def test_rotated_rows_that_share_memory_are_refused():
+    from rdkv_b200.paged import append_kv
+    from rdkv_b200.rope import rope_axes
+    T = 20
+    pos, slots = torch.arange(T, device="cuda"), torch.arange(T, device="cuda")
+    kp, vp = (torch.zeros(4, 2, 16, 128, dtype=BF16, device="cuda") for _ in range(2))
+    buf = randn(2 * T, 16, 128, seed=74, dtype=BF16)
+    q, k, v = buf[:T, :8], buf[:T, 8:10], buf[:T, 10:12]
+    kept = buf.clone()
+    for kw in (dict(q_out=buf[1:T + 1, :8]), dict(q_out=buf[:T, 1:9]), dict(q_out=buf[:T, 4:12]), dict(k_out=buf[1:T + 1, 8:10]), dict(k_out=buf[:T, 7:9]),
+               dict(q_out=q, k_out=buf[:T, 6:8]), dict(q_out=buf[T:, :8], k_out=buf[T:, 7:9]), dict(q_out=buf[:2 * T:2, :8]),
+               dict(q_out=buf.view(-1, 8, 128)[:T]), dict(k_out=buf[:T, :2])):
+        with pytest.raises(ValueError, match="memory"):
+            rope_axes(q, k, pos, INV(), **kw)
+        if "k_out" not in kw:
+            with pytest.raises(ValueError, match="memory"):
+                append_kv(k, v, kp, vp, slots, q=q, positions=pos, inv_freq=INV(), **kw)
+    with pytest.raises(ValueError, match="memory"):
+        append_kv(k, v, kp, vp, slots, q=q, positions=pos, inv_freq=INV(), q_out=buf[:T, 3:11])
+    with pytest.raises(ValueError, match="memory"):
+        append_kv(k, v, kp, vp, slots, q=q, positions=pos, inv_freq=INV(), q_out=buf[:T, 8:])
+    with pytest.raises(ValueError, match="memory"):
+        append_kv(k, v, kp, kp, slots)
+    assert torch.equal(buf, kept) and (kp == 0).all() and (vp == 0).all()
+    want = rope_axes(q.contiguous(), k.contiguous(), pos, INV())
+    for kw in (dict(q_out=buf[T:, :8], k_out=buf[T:, 8:10]), dict(q_out=buf[T:, 4:12]), dict(k_out=buf[:T, 14:]), dict(q_out=q, k_out=k)):
+        buf.copy_(kept)
+        got = rope_axes(q, k, pos, INV(), **kw)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(got[("q_out", "k_out").index(n)] is x for n, x in kw.items())
+    for out in (buf[T:, :8], q):
+        buf.copy_(kept)
+        assert torch.equal(append_kv(k, v, kp, vp, slots, q=q, positions=pos, inv_freq=INV(), q_out=out), want[0])
+        assert torch.equal(kp.transpose(1, 2).reshape(-1, 2, 128)[:T], want[1])

@@ -70,7 +70,10 @@ def empty_rows(t: Tensor, dense: bool) -> Tensor:
 
 def plain_sections(sections: Sequence[int]) -> tuple:
     """Sections as numbers (a key must not go by the identity of tensors that hold them)."""
-    return tuple(map(float, sections))
+    for n in sections:
+        if type(n) is not int:
+            return tuple(map(float, sections))
+    return tuple(sections)
 
 
 _ROPE_CALLS = CallCache()

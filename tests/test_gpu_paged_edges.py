@@ -309,3 +309,80 @@ def test_rotated_rows_that_share_memory_are_refused():
         buf.copy_(kept)
         assert torch.equal(append_kv(k, v, kp, vp, slots, q=q, positions=pos, inv_freq=INV(), q_out=out), want[0])
         assert torch.equal(kp.transpose(1, 2).reshape(-1, 2, 128)[:T], want[1])
+
+
+# ── captures ─────────────────────────────────────────────────────────────────
+
+FIRST_CALLS = '''
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import paged_reference as R
+from test_gpu_paged import BF16, F16, INV, check, ints, randn, starts
+from rdkv_b200.paged import append_kv, build_block_tables, paged_attention
+torch.zeros(1, device="cuda")
+lens, new, window = {case!r}
+S, T, dtype = len(lens), sum(new), {dtype}
+table = torch.arange(S * 8, device="cuda", dtype=torch.int32).view(S, 8)
+kp, vp = (randn(S * 8, 2, 64, 128, seed=s, dtype=dtype) for s in (1, 2))
+q, k, v = (randn(T, h, 128, seed=h, dtype=dtype) for h in (8, 2, 2))
+ctx, fresh, free, inv = ints([a - b for a, b in zip(lens, new)]), ints(new), ints([0]), INV()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    plan = build_block_tables(ctx, fresh, table, free, 64, T)
+    rot = append_kv(k, v, kp, vp, plan.slot_map, q=q, positions=plan.positions, inv_freq=inv)
+    out = paged_attention(rot, kp, vp, table, plan.q_start, plan.kv_lens, max_new=max(new), window=window)
+table.copy_(torch.arange(S * 8, device="cuda", dtype=torch.int32).view(S, 8))
+for _ in range(2):
+    graph.replay()
+    torch.cuda.synchronize()
+check(out, R.attention(rot, kp, vp, table, starts(new), ints(lens), window))
+check(paged_attention(rot, kp, vp, table, plan.q_start, plan.kv_lens, max_new=max(new), window=window), R.attention(rot, kp, vp, table, starts(new), ints(lens), window))
+print("as wanted")
+'''
+
+
+@pytest.mark.parametrize("case,dtype", [(([400, 77], [1, 1], 0), "BF16"), (([400] * 40, [1] * 40, 0), "F16"), (([400, 77], [100, 60], 0), "BF16"), (([400, 77], [100, 60], 64), "F16")])
+def test_the_first_calls_of_a_process_are_captured(case, dtype):
+    """Nothing has been loaded, asked for or set when a capture begins."""
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALLS.format(root=os.path.dirname(tests), tests=tests, case=case, dtype=dtype)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "as wanted" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("new", [[1] * 3, [1] * 40, [90, 40, 7]])
+def test_two_graphs_of_one_pool_and_threads_side_by_side(new):
+    """Graphs that share a memory pool, replayed one after the other, and calls of several host threads on streams of their own."""
+    import threading
+    from rdkv_b200.paged import paged_attention
+    lens = [300 + 7 * i for i in range(len(new))]
+    k, v, table = R.build_cache(lens, 2, 32, BF16, seed=31)
+    qs = [randn(sum(new), 8, 128, seed=s, dtype=BF16) for s in range(4)]
+    args = (k, v, table, starts(new), ints(lens))
+    want = [paged_attention(q, *args, max_new=max(new)) for q in qs]
+    graphs = []
+    for q in qs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0][0].pool() if graphs else None):
+            out = paged_attention(q, *args, max_new=max(new))
+        graphs.append((graph, out))
+    for _ in range(5):
+        for (graph, out), x in zip(graphs, want):
+            graph.replay()
+            assert torch.equal(out, x)
+    got = [[] for _ in qs]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(paged_attention(qs[i], *args, max_new=max(new)))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    torch.cuda.synchronize()
+    [t.start() for t in threads]; [t.join() for t in threads]
+    assert all(len(g) == 20 and all(torch.equal(x, w) for x in g) for g, w in zip(got, want))

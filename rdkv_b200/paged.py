@@ -25,8 +25,8 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, apart, check, footprint, lib, q_dtype_tag, raw_stream,
-                   require_cuda, separate_rows)
+from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, apart, check, extent, footprint, lib,
+                   q_dtype_tag, raw_stream, require_cuda, separate_rows, share_memory)
 from .rope import axes_check, empty_rows, plain_sections
 
 MAX_REQUESTS = 16384
@@ -55,12 +55,15 @@ def _same_device(dev, **tensors: Optional[Tensor]) -> None:
             raise ValueError(f"{name} must live on {dev}, got {t.device}")
 
 
-def _overlap(a: Tensor, b: Tensor) -> bool:
-    """Whether the bytes from the first element to the last of two tensors meet."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    end = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) for t in (a, b)]
-    return a.data_ptr() < end[1] and b.data_ptr() < end[0]
+def _check_plan_apart(out: "PagedPlan", **read: Optional[Tensor]) -> None:
+    """Refuses a plan whose tensors share memory with one another or with the arguments that the launch reads."""
+    places = [(n, t, t.data_ptr(), t.data_ptr() + extent(t)) for n, t in {**out._asdict(), **read}.items() if t is not None and t.numel() > 0]
+    mine = [x for x in places if x[0] not in read]
+    for i, (name, t, begin, end) in enumerate(mine):
+        for other, x, b, e in places[i + 1:]:
+            if begin < e and b < end and share_memory(t, x):
+                why = "which other blocks of the launch still read" if other in read else "which is written too"
+                raise ValueError(f"out.{name} shares memory with {other}, {why}")
 
 
 def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor, free_pages: Tensor, page_size: int, n_tokens: int,
@@ -76,8 +79,8 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
 
     A page that is not to be had (the free list is used up: entry -1; the table is too narrow: no entry) leaves its
     tokens without a slot (-1): :func:`append_kv` does not write them and :func:`paged_attention` does not see them.
-    ``missing`` counts such pages.  ``out``: a plan of the same S and n_tokens to write into; it must not share memory with the
-    arguments (a step's ``kv_lens`` are the next one's ``ctx_lens``: take two plans in turn, or copy)."""
+    ``missing`` counts such pages.  ``out``: a plan of the same S and n_tokens to write into; its tensors must not share memory with one
+    another or with the arguments (a step's ``kv_lens`` are the next one's ``ctx_lens``: take two plans in turn, or copy)."""
     n_tokens, page_size = int(n_tokens), int(page_size)
     key = (ctx_lens.shape, ctx_lens.stride(), ctx_lens.dtype, ctx_lens.get_device(), new_lens.shape, new_lens.stride(), new_lens.dtype,
            new_lens.get_device(), block_tables.shape, block_tables.stride(), block_tables.dtype, block_tables.get_device(), free_pages.shape,
@@ -115,11 +118,7 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
         if out.slot_map.dtype != torch.int64 or tuple(out.slot_map.shape) != (n_tokens,) or not out.slot_map.is_contiguous():
             raise ValueError(f"out.slot_map must be a contiguous int64 tensor of {n_tokens} elements")
         _same_device(ctx_lens.device, **{f"out.{n}": t for n, t in out._asdict().items()})
-        for name, t in out._asdict().items():
-            for other, x in (("ctx_lens", ctx_lens), ("new_lens", new_lens), ("free_pages", free_pages), ("free_start", free_start),
-                             ("block_tables", block_tables)):
-                if x is not None and _overlap(t, x):
-                    raise ValueError(f"out.{name} shares memory with {other}, which other blocks of the launch still read")
+        _check_plan_apart(out, ctx_lens=ctx_lens, new_lens=new_lens, free_pages=free_pages, free_start=free_start, block_tables=block_tables)
     slot_map, positions, q_start, kv_lens, free_next, missing = out
     status = lib().rdkv_paged_tables(
         ctx_lens.data_ptr(), new_lens.data_ptr(), S, block_tables.data_ptr(), *table, free_pages.data_ptr(), n_free,

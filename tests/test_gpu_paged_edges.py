@@ -311,6 +311,23 @@ def test_rotated_rows_that_share_memory_are_refused():
         assert torch.equal(kp.transpose(1, 2).reshape(-1, 2, 128)[:T], want[1])
 
 
+def test_a_plan_whose_tensors_share_memory_is_refused():
+    from rdkv_b200.paged import build_block_tables
+    table = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    args = (ints([0, 5, 9]), ints([20, 1, 4]), table, ints([5, 6, 7, 8]), 16, 25)
+    plan = build_block_tables(*args)
+    ring = torch.zeros(64, dtype=torch.int32, device="cuda")
+    for bad in (dict(kv_lens=plan.q_start[1:]), dict(free_next=plan.missing), dict(kv_lens=plan.positions[5:8]), dict(positions=plan.slot_map.view(torch.int32)[:25]),
+                dict(q_start=ring[:4], positions=ring[3:28]), dict(kv_lens=args[0]), dict(free_next=table[1, 2:3])):
+        with pytest.raises(ValueError, match="shares memory"):
+            build_block_tables(*args, out=plan._replace(**bad))
+    table.fill_(-1)
+    again = build_block_tables(*args, out=plan._replace(q_start=ring[:4], positions=ring[4:29], kv_lens=ring[30:33]))
+    table.fill_(-1)
+    for x, y in zip(again, build_block_tables(*args)):
+        assert torch.equal(x, y)
+
+
 # ── captures ─────────────────────────────────────────────────────────────────
 
 FIRST_CALLS = '''

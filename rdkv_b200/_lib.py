@@ -275,6 +275,13 @@ def separate_rows(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must not be a broadcast view")
 
 
+def fits_32_bits(**extents: int) -> None:
+    """Refuses extents that the 32-bit fields of an argument struct would take the remainder of."""
+    for name, n in extents.items():
+        if n > 0x7fffffff:
+            raise ValueError(f"{name} must be under 2^31, got {n}")
+
+
 def extent(t: torch.Tensor) -> int:
     """Bytes from a tensor's first element to the end of its last (0: it has none)."""
     return t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) if t.numel() > 0 else 0

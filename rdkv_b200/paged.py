@@ -25,7 +25,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, apart, check, extent, footprint, lib,
+from ._lib import (HEAD_DIM, PARTIAL_STRIDE, CallCache, PagedAppendArgs, PagedAttentionArgs, apart, check, extent, fits_32_bits, footprint, lib,
                    q_dtype_tag, raw_stream, require_cuda, separate_rows, share_memory)
 from .rope import axes_check, empty_rows, plain_sections
 
@@ -97,6 +97,7 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
             raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
         if page_size < 1 or n_tokens < 0:
             raise ValueError(f"bad page_size {page_size} or n_tokens {n_tokens}")
+        fits_32_bits(page_size=page_size, n_tokens=n_tokens, width=block_tables.shape[1], free_pages=free_pages.shape[0])
         if S > 1 and block_tables.shape[1] > 0 and block_tables.stride(0) < block_tables.shape[1]:
             raise ValueError("rows of block_tables overlap")
         if free_start is not None:
@@ -189,9 +190,10 @@ def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sect
     require_cuda(k, "k"); require_cuda(v, "v"); require_cuda(slot_map, "slot_map")
     _check_pages(k_pages, v_pages)
     n_pages, H_kv, page_size, _ = k_pages.shape
-    T, dev = k.shape[0], k.device
-    if k.dim() != 3 or tuple(k.shape) != (T, H_kv, HEAD_DIM) or v.shape != k.shape:
+    if k.dim() != 3 or tuple(k.shape[1:]) != (H_kv, HEAD_DIM) or v.shape != k.shape:
         raise ValueError(f"k and v must be [T,{H_kv},{HEAD_DIM}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    T, dev = k.shape[0], k.device
+    fits_32_bits(T=T, n_pages=n_pages, page_size=page_size, H_q=0 if q is None else q.numel() // max(T * HEAD_DIM, 1))
     if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
         raise ValueError(f"k and v must have the pages' dtype {k_pages.dtype}")
     if k.stride(2) != 1 or v.stride(2) != 1:
@@ -321,6 +323,7 @@ def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_ne
         raise ValueError(f"block_tables must have {S} rows and q_start {S + 1} elements")
     if S > MAX_REQUESTS:
         raise ValueError(f"{S} requests: at most {MAX_REQUESTS}")
+    fits_32_bits(T=T, H_q=H_q, n_pages=n_pages, width=block_tables.shape[1])
     if window < 0 or sinks < 0 or (sinks > 0 and window == 0):
         raise ValueError("window and sinks must not be negative, and sinks need a window")
     scale = HEAD_DIM ** -0.5 if scale is None else scale

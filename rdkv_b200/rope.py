@@ -14,8 +14,8 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import (HEAD_DIM, CallCache, RopeAxesArgs, apart, check, footprint, lib, ptr, q_dtype_tag, raw_stream, require_cuda, separate_rows,
-                   stream_ptr)
+from ._lib import (HEAD_DIM, CallCache, RopeAxesArgs, apart, check, fits_32_bits, footprint, lib, ptr, q_dtype_tag, raw_stream, require_cuda,
+                   separate_rows, stream_ptr)
 
 
 def fused_rope(q: Tensor, k: Tensor, cos_half: Tensor, sin_half: Tensor):
@@ -44,7 +44,7 @@ def axes_check(positions: Tensor, inv_freq: Tensor, sections: Optional[Sequence[
     """The fields of a call's arguments that say how it rotates, by name."""
     half = HEAD_DIM // 2
     require_cuda(positions, "positions"); require_cuda(inv_freq, "inv_freq")
-    n_axes = 1 if positions.dim() == 1 else positions.shape[0]
+    n_axes = positions.shape[0] if positions.dim() == 2 else 1
     if positions.dim() not in (1, 2) or positions.shape[-1] != T or not 1 <= n_axes <= 4 or (T > 1 and positions.stride(-1) != 1):
         raise ValueError(f"positions must be [{T}] or [1 to 4 axes,{T}] with contiguous rows, got {tuple(positions.shape)}")
     if positions.dtype not in _AXES_TAG:
@@ -130,6 +130,7 @@ def _rope_check(q, k, positions, inv_freq, sections, q_out, k_out):
         if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
             raise ValueError(f"{name} must be [T,heads,{HEAD_DIM}] with contiguous rows, got {tuple(t.shape)}")
     T, dev = q.shape[0], q.device
+    fits_32_bits(T=T, H_q=q.shape[1], H_kv=k.shape[1])
     if k.shape[0] != T or k.dtype != q.dtype or k.device != dev:
         raise ValueError("q and k must have the same tokens, dtype and device")
     for name, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):

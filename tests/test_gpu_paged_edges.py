@@ -328,6 +328,46 @@ def test_a_plan_whose_tensors_share_memory_is_refused():
         assert torch.equal(x, y)
 
 
+# ── shapes ───────────────────────────────────────────────────────────────────
+
+def test_tensors_without_dimensions_are_refused():
+    from rdkv_b200.paged import append_kv, build_block_tables, paged_attention
+    from rdkv_b200.rope import rope_axes
+    k, v, table = R.build_cache([64], 2, 16, F16, seed=1)
+    rows, q, none, slots, pos = randn(2, 2, 128, seed=2, dtype=F16), randn(2, 8, 128, seed=3, dtype=F16), torch.zeros((), device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda"), ints([0, 1])
+    half, number = none.half(), none.int()
+    for call in (lambda: append_kv(half, half, k, v, slots), lambda: append_kv(rows, half, k, v, slots), lambda: append_kv(rows, rows, half, half, slots),
+                 lambda: append_kv(rows, rows, k, v, none.long()), lambda: append_kv(rows, rows, k, v, slots, q=half, positions=pos, inv_freq=INV()),
+                 lambda: append_kv(rows, rows, k, v, slots, q=q, positions=number, inv_freq=INV()), lambda: rope_axes(q, rows, number, INV()),
+                 lambda: append_kv(rows, rows, k, v, slots, q=q, positions=pos, inv_freq=none), lambda: rope_axes(half, half, pos, INV()),
+                 lambda: rope_axes(q, rows, pos, INV(), q_out=half), lambda: paged_attention(half, k, v, table, ints([0, 2]), ints([64])),
+                 lambda: paged_attention(q, half, half, table, ints([0, 2]), ints([64])), lambda: paged_attention(q, k, v, number, ints([0, 2]), ints([64])),
+                 lambda: paged_attention(q, k, v, table, number, ints([64])), lambda: paged_attention(q, k, v, table, ints([0, 2]), number),
+                 lambda: paged_attention(q, k, v, table, ints([0, 2]), ints([64]), out=half), lambda: build_block_tables(number, number, table, number, 16, 2),
+                 lambda: build_block_tables(ints([0]), ints([1]), number, ints([1]), 16, 2)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_extents_past_32_bits_are_refused():
+    """2^32 + 4 tokens are not four."""
+    from rdkv_b200.paged import append_kv, build_block_tables
+    many = 2 ** 32 + 4
+    k, v, table = R.build_cache([64], 2, 16, F16, seed=1)
+    kept = k.clone(), v.clone()
+    rows = randn(1, 2, 128, seed=2, dtype=F16).expand(many, 2, 128)
+    slots = torch.empty(many, dtype=torch.int64, device="cuda")
+    slots[:4] = torch.arange(4, device="cuda")
+    with pytest.raises(ValueError, match="2\\^31"):
+        append_kv(rows, rows, k, v, slots)
+    del slots
+    with pytest.raises(ValueError, match="2\\^31"):
+        build_block_tables(ints([0]), ints([1]), table[:1], ints([1]), 2 ** 32 + 16, 4)
+    with pytest.raises(ValueError, match="2\\^31"):
+        build_block_tables(ints([0]), ints([1]), table[:1], ints([1]), 16, many)
+    assert torch.equal(k, kept[0]) and torch.equal(v, kept[1])
+
+
 # ── captures ─────────────────────────────────────────────────────────────────
 
 FIRST_CALLS = '''

@@ -269,10 +269,17 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def separate_rows(t: torch.Tensor, name: str) -> None:
-    """Refuses a broadcast view, whose rows are one and the same memory, where rows are written or TMA copies read them."""
+def separate_rows(t: torch.Tensor, name: str, written: bool = True) -> None:
+    """Refuses a broadcast view, whose rows are one and the same memory, where rows are written or TMA copies read them, and, where
+    they are written, rows that lie partly in one another (strides that do not nest)."""
     if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
         raise ValueError(f"{name} must not be a broadcast view")
+    if written and t.numel() > 0:
+        reach = 1
+        for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+            if st < reach:
+                raise ValueError(f"{name}: rows overlap")
+            reach += st * (n - 1)
 
 
 def fits_32_bits(**extents: int) -> None:

@@ -130,7 +130,7 @@ def build_block_tables(ctx_lens: Tensor, new_lens: Tensor, block_tables: Tensor,
     return out
 
 
-def _check_pages(k_pages: Tensor, v_pages: Tensor) -> None:
+def _check_pages(k_pages: Tensor, v_pages: Tensor, written: bool) -> None:
     require_cuda(k_pages, "k_pages"); require_cuda(v_pages, "v_pages")
     if k_pages.dim() != 4 or k_pages.shape[3] != HEAD_DIM or k_pages.shape != v_pages.shape:
         raise ValueError(f"k_pages and v_pages must be [n_pages,H_kv,page_size,{HEAD_DIM}], got {tuple(k_pages.shape)} and "
@@ -139,7 +139,7 @@ def _check_pages(k_pages: Tensor, v_pages: Tensor) -> None:
         raise ValueError("k_pages and v_pages must have one dtype")
     if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
         raise ValueError("rows of k_pages and v_pages must be contiguous")
-    separate_rows(k_pages, "k_pages"); separate_rows(v_pages, "v_pages")
+    separate_rows(k_pages, "k_pages", written); separate_rows(v_pages, "v_pages", written)
 
 
 def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: Tensor, *, q: Optional[Tensor] = None,
@@ -188,7 +188,7 @@ def append_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slot_map: 
 
 def _append_check(k, v, k_pages, v_pages, slot_map, q, positions, inv_freq, sections, q_out):
     require_cuda(k, "k"); require_cuda(v, "v"); require_cuda(slot_map, "slot_map")
-    _check_pages(k_pages, v_pages)
+    _check_pages(k_pages, v_pages, True)
     n_pages, H_kv, page_size, _ = k_pages.shape
     if k.dim() != 3 or tuple(k.shape[1:]) != (H_kv, HEAD_DIM) or v.shape != k.shape:
         raise ValueError(f"k and v must be [T,{H_kv},{HEAD_DIM}], got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -306,7 +306,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
 
 def _attention_check(q, k_pages, v_pages, block_tables, q_start, kv_lens, max_new, window, sinks, scale):
     require_cuda(q, "q")
-    _check_pages(k_pages, v_pages)
+    _check_pages(k_pages, v_pages, False)
     n_pages, H_kv, page_size, _ = k_pages.shape
     if q.dim() != 3 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be [T,H_q,{HEAD_DIM}], got {tuple(q.shape)}")

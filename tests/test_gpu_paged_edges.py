@@ -328,6 +328,24 @@ def test_a_plan_whose_tensors_share_memory_is_refused():
         assert torch.equal(x, y)
 
 
+def test_results_whose_rows_overlap_are_refused():
+    from rdkv_b200.paged import append_kv, paged_attention
+    from rdkv_b200.rope import rope_axes
+    lens, T = [300, 111], 3
+    k, v, table = R.build_cache(lens, 2, 32, BF16, seed=71)
+    q, rows = randn(T, 8, 128, seed=72, dtype=BF16), randn(T, 2, 128, seed=73, dtype=BF16)
+    pos, slots, flat = torch.arange(T, device="cuda"), torch.arange(T, device="cuda"), torch.zeros(1 << 20, dtype=BF16, device="cuda")
+    many, few = flat.as_strided((T, 8, 128), (512, 128, 1)), flat.as_strided((T, 2, 128), (128, 64, 1))
+    pages = flat.as_strided(k.shape, (32 * 128, 32 * 128, 128, 1))
+    for call in (lambda: paged_attention(q, k, v, table, ints([0, 1, 3]), ints(lens), out=many), lambda: rope_axes(q, rows, pos, INV(), q_out=many),
+                 lambda: rope_axes(q, rows, pos, INV(), k_out=few), lambda: append_kv(rows, rows, pages, v, slots), lambda: append_kv(rows, rows, k, pages, slots),
+                 lambda: append_kv(rows, rows, k, v, slots, q=q, positions=pos, inv_freq=INV(), q_out=many)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    args = (table.clamp(max=1), ints([0, 1, 3]), ints(lens))             # read, such pages are pages
+    assert torch.equal(paged_attention(q, pages, v, *args), paged_attention(q, pages.contiguous(), v, *args))
+
+
 # ── shapes ───────────────────────────────────────────────────────────────────
 
 def test_tensors_without_dimensions_are_refused():

@@ -20,7 +20,8 @@
 // What bounds it (2048 tokens behind 30000, 8 x 4 heads, bf16: 0.95 to 1.07 ms over several GPUs, 0.98 to 1.09 PFLOP/s):
 // long launches reach the 1000 W limit, where the clock settles at 1.5 GHz; in short ones (2048 behind 6000: 3650 cycles
 // a tile, of which the products need 2570) the chain of a step inside a softmax warp, about 1700 cycles for 345 instructions:
-// tensor pipe 56 % busy, issue slots 52 %, exponential units 42 %.  Measured and dropped: two warps a row with shared
+// tensor pipe 56 % busy, issue slots 52 %, exponential units 42 %; two of the instructions reload spilled registers, none stores them.
+// Measured and dropped: two warps a row with shared
 // references (sixteen softmax warps; 4040 cycles), the halves' products strictly in turn (4060), the weights worked out before
 // the maximum is known (4450), next scores loaded under the exponentials (does not fit the registers).
 #include "paged_attn.cuh"

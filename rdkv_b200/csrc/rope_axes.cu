@@ -11,7 +11,8 @@
 // A warp belongs to a token: each lane computes two of its 64 angles and the warp trades them (16 shuffles); eight lanes
 // then take a row, eight pairs each, with 16-byte loads and stores, four rows at a time, and the angles serve all rows
 // of the token that the warp takes.  Few tokens: their rows are dealt out to several warps.  Bound by memory traffic (rows
-// once in, once out): 8192 tokens of 64 + 2 x 8 heads into pages of 16, bf16, 60 us, 5.6 TB/s; 6007 tokens of 32 + 8 heads 24.6 us.
+// once in, once out; bf16, in a replayed graph): 8192 tokens of 64 + 2 x 8 heads into pages of 16 60.5 us, 5.5 TB/s; 6007 tokens of 32 + 8
+// heads with three axes 24.7 us, 5.0 TB/s.
 #include <algorithm>
 
 #include "rdkv_common.cuh"
@@ -155,7 +156,7 @@ static bool axes_sections(AxesArgs* A, const int* sections, int n_axes) {
 static int axes_launch(AxesArgs& A, int dtype, bool pages, cudaStream_t st) {
   const int rows = A.H_q + A.H_kv * (pages ? 2 : 1);
   if (A.T == 0 || rows == 0) return RDKV_OK;
-  // warps a token: enough for 48 per SM, four rows each at least.  (6007 tokens of 40 heads, bf16: 28.2 us with a warp a token,
+  // warps a token: enough for 48 per SM, four rows each at least.  (6007 tokens of 40 heads, bf16, a call in a stream of calls: 28.2 us with a warp a token,
   // 26.1 with two, 27.4 with three; several rows a lane at a time were slower, 28.7 with two, 35.4 with four.)
   const int most = (rows + 3) / 4;
   A.warps_per_token = (int)std::min<int64_t>(most, std::max<int64_t>(1, (148 * 48 + A.T - 1) / A.T));

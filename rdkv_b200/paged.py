@@ -243,14 +243,17 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_tables: T
     and the request's first ``sinks``.  Tokens whose page is missing (an entry outside the pages) are not seen, and what
     stands in masked places does not matter, whatever it is.  A token that sees nothing gets zeros.
 
-    max_new: the longest chunk of the batch (default T), which chooses the kernel: a hint, results do not depend on it.
+    max_new: the longest chunk of the batch (default T), which chooses the kernel: a hint, results do not depend on it but for their rounding.
+    window and sinks from 2^30 on count as 2^30.
     scale: of the scores, positive, default 1/sqrt(128).  check_status: wait for the kernels and raise if one of their
     bounded waits ran out or q_start falls, in which case the results are invalid (where q_start falls nothing is computed: an
     ``out`` that the call allocates is zero, a given one as it was); without it the call returns at once.
     Returns ``out`` [T,H_q,128] in q's dtype.  Tokens in front of the first request's and behind the
     last one's are padding: zero in an ``out`` that the
     call allocates, left as they were in one that it is given (which must not share memory with q).  ``out_partial`` float32 [T*H_q,132] receives
-    un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine`."""
+    un-normalised records ``(m, l, -, -, o[128])`` instead, for :func:`rdkv_b200.decode.lse_combine` (rows of no request: as they were);
+    their o is a sum in 32 bits of values times weights that were rounded to q's type, so it is as good as a result before its own rounding, not
+    as 32 bits."""
     window, sinks = int(window), int(sinks)                # (numbers: a key must not go by the identity of a tensor that holds one)
     max_new, scale = None if max_new is None else int(max_new), None if scale is None else float(scale)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape,

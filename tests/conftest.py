@@ -15,6 +15,17 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run with -m gpu on a B200)")
 
 
+# Expects the positions of query rows that the definition contradicts: row t of request i stands at kv_lens[i] - (q_start[i+1] - t), also where
+# q_start goes past the query tensor (tests/test_gpu_paged_edges.py::test_starts_behind_the_last_row_keep_positions).  Its starts
+# [0, 0, 300] over 203 rows go to the reference as [0, 0, 203], which puts row 0 at 333 - 203 instead of 333 - 300.  It runs
+# last, so that a run that ends with its first failure has run all others.
+KNOWN_WRONG = "test_rows_in_front_and_starts_outside[start1-"
+
+
+def pytest_collection_modifyitems(items):
+    items.sort(key=lambda item: item.name.startswith(KNOWN_WRONG))
+
+
 def load_golden(name):
     with np.load(os.path.join(GOLDEN, name), allow_pickle=False) as z:
         return {k: z[k] for k in z.files}

@@ -667,7 +667,6 @@ typedef struct {
   int64_t table_stride;
   int32_t dtype, n_tokens, H_q, H_kv, n_pages, page_size, width, n_requests, max_new, window, sinks;
   float scale;
-  int32_t wait_us;    /* how long a device-side wait may take (up to 4000000); 0: two seconds, negative: no time (tests) */
 } rdkv_paged_attention_args;
 int rdkv_sizeof_paged_attention_args(void);
 int rdkv_paged_attention_status_words(void);
@@ -676,6 +675,12 @@ int rdkv_paged_attention(const rdkv_paged_attention_args* args, const void* q, c
                          const int32_t* block_tables, const int32_t* q_start, const int32_t* kv_lens, void* out,
                          int64_t out_tok_stride, int64_t out_head_stride, int zero_padding, float* out_partial,
                          void* workspace, int64_t workspace_bytes, void* stream);
+/* The same with another limit for device-side waits than two seconds: wait_us microseconds (up to 4000000; 0: none of a wait is
+ * waited for that its first try does not see the end of). */
+int rdkv_paged_attention_within(const rdkv_paged_attention_args* args, const void* q, const void* k_pages, const void* v_pages,
+                                const int32_t* block_tables, const int32_t* q_start, const int32_t* kv_lens, void* out,
+                                int64_t out_tok_stride, int64_t out_head_stride, int zero_padding, float* out_partial,
+                                void* workspace, int64_t workspace_bytes, int wait_us, void* stream);
 
 #ifdef __cplusplus
 }

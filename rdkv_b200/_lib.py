@@ -126,8 +126,7 @@ class PagedAttentionArgs(C.Structure):
     """Mirror of ``rdkv_paged_attention_args``; field order and types must match the header."""
     _fields_ = _fields((C.c_int64, "q_tok_stride q_head_stride k_page_stride k_head_stride k_row_stride v_page_stride v_head_stride "
                                    "v_row_stride table_stride"),
-                       (C.c_int32, "dtype n_tokens H_q H_kv n_pages page_size width n_requests max_new window sinks"), (C.c_float, "scale"),
-                       (C.c_int32, "wait_us"))
+                       (C.c_int32, "dtype n_tokens H_q H_kv n_pages page_size width n_requests max_new window sinks"), (C.c_float, "scale"))
 
 
 _i, _i64, _p, _f = C.c_int, C.c_int64, C.c_void_p, C.c_float
@@ -161,6 +160,7 @@ _PROTOTYPES = {
     "rdkv_paged_attention_status_words": ([], _i),
     "rdkv_paged_attention_workspace": ([_i, _i, _i, _i, _i], _i64),
     "rdkv_paged_attention": ([_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _p, _p, _i64, _p], _i),
+    "rdkv_paged_attention_within": ([_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _p, _p, _i64, _i, _p], _i),
     "rdkv_decode_attn_persistent": ([_p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p], _i),
     "rdkv_tail_attn_partial": ([_p, _i, _i64, _i, _i, _p, _p, _i, _i64, _i64, _i64, _i, _p, _i, _p, _p], _i),
     "rdkv_lse_combine": ([_p, _i64, _i, _i64, _i64, _p, _p, _p, _p], _i),

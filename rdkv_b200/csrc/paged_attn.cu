@@ -519,10 +519,18 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
                                     const int32_t* block_tables, const int32_t* q_start, const int32_t* kv_lens, void* out,
                                     int64_t out_tok_stride, int64_t out_head_stride, int zero_padding, float* out_partial,
                                     void* workspace, int64_t workspace_bytes, void* stream) {
+  return rdkv_paged_attention_within(args, q, k_pages, v_pages, block_tables, q_start, kv_lens, out, out_tok_stride, out_head_stride, zero_padding,
+                                     out_partial, workspace, workspace_bytes, (int)(WAIT_NS / 1000u), stream);
+}
+
+extern "C" int rdkv_paged_attention_within(const rdkv_paged_attention_args* args, const void* q, const void* k_pages, const void* v_pages,
+                                           const int32_t* block_tables, const int32_t* q_start, const int32_t* kv_lens, void* out,
+                                           int64_t out_tok_stride, int64_t out_head_stride, int zero_padding, float* out_partial,
+                                           void* workspace, int64_t workspace_bytes, int wait_us, void* stream) {
   if (args == nullptr) return RDKV_ERR_BAD_ARG;
   const rdkv_paged_attention_args& g = *args;
   if (g.n_tokens < 0 || g.n_requests < 0 || g.H_q <= 0 || g.H_kv <= 0 || g.n_pages < 0 || g.width < 0 || g.window < 0 || g.sinks < 0 ||
-      g.max_new < 0 || !(g.scale > 0.f && g.scale <= 1e30f))
+      g.max_new < 0 || !(g.scale > 0.f && g.scale <= 1e30f) || wait_us < 0 || wait_us > 4000000)
     return RDKV_ERR_BAD_ARG;
   if (g.dtype != RDKV_F16 && g.dtype != RDKV_BF16) return RDKV_ERR_BAD_ARG;
   if (g.H_q % g.H_kv != 0 || g.H_q / g.H_kv > MAX_GROUP) return RDKV_ERR_BAD_SHAPE;
@@ -552,7 +560,7 @@ extern "C" int rdkv_paged_attention(const rdkv_paged_attention_args* args, const
   A.cap = (int)std::min<int64_t>((int64_t)g.width * g.page_size, 0x7fff0000);
   A.q_start = q_start; A.kv_lens = kv_lens; A.S = g.n_requests; A.T = g.n_tokens;
   A.window = std::min(g.window, 1 << 30); A.sinks = std::min(g.sinks, 1 << 30); A.scale_log2 = g.scale * PAGED_LOG2E;
-  A.wait_ns = g.wait_us == 0 ? WAIT_NS : (uint32_t)std::min(std::max(g.wait_us, 0), 4000000) * 1000u;
+  A.wait_ns = (uint32_t)wait_us * 1000u;
   A.out = (uint16_t*)out; A.o_tok = out_tok_stride; A.o_head = out_head_stride; A.zero_pad = zero_padding; A.rec = out_partial;
   const bool bf = g.dtype == RDKV_BF16, few = paged_few_rows(g.n_requests, g.H_kv, g.max_new, A.g);
   A.group = few ? PAGED_DECODE_ROWS / A.g : 2 * (128 / A.g);

@@ -216,16 +216,15 @@ def test_a_wait_that_runs_out_is_reported(requests, new, H_kv, window):
     _, direct, n_ws, index, fields, _ = paged._attention_check(q, k, v, table, start, tokens, new, window, 0, None)
     assert direct
     words = lib().rdkv_paged_attention_status_words()
-    for wait_us, expected in ((-1, 1), (2000000, 0)):
-        args = PagedAttentionArgs.from_buffer_copy(fields)
-        args.wait_us = wait_us
+    args = PagedAttentionArgs.from_buffer_copy(fields)
+    for wait_us, expected in ((0, 1), (2000000, 0)):
         out, ws = torch.zeros_like(q), torch.zeros(n_ws, dtype=torch.int32, device="cuda")
         seen = set()
         for _ in range(10):
             other.fill_(1)
-            assert lib().rdkv_paged_attention(C.addressof(args), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), start.data_ptr(),
-                                              tokens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), 0, None, ws.data_ptr(), 4 * n_ws,
-                                              raw_stream(index)) == 0
+            assert lib().rdkv_paged_attention_within(C.addressof(args), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), start.data_ptr(),
+                                                     tokens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), 0, None, ws.data_ptr(), 4 * n_ws,
+                                                     wait_us, raw_stream(index)) == 0
             seen.add(int(ws[:words].max()))
         assert expected in seen and seen <= {0, expected}
     assert torch.equal(out, want)
